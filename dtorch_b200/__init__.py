@@ -6,6 +6,8 @@
 * ``DeviceMesh``, ``Shard``, ``Replicate``, ``Partial``, ``init_device_mesh``, ``DTensor`` (``redistribute``):
   the reference's Python API over the C++ host layer (``_host``: ThreadGroup, kernel-stream threads,
   redistribute executor).
+* ``QuantizedKVCache`` and ``kv_cache_append`` / ``kv_cache_read`` / ``kv_cache_attention`` / ``kv_cache_evict``: keys
+  and values of decoder attention in 8 bits, and the attention that reads them.
 """
 
 __version__ = "0.1.0"
@@ -14,12 +16,20 @@ _DTENSOR_NAMES = ("DeviceMesh", "Placement", "Shard", "Replicate", "Partial", "i
                   "get_placements_from_dict",
                   "cuda_device_of", "clear", "redistribute_many", "reduce", "set_pool_bytes")
 
+_KV_CACHE_NAMES = ("QuantizedKVCache", "kv_cache_append", "kv_cache_read", "kv_cache_attention", "kv_cache_evict")
+
 
 def __getattr__(name):
     if name in _DTENSOR_NAMES:
         from . import dtensor
 
         return getattr(dtensor, name)
+    if name in _KV_CACHE_NAMES:
+        from . import kv_cache
+
+        # bound in the package, so that the next use is a plain lookup
+        globals().update({k: getattr(kv_cache, k) for k in _KV_CACHE_NAMES})
+        return globals()[name]
     if name == "scaled_dot_product_attention_with_cp":
         from . import context_parallel
 

@@ -38,22 +38,33 @@ def _newer(target: str, sources) -> bool:
     return any(os.path.getmtime(s) > t for s in sources)
 
 
+CAPI_SRCS = ["dt_comm.cu", "dt_kv.cu"]
+
+
 def build_capi(force: bool = False, verbose: bool = False) -> str:
     os.makedirs(LIBDIR, exist_ok=True)
     out = os.path.join(LIBDIR, "libdtorch_b200.so")
     srcs = [os.path.join(CSRC, f) for f in sorted(os.listdir(CSRC)) if f.endswith((".cu", ".cuh", ".h"))]
     srcs.append(os.path.join(ROOT, "include", "dtorch_b200.h"))
     if force or _newer(out, srcs):
-        cmd = [nvcc(), *NVCC_FLAGS, *ARCH, "-shared", "-cudart", "static", "-o", out + ".tmp",
-               os.path.join(CSRC, "dt_comm.cu")]
-        if verbose:
-            print(" ".join(cmd), flush=True)
-        subprocess.run(cmd, check=True)
+        objdir = os.path.join(HERE, "_build")
+        os.makedirs(objdir, exist_ok=True)
+        objs, procs = [], []
+        for f in CAPI_SRCS:
+            obj = os.path.join(objdir, f.replace(".cu", ".cu.o"))
+            objs.append(obj)
+            cmd = [nvcc(), *NVCC_FLAGS, *ARCH, "-c", "-o", obj, os.path.join(CSRC, f)]
+            if verbose:
+                print(" ".join(cmd), flush=True)
+            procs.append(subprocess.Popen(cmd))
+        if any([p.wait() != 0 for p in procs]):
+            raise RuntimeError("C ABI library compile failed")
+        subprocess.run([nvcc(), *ARCH, "-shared", "-cudart", "static", "-o", out + ".tmp", *objs], check=True)
         os.replace(out + ".tmp", out)
     return out
 
 
-HOST_SRCS = ["placement.cpp", "sym_pool.cpp", "thread_group.cpp", "redistribute.cpp", "bindings.cpp"]
+HOST_SRCS = ["placement.cpp", "sym_pool.cpp", "thread_group.cpp", "redistribute.cpp", "kv_cache.cpp", "bindings.cpp"]
 
 
 def build_host(force: bool = False, verbose: bool = False) -> str:

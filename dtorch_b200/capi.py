@@ -32,6 +32,10 @@ DT_ALGO_TWOSHOT = 0x20
 DT_ALGO_NVLS = 0x40
 DT_ALGO_NCCL = 0x80
 
+DT_KV_INT8, DT_KV_E4M3 = 0, 1
+DT_KV_CAUSAL = 0x1
+DT_KV_ACCUMULATE = 0x2
+
 MAX_RANKS = 8
 
 # (name, restype, argtypes) of every exported entry point; the CPU test suite checks this list against the
@@ -79,7 +83,20 @@ SIGNATURES = [
     ("dt_all_gather_list", _I, [_P, _I, _P, _SZ, _P, _P, _P]),
     ("dt_all_gather_sub_split", _I, [_P, _I, _P, _P, _SZ, _P, _P, _SZ, _P]),
     ("dt_peer_copy", _I, [_P, _I, _P, _I, _SZ, _P]),
+    ("dt_kv_append", _I, [_P, _P, _P, _I64, _P, _P, _I, _P, _P, _P]),
+    ("dt_kv_read", _I, [_P, _P, _P, _I64, _I64, _P, _P, _I, _P]),
+    ("dt_kv_attention_workspace", _I, [_P, _I64, _I64, _I, _P]),
+    ("dt_kv_attention", _I, [_P, _P, _I64, _I64, _P, _I, _P, _P, ctypes.c_float, _I, _P, _P, _P, _P, _SZ, _P]),
+    ("dt_kv_evict_workspace", _I, [_P, _I64, _P]),
+    ("dt_kv_evict", _I, [_P, _P, _P, _P, _I64, _I64, _P, _P, _P, _P, _SZ, _P]),
 ]
+
+
+class KvCache(ctypes.Structure):
+    """dt_kv_cache: an 8-bit key/value cache by its device pointers and sizes."""
+
+    _fields_ = [("key", _P), ("value", _P), ("key_scale", _P), ("value_scale", _P), ("batch", _I64),
+                ("kv_heads", _I64), ("capacity", _I64), ("head_dim", _I64), ("block", _I64), ("code", _I)]
 
 
 class DtError(RuntimeError):
@@ -319,3 +336,40 @@ def local_all_gather(ins, out, outer, lens, inner_bytes, stream=0):
 def local_all_to_all(ins, outs, in_shape, src_dim, dst_dim, src_lens, elem_bytes, stream=0):
     check(lib().dt_local_all_to_all(len(ins), ptr_array(ins), ptr_array(outs), len(in_shape), i64_array(in_shape),
                                     src_dim, dst_dim, i64_array(src_lens), elem_bytes, stream), "dt_local_all_to_all")
+
+
+# ---- 8-bit key/value cache ----
+def kv_append(cache, key, value, tokens, key_strides, value_strides, dtype, lengths, counts=None, stream=0):
+    check(lib().dt_kv_append(ctypes.byref(cache), key, value, tokens, i64_array(key_strides), i64_array(value_strides),
+                             dtype, lengths, counts, stream), "dt_kv_append")
+
+
+def kv_read(cache, lengths, first, first_all, count, key, value, dtype, stream=0):
+    check(lib().dt_kv_read(ctypes.byref(cache), lengths, first, first_all, count, key, value, dtype, stream),
+          "dt_kv_read")
+
+
+def kv_attention_workspace(cache, query_heads, tokens, with_weights=False) -> int:
+    n = ctypes.c_size_t()
+    check(lib().dt_kv_attention_workspace(ctypes.byref(cache), query_heads, tokens, int(with_weights), ctypes.byref(n)),
+          "dt_kv_attention_workspace")
+    return n.value
+
+
+def kv_attention(cache, query, query_heads, tokens, query_strides, dtype, lengths, counts, scale, flags, out, lse, weights,
+                 workspace, workspace_bytes, stream=0):
+    check(lib().dt_kv_attention(ctypes.byref(cache), query, query_heads, tokens, i64_array(query_strides), dtype, lengths,
+                                counts, scale, flags, out, lse, weights, workspace, workspace_bytes, stream),
+          "dt_kv_attention")
+
+
+def kv_evict_workspace(cache, budget) -> int:
+    n = ctypes.c_size_t()
+    check(lib().dt_kv_evict_workspace(ctypes.byref(cache), budget, ctypes.byref(n)), "dt_kv_evict_workspace")
+    return n.value
+
+
+def kv_evict(src, dst, lengths, weights, budget, recent, dst_lengths, dst_weights, kept, workspace, workspace_bytes,
+             stream=0):
+    check(lib().dt_kv_evict(ctypes.byref(src), ctypes.byref(dst), lengths, weights, budget, recent, dst_lengths,
+                            dst_weights, kept, workspace, workspace_bytes, stream), "dt_kv_evict")

@@ -29,6 +29,7 @@
 #include <nccl.h>  // types only: the functions are looked up at run time (nccl_api)
 
 #include "../../include/dtorch_b200.h"
+#include "dt_internal.h"
 #include "dt_kernels.cuh"
 
 using namespace dtb;
@@ -2275,6 +2276,14 @@ int dt_local_all_to_all(int n, const void* const* ins, void* const* outs, int nd
 }
 
 }  // extern "C"
+
+namespace dtb {
+
+int set_error(int status, const std::string& msg) { return fail(status, msg); }
+int check_launch(const char* what) { return launch_check(what); }
+int current_device(int* dev, int* sms) { return current_device_sms(dev, sms); }
+
+}  // namespace dtb
 
 // =============================================================================================================
 // Host-partials all-reduce that allocates nothing on the device

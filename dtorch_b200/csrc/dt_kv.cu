@@ -1,0 +1,1420 @@
+// The 8-bit key/value cache of include/dtorch_b200.h: append, read, attention of few query rows, eviction, and the host
+// entry points.
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "dt_internal.h"
+#include "dt_kv.cuh"
+
+using namespace dtb;
+
+namespace {
+
+// ---------------------------------------------------------------------------------------------------------------
+// Quantisation
+// ---------------------------------------------------------------------------------------------------------------
+constexpr float kNan = __builtin_nanf("");
+
+// amax / limit, up to the next bfloat16. amax has at most 15 significant bits, so unless the quotient is a bfloat16
+// itself it is much further from one than fp32's rounding of it: the result is that of the exact quotient.
+template <bool E4M3>
+__device__ __forceinline__ float scale_of(float amax) {
+    const float s = amax / (E4M3 ? 448.0f : 127.0f);
+    return __uint_as_float((__float_as_uint(s) + 0xffffu) & 0xffff0000u);
+}
+
+// Codes of four values. The scale has 8 significant bits and the values at most 15: an exact quotient that is not
+// half way between two codes is at least 2^-17 of it away from there, further than fp32's division is off.
+template <bool E4M3>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float s) {
+    if (!(s > 0.0f)) return 0;  // 0: the block is all zero; NaN: the block is marked
+    a /= s;
+    b /= s;
+    c /= s;
+    d /= s;
+    if constexpr (E4M3) {
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+        return lo | (hi << 16);
+    } else {
+        const uint32_t lo = (__float2int_rn(a) & 0xff) | ((__float2int_rn(b) & 0xff) << 8);
+        const uint32_t hi = (__float2int_rn(c) & 0xff) | ((__float2int_rn(d) & 0xff) << 8);
+        return lo | (hi << 16);
+    }
+}
+
+// The four codes of a word as fp32 (without the scale).
+template <bool E4M3>
+__device__ __forceinline__ void decode4(uint32_t w, float* v) {
+    uint32_t lo, hi;
+    codes_to_half<E4M3, 0>(w, lo, hi);
+    const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo));
+    const float2 b = __half22float2(*reinterpret_cast<__half2*>(&hi));
+    v[0] = a.x * code_unit<E4M3>();
+    v[1] = a.y * code_unit<E4M3>();
+    v[2] = b.x * code_unit<E4M3>();
+    v[3] = b.y * code_unit<E4M3>();
+}
+
+struct KvAppendArgs {
+    uint8_t* codes[2];
+    float* scales[2];
+    const uint16_t* src[2];
+    int64_t stride[2][3];
+    bool vec[2];
+    const int32_t* lengths;
+    const int32_t* counts;
+    int64_t capacity;
+    int heads, head_dim, tokens, block_shift, spans;
+    bool bf16;
+};
+
+constexpr int kAppendThreads = 256;
+
+// One block of the cache (`block` tokens of a head, keys or values) per CTA: largest |x| of the new tokens, the
+// block's scale, their codes; where the scale grows, the earlier tokens' codes again. The new tokens stay in registers
+// between the two passes (VPT vectors of 16 elements a thread), so every element is read once. The largest |x| is
+// taken on the bit patterns: it also finds infinities and NaN, which a floating maximum would drop.
+template <bool E4M3, int VPT>
+__global__ void __launch_bounds__(kAppendThreads) k_kv_append(KvAppendArgs a) {
+    const int tid = threadIdx.x;
+    int64_t b = blockIdx.x;
+    const int i = static_cast<int>(b % a.spans);
+    b /= a.spans;
+    const int kv = static_cast<int>(b & 1);
+    b >>= 1;
+    const int h = static_cast<int>(b % a.heads);
+    const int n = static_cast<int>(b / a.heads);
+    const int len = kv_length(a.lengths, n, a.capacity);
+    const int cnt = kv_count(a.counts, n, a.tokens);
+    const int block = 1 << a.block_shift;
+    const int64_t slot = (static_cast<int64_t>(len >> a.block_shift) + i) << a.block_shift;  // first token of the block
+    const int64_t end = min(min(slot + block, static_cast<int64_t>(len) + cnt), a.capacity);
+    const int64_t begin = max(slot, static_cast<int64_t>(len));
+    if (begin >= end) return;
+    const int held = static_cast<int>(begin - slot);
+    const int fresh = static_cast<int>(end - begin);
+    const int cpr = a.head_dim >> 4;  // vectors of 16 elements in a row
+    const size_t head = static_cast<size_t>(n) * a.heads + h;
+    uint8_t* dst = a.codes[kv] + (head * a.capacity + slot) * a.head_dim;
+    float* scale = a.scales[kv] + head * (a.capacity >> a.block_shift) + (slot >> a.block_shift);
+    const uint16_t* src = a.src[kv] + n * a.stride[kv][0] + h * a.stride[kv][1];
+
+    uint32_t x[VPT][8];
+    uint32_t most = 0;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int idx = v * kAppendThreads + tid;
+        if (idx < fresh * cpr) {
+            const int t = idx / cpr;
+            const uint16_t* p = src + (begin - len + t) * a.stride[kv][2] + (idx - t * cpr) * 16;
+            if (a.vec[kv]) {
+                const uint4 lo = *reinterpret_cast<const uint4*>(p);
+                const uint4 hi = *reinterpret_cast<const uint4*>(p + 8);
+                x[v][0] = lo.x, x[v][1] = lo.y, x[v][2] = lo.z, x[v][3] = lo.w;
+                x[v][4] = hi.x, x[v][5] = hi.y, x[v][6] = hi.z, x[v][7] = hi.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) x[v][j] = p[2 * j] | (static_cast<uint32_t>(p[2 * j + 1]) << 16);
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) most = __vmaxu2(most, x[v][j] & 0x7fff7fffu);
+        }
+    }
+    const float old = held > 0 ? *scale : 0.0f;
+    most = max(most & 0xffffu, most >> 16);
+    __shared__ uint32_t part[kAppendThreads / 32];
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((tid & 31) == 0) part[tid >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, part[w]);
+    float s = old;
+    if (most >= (a.bf16 ? 0x7f80u : 0x7c00u)) {
+        s = kNan;
+    } else {
+        const float now = scale_of<E4M3>(unpack16(most, a.bf16).x);
+        if (now > s) s = now;  // an old NaN stays
+    }
+    if (tid == 0) *scale = s;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int idx = v * kAppendThreads + tid;
+        if (idx < fresh * cpr) {
+            uint32_t q[4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float2 lo = unpack16(x[v][2 * j], a.bf16);
+                const float2 hi = unpack16(x[v][2 * j + 1], a.bf16);
+                q[j] = encode4<E4M3>(lo.x, lo.y, hi.x, hi.y, s);
+            }
+            *reinterpret_cast<uint4*>(dst + static_cast<size_t>(held) * a.head_dim + static_cast<size_t>(idx) * 16) =
+                make_uint4(q[0], q[1], q[2], q[3]);
+        }
+    }
+    if (held > 0 && s > old) {
+        for (int idx = tid; idx < held * cpr; idx += kAppendThreads) {
+            uint4* p = reinterpret_cast<uint4*>(dst) + idx;
+            const uint4 w = *p;
+            uint32_t q[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float f[4];
+                decode4<E4M3>(q[j], f);
+                q[j] = encode4<E4M3>(f[0] * old, f[1] * old, f[2] * old, f[3] * old, s);
+            }
+            *p = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+    }
+}
+
+struct KvReadArgs {
+    const uint8_t* codes[2];
+    const float* scales[2];
+    void* out[2];
+    const int32_t* lengths;
+    const int32_t* first;
+    int64_t first_all, count, capacity, vectors;  // vectors of 16 elements in one output
+    int heads, head_dim, block_shift;
+    int dtype;
+};
+
+// A vector of 16 elements a thread: 16 bytes of codes in, 32 or 64 bytes out.
+template <bool E4M3>
+__global__ void __launch_bounds__(256) k_kv_read(KvReadArgs a) {
+    const int cpr = a.head_dim >> 4;
+    const int kv = blockIdx.y;
+    if (a.out[kv] == nullptr) return;
+    for (int64_t v = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; v < a.vectors;
+         v += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        int64_t r = v / cpr;
+        const int c = static_cast<int>(v - r * cpr);
+        const int64_t head = r / a.count;
+        const int64_t i = r - head * a.count;
+        const int n = static_cast<int>(head / a.heads);
+        const int64_t t = (a.first != nullptr ? a.first[n] : a.first_all) + i;
+        float f[16];
+        if (t >= 0 && t < kv_length(a.lengths, n, a.capacity)) {
+            const float s = a.scales[kv][head * (a.capacity >> a.block_shift) + (t >> a.block_shift)];
+            const uint4 w = reinterpret_cast<const uint4*>(a.codes[kv] + (head * a.capacity + t) * a.head_dim)[c];
+            decode4<E4M3>(w.x, f);
+            decode4<E4M3>(w.y, f + 4);
+            decode4<E4M3>(w.z, f + 8);
+            decode4<E4M3>(w.w, f + 12);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) f[j] *= s;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 16; ++j) f[j] = 0.0f;
+        }
+        if (a.dtype == DT_FLOAT32) {
+            float4* o = reinterpret_cast<float4*>(a.out[kv]) + v * 4;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
+        } else {
+            uint32_t q[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (a.dtype == DT_BFLOAT16) {
+                    const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+                    q[j] = *reinterpret_cast<const uint32_t*>(&p);
+                } else {
+                    q[j] = pack_half2(f[2 * j], f[2 * j + 1]);
+                }
+            }
+            uint4* o = reinterpret_cast<uint4*>(a.out[kv]) + v * 2;
+            o[0] = make_uint4(q[0], q[1], q[2], q[3]);
+            o[1] = make_uint4(q[4], q[5], q[6], q[7]);
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Attention of few query rows (single tokens, drafts)
+// ---------------------------------------------------------------------------------------------------------------
+// 16 query rows of a key head against tiles of 128 tokens. The tiles of all (sequence, head, row tile) items stand in
+// one list, and every CTA takes an equal stretch of it, whatever the lengths: a stretch may end one item and begin the
+// next. An item inside one stretch is finished there; the others leave (running maximum, sum, unnormalised output) in
+// the workspace, and k_kv_merge joins them in the order of the list.
+//
+// Within a CTA each of the four warps streams its own 32 tokens of every tile through shared memory with cp.async and
+// keeps its own softmax state: no barrier inside the loop; the four states are joined once per item.
+// Scores and outputs use mma.m16n8k16 with fp16 operands: this path is bound by reading the cache, and 16 rows would
+// leave 7/8 of a tcgen05 tile empty. Which elements share a k16 step is free as long as queries and keys agree, so a
+// lane takes 16 consecutive bytes of a key row, enough for four steps.
+constexpr int kTile = 128;
+constexpr int kWarpTokens = 32;
+constexpr int kAttnThreads = 128;
+constexpr float kShift = 10.0f;  // weights are kept as 2^(x - max + 10): fp16 then reaches down to 2^-34 of the largest
+
+struct KvPartials {
+    float* out;     // [slot][16][EP]
+    float2* stats;  // [slot][16]: maximum (log2), sum
+    float* scores;  // [item][16][capacity] log2 scores, or null
+    float* lse2;    // [batch * kv_heads][rows]: log2 of the sum of 2^score
+};
+
+template <int EP>
+struct AttnShape {
+    static constexpr int kChunks = EP / 16;
+    static constexpr int kStages = EP == 64 ? 4 : 3;
+    static constexpr int kSliceBytes = kWarpTokens * EP;      // keys, or values, of one warp's tokens
+    static constexpr int kStageBytes = 2 * kSliceBytes;
+    static constexpr int kWarpBytes = kStages * kStageBytes;
+    static constexpr int kScaleBytes = 4 * kStages * 2 * 4;   // after the four warps' stages
+    static constexpr int kSmem = 4 * kWarpBytes + kScaleBytes + 4 * 16 * 8 + 64;
+    static_assert(kWarpBytes >= 16 * EP * 4, "the outputs of an item's join reuse a warp's stages");
+};
+
+// Byte offset of 16-byte chunk `c` of row `r`: chunks are permuted within 128 bytes so that neither the key reads (two
+// rows of four chunks a phase) nor the value reads (eight rows of one chunk) meet in a bank.
+template <int EP>
+__device__ __forceinline__ int swizzled(int r, int c) {
+    if constexpr (EP == 64) {
+        const int line = r >> 1;
+        return line * 128 + (((((r & 1) << 2) | c) ^ (line & 3)) << 4);
+    } else {
+        const int f = ((r & 1) << 2) | ((r >> 1) & 3);
+        return r * EP + ((c & ~7) << 4) + (((c & 7) ^ f) << 4);
+    }
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t smem, const void* gmem, bool live) {
+    const int bytes = live ? 16 : 0;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ void cp_async4(uint32_t smem, const void* gmem) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem), "l"(gmem) : "memory");
+}
+
+__device__ __forceinline__ void mma16816(float* d, uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                         uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// Address of query row `row` (of a key head) of a sequence, or null outside.
+__device__ __forceinline__ const uint16_t* query_row(const KvAttnArgs& a, int n, int h, int row) {
+    if (row >= a.rows) return nullptr;
+    const int t = row / a.group, j = row - t * a.group;
+    return static_cast<const uint16_t*>(a.query) + n * a.q_stride_n +
+           static_cast<int64_t>(h * a.group + j) * a.q_stride_h + t * a.q_stride_t;
+}
+
+// The A fragments of 16 query rows as fp16, and each lane's two row factors (inverse of the rows' powers of two).
+// Registers [kc * 16 + s * 4 + i]: 64-wide span kc, step s, fragment register i.
+template <int EP>
+__device__ __forceinline__ void load_query(const KvAttnArgs& a, int n, int h, int row0, uint32_t* q, float* inv) {
+    const int lane = threadIdx.x & 31, c = lane & 3;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const uint16_t* p = query_row(a, n, h, row0 + (lane >> 2) + half * 8);
+        uint32_t x[EP / 8];
+        float amax = 0.0f;
+#pragma unroll
+        for (int kc = 0; kc < EP / 64; ++kc) {
+            const int e = kc * 64 + c * 16;
+            const bool live = p != nullptr && e < a.head_dim;
+            if (live && a.q_vec) {
+                const uint4 u = *reinterpret_cast<const uint4*>(p + e);
+                const uint4 w = *reinterpret_cast<const uint4*>(p + e + 8);
+                x[kc * 8 + 0] = u.x, x[kc * 8 + 1] = u.y, x[kc * 8 + 2] = u.z, x[kc * 8 + 3] = u.w;
+                x[kc * 8 + 4] = w.x, x[kc * 8 + 5] = w.y, x[kc * 8 + 6] = w.z, x[kc * 8 + 7] = w.w;
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j)
+                    x[kc * 8 + j] = live ? p[e + 2 * j] | (static_cast<uint32_t>(p[e + 2 * j + 1]) << 16) : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 f = unpack16(x[kc * 8 + j], a.query_bf16);
+                amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+            }
+        }
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+        float mul;
+        row_power(amax, mul, inv[half]);
+#pragma unroll
+        for (int kc = 0; kc < EP / 64; ++kc)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float2 f = unpack16(x[kc * 8 + j], a.query_bf16);
+                // words 2s and 2s + 1 of the lane's 16 elements are step s's k columns (2c, 2c+1) and (2c+8, 2c+9)
+                q[kc * 16 + (j >> 1) * 4 + (j & 1) * 2 + half] = pack_half2(f.x * mul, f.y * mul);
+            }
+    }
+}
+
+// Tiles of a sequence of `len` tokens: at least one, so that an empty sequence's outputs are written too.
+__device__ __forceinline__ int tiles_of(int len) { return len <= 0 ? 1 : (len + kTile - 1) / kTile; }
+
+// Position of tile `x` of the list. All threads of the warp call it; n = batch if x is behind the end.
+struct TilePos {
+    int n;         // sequence
+    int item;      // (head, row tile) within the sequence
+    int tile;      // within the item
+    int64_t base;  // list position of the sequence's first tile
+};
+
+__device__ __forceinline__ TilePos find_tile(const KvAttnArgs& a, int per_seq, int64_t x) {
+    const int lane = threadIdx.x & 31;
+    int64_t base = 0;
+    for (int n0 = 0; n0 < a.batch; n0 += 32) {
+        const int n = n0 + lane;
+        const int64_t mine = n < a.batch ? static_cast<int64_t>(tiles_of(kv_length(a.lengths, n, a.capacity))) * per_seq
+                                         : 0;
+        int64_t incl = mine;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+            if (lane >= d) incl += o;
+        }
+        const uint32_t over = __ballot_sync(0xffffffffu, base + incl > x);
+        if (over != 0) {
+            const int who = __ffs(over) - 1;
+            const int64_t b = __shfl_sync(0xffffffffu, base + incl - mine, who);
+            const int tiles = static_cast<int>(__shfl_sync(0xffffffffu, mine, who) / per_seq);
+            const int64_t rem = x - b;
+            return TilePos{n0 + who, static_cast<int>(rem / tiles), static_cast<int>(rem % tiles), b};
+        }
+        base += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    return TilePos{a.batch, 0, 0, base};
+}
+
+template <bool E4M3, int EP>
+__global__ void __launch_bounds__(kAttnThreads, EP == 256 ? 1 : EP == 128 ? 2 : 3) k_kv_attend(KvAttnArgs a, KvPartials w, int row_tiles) {
+    using S = AttnShape<EP>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c4 = lane & 3, r4 = lane >> 2;
+    uint8_t* const stages = smem + warp * S::kWarpBytes;
+    float* const scales = reinterpret_cast<float*>(smem + 4 * S::kWarpBytes) + warp * S::kStages * 2;
+    float2* const joined = reinterpret_cast<float2*>(smem + 4 * S::kWarpBytes + S::kScaleBytes);  // [warp][16]
+    const uint32_t stages_s = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
+    const uint32_t scales_s = static_cast<uint32_t>(__cvta_generic_to_shared(scales));
+    const int per_seq = a.kv_heads * row_tiles;
+
+    // this CTA's stretch of the list
+    const int64_t total = find_tile(a, per_seq, INT64_MAX).base;
+    const int64_t each = (total + gridDim.x - 1) / gridDim.x;
+    int64_t x = each * blockIdx.x;
+    const int64_t x_end = min(x + each, total);
+    if (x >= x_end) return;
+    TilePos pos = find_tile(a, per_seq, x);
+
+    while (x < x_end) {
+        const int n = pos.n, h = pos.item / row_tiles, rt = pos.item % row_tiles;
+        const int len = kv_length(a.lengths, n, a.capacity), cnt = kv_count(a.counts, n, a.tokens);
+        const int tiles = tiles_of(len);
+        const int t0 = pos.tile;
+        const int nt = static_cast<int>(min(static_cast<int64_t>(tiles - t0), x_end - x));
+        const size_t head = static_cast<size_t>(n) * a.kv_heads + h;
+        const uint8_t* const kbase = a.key + head * a.capacity * a.head_dim;
+        const uint8_t* const vbase = a.value + head * a.capacity * a.head_dim;
+        const float* const ks = a.key_scale + head * a.nblocks;
+        const float* const vs = a.value_scale + head * a.nblocks;
+        const int row_lo = rt * 16 + r4, row_hi = row_lo + 8;
+        const int lim_lo = kv_limit(a, row_lo, len, cnt), lim_hi = kv_limit(a, row_hi, len, cnt);
+        float* const scores = w.scores == nullptr ? nullptr
+                                                  : w.scores + (head * row_tiles + rt) * 16 * static_cast<size_t>(a.capacity);
+
+        auto fetch = [&](int it) {
+            const int st = it % S::kStages;
+            const int tok = (t0 + it) * kTile + warp * kWarpTokens;
+            if (it < nt && tok < len) {
+                const uint32_t ks_s = stages_s + st * S::kStageBytes, vs_s = ks_s + S::kSliceBytes;
+                const size_t off = static_cast<size_t>(tok) * a.head_dim;
+#pragma unroll
+                for (int j = 0; j < S::kChunks; ++j) {
+                    const int idx = j * 32 + lane, r = idx / S::kChunks, c = idx % S::kChunks;
+                    const bool live = tok + r < len && c * 16 < a.head_dim;
+                    const size_t o = live ? off + static_cast<size_t>(r) * a.head_dim + c * 16 : off;
+                    cp_async16(ks_s + swizzled<EP>(r, c), kbase + o, live);
+                    cp_async16(vs_s + swizzled<EP>(r, c), vbase + o, live);
+                }
+                if (lane < 2) {
+                    const int b = tok >> a.block_shift;
+                    cp_async4(scales_s + (st * 2 + lane) * 4, lane == 0 ? ks + b : vs + b);
+                }
+            }
+            asm volatile("cp.async.commit_group;" ::: "memory");
+        };
+
+        float o[EP / 16][2][4];
+#pragma unroll
+        for (int i = 0; i < EP / 16; ++i)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) o[i][j >> 2][j & 3] = 0.0f;
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+
+#pragma unroll
+        for (int it = 0; it < S::kStages - 1; ++it) fetch(it);
+        uint32_t q[EP / 4];
+        float f[2];
+        load_query<EP>(a, n, h, rt * 16, q, f);
+        f[0] *= a.scale_log2 * code_unit<E4M3>();
+        f[1] *= a.scale_log2 * code_unit<E4M3>();
+
+        for (int it = 0; it < nt; ++it) {
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
+            __syncwarp();
+            fetch(it + S::kStages - 1);
+            const int tok = (t0 + it) * kTile + warp * kWarpTokens;
+            if (tok >= len) continue;
+            const int st = it % S::kStages;
+            const uint8_t* const kst = stages + st * S::kStageBytes;
+            const float kscale = scales[st * 2], vscale = scales[st * 2 + 1] * code_unit<E4M3>();
+
+            float s[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+#pragma unroll
+                for (int kc = 0; kc < EP / 64; ++kc) {
+                    const uint4 k4 = *reinterpret_cast<const uint4*>(kst + swizzled<EP>(j * 8 + r4, kc * 4 + c4));
+                    const uint32_t kw[4] = {k4.x, k4.y, k4.z, k4.w};
+#pragma unroll
+                    for (int step = 0; step < 4; ++step) {
+                        uint32_t b0, b1;
+                        codes_to_half<E4M3, 0>(kw[step], b0, b1);
+                        const uint32_t* qa = q + kc * 16 + step * 4;
+                        mma16816(s[j], qa[0], qa[1], qa[2], qa[3], b0, b1);
+                    }
+                }
+            }
+            const float g[2] = {f[0] * kscale, f[1] * kscale};
+            float top[2] = {-INFINITY, -INFINITY};
+            const bool ragged = tok + kWarpTokens > min(lim_lo, lim_hi);
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = s[j][i] * g[i >> 1];
+                    if (ragged && tok + j * 8 + c4 * 2 + (i & 1) >= (i < 2 ? lim_lo : lim_hi)) v = -INFINITY;
+                    s[j][i] = v;
+                    top[i >> 1] = fmaxf(top[i >> 1], v);
+                }
+            if (scores != nullptr) {
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const size_t t = tok + j * 8 + c4 * 2;  // the capacity is a multiple of 32: the pair is inside
+                    *reinterpret_cast<float2*>(scores + r4 * static_cast<size_t>(a.capacity) + t) =
+                        make_float2(s[j][0], s[j][1]);
+                    *reinterpret_cast<float2*>(scores + (r4 + 8) * static_cast<size_t>(a.capacity) + t) =
+                        make_float2(s[j][2], s[j][3]);
+                }
+            }
+            float base[2];
+            bool grown = false;
+            float alpha[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+                const float now = fmaxf(m[i], top[i]);
+                alpha[i] = now == m[i] ? 1.0f : ex2(m[i] - now);
+                grown |= now != m[i];
+                m[i] = now;
+                base[i] = now == -INFINITY ? 0.0f : now - kShift;  // a row that saw nothing: 2^-inf = 0
+            }
+            if (__any_sync(0xffffffffu, grown)) {
+                l[0] *= alpha[0];
+                l[1] *= alpha[1];
+#pragma unroll
+                for (int i = 0; i < EP / 16; ++i)
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) o[i][j >> 2][j & 3] *= alpha[(j & 3) >> 1];
+            }
+            uint32_t p[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    s[j][i] = ex2(s[j][i] - base[i >> 1]);
+                    l[i >> 1] += s[j][i];
+                }
+                // fp16 weights: 11 significant bits, half a bf16 output's rounding at most
+                p[j][0] = pack_half2(s[j][0], s[j][1]);
+                p[j][1] = pack_half2(s[j][2], s[j][3]);
+            }
+            // values: 8 x 8 pairs of bytes transposed on the way in; even and odd elements become two column tiles
+            const uint32_t vst = stages_s + st * S::kStageBytes + S::kSliceBytes;
+#pragma unroll
+            for (int e = 0; e < EP / 16; ++e) {
+                uint32_t v[4];
+                asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                             : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
+                             : "r"(vst + swizzled<EP>(lane, e)));
+                float even[4] = {0.0f, 0.0f, 0.0f, 0.0f}, odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    uint32_t e0, o0, e1, o1;
+                    codes_to_half<E4M3, 1>(v[2 * j], e0, o0);
+                    codes_to_half<E4M3, 1>(v[2 * j + 1], e1, o1);
+                    mma16816(even, p[2 * j][0], p[2 * j][1], p[2 * j + 1][0], p[2 * j + 1][1], e0, e1);
+                    mma16816(odd, p[2 * j][0], p[2 * j][1], p[2 * j + 1][0], p[2 * j + 1][1], o0, o1);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    o[e][0][i] = fmaf(vscale, even[i], o[e][0][i]);
+                    o[e][1][i] = fmaf(vscale, odd[i], o[e][1][i]);
+                }
+            }
+        }
+
+        // join the four warps' states; the stages are free once every warp's copies have landed
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
+            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
+            if (c4 == 0) joined[warp * 16 + r4 + i * 8] = make_float2(m[i], l[i]);
+        }
+        float* const mine = reinterpret_cast<float*>(stages);
+        __syncwarp();
+#pragma unroll
+        for (int e = 0; e < EP / 16; ++e)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<float4*>(mine + (r4 + i * 8) * EP + e * 16 + c4 * 4) =
+                    make_float4(o[e][0][i * 2], o[e][1][i * 2], o[e][0][i * 2 + 1], o[e][1][i * 2 + 1]);
+        __syncthreads();
+        const bool whole = nt == tiles;
+        // a CTA has at most two open ends: an item that began before its stretch, and one that goes on behind it
+        const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1);
+        for (int idx = threadIdx.x; idx < 16 * (EP / 4); idx += kAttnThreads) {
+            const int r = idx / (EP / 4), e = (idx % (EP / 4)) * 4;
+            float2 ml[4];
+            float mm = -INFINITY, ll = 0.0f;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                ml[k] = joined[k * 16 + r];
+                mm = fmaxf(mm, ml[k].x);
+            }
+            float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const float g = ml[k].x == mm ? 1.0f : ex2(ml[k].x - mm);
+                ll += ml[k].y * g;
+                const float4 v = *reinterpret_cast<const float4*>(smem + k * S::kWarpBytes + (r * EP + e) * 4);
+                acc.x = fmaf(v.x, g, acc.x);
+                acc.y = fmaf(v.y, g, acc.y);
+                acc.z = fmaf(v.z, g, acc.z);
+                acc.w = fmaf(v.w, g, acc.w);
+            }
+            if (!whole) {
+                reinterpret_cast<float4*>(w.out)[(slot * 16 + r) * (EP / 4) + e / 4] = acc;
+                if (e == 0) w.stats[slot * 16 + r] = make_float2(mm, ll);
+                continue;
+            }
+            const int row = rt * 16 + r;
+            if (row >= a.rows) continue;
+            const float g = ll == 0.0f ? 0.0f : 1.0f / ll;
+            const int t = row / a.group, j = row - t * a.group;
+            const size_t orow = (static_cast<size_t>(n) * a.kv_heads * a.group + h * a.group + j) * a.tokens + t;
+            if (e < a.head_dim) {
+                uint2 u;
+                if (a.query_bf16) {
+                    const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * g, acc.y * g);
+                    const __nv_bfloat162 hi = __floats2bfloat162_rn(acc.z * g, acc.w * g);
+                    u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+                } else {
+                    u = make_uint2(pack_half2(acc.x * g, acc.y * g), pack_half2(acc.z * g, acc.w * g));
+                }
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) = u;
+            }
+            if (e == 0) {
+                const float lse2 = ll == 0.0f ? -INFINITY : mm + log2f(ll) - kShift;
+                if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
+                if (w.lse2 != nullptr) w.lse2[head * a.rows + row] = lse2;
+            }
+        }
+        __syncthreads();  // the stages are written again
+        x += nt;
+        if (x < x_end) pos = find_tile(a, per_seq, x);
+    }
+}
+
+// Joins the parts of the items that more than one CTA of k_kv_attend (of `grid` CTAs) worked on: one (item, row) per
+// CTA, a thread per four output elements.
+template <int EP>
+__global__ void __launch_bounds__(EP / 4 < 32 ? 32 : EP / 4) k_kv_merge(KvAttnArgs a, KvPartials w, int row_tiles, int grid) {
+    const int per_seq = a.kv_heads * row_tiles;
+    const int64_t item = blockIdx.x / 16;
+    const int r = blockIdx.x % 16;
+    const int n = static_cast<int>(item / per_seq), in_seq = static_cast<int>(item % per_seq);
+    const int h = in_seq / row_tiles, row = (in_seq % row_tiles) * 16 + r;
+    if (row >= a.rows) return;
+    // list position of the item's first tile
+    int64_t total = 0, first = 0;
+    {
+        const int lane = threadIdx.x & 31;
+        for (int n0 = 0; n0 < a.batch; n0 += 32) {
+            const int k = n0 + lane;
+            int64_t t = k < a.batch ? static_cast<int64_t>(tiles_of(kv_length(a.lengths, k, a.capacity))) * per_seq : 0;
+            int64_t before = k < n ? t : 0;
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1) {
+                t += __shfl_xor_sync(0xffffffffu, t, d);
+                before += __shfl_xor_sync(0xffffffffu, before, d);
+            }
+            total += t;
+            first += before;
+        }
+    }
+    const int tiles = tiles_of(kv_length(a.lengths, n, a.capacity));
+    first += static_cast<int64_t>(in_seq) * tiles;
+    const int64_t each = (total + grid - 1) / grid;
+    const int c0 = static_cast<int>(first / each), c1 = static_cast<int>((first + tiles - 1) / each);
+    if (c0 == c1) return;
+    const int e = threadIdx.x * 4;
+    float mm = -INFINITY;
+    for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, w.stats[(static_cast<size_t>(c) * 2 + (c == c0 ? 1 : 0)) * 16 + r].x);
+    float ll = 0.0f;
+    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 4
+    for (int c = c0; c <= c1; ++c) {
+        const size_t slot = (static_cast<size_t>(c) * 2 + (c == c0 ? 1 : 0)) * 16 + r;
+        const float2 ml = w.stats[slot];
+        const float g = ml.x == mm ? 1.0f : ex2(ml.x - mm);
+        ll += ml.y * g;
+        if (e < EP) {
+            const float4 v = reinterpret_cast<const float4*>(w.out)[slot * (EP / 4) + threadIdx.x];
+            acc.x = fmaf(v.x, g, acc.x);
+            acc.y = fmaf(v.y, g, acc.y);
+            acc.z = fmaf(v.z, g, acc.z);
+            acc.w = fmaf(v.w, g, acc.w);
+        }
+    }
+    const float g = ll == 0.0f ? 0.0f : 1.0f / ll;
+    const int t = row / a.group, j = row - t * a.group;
+    const size_t head = static_cast<size_t>(n) * a.kv_heads + h;
+    const size_t orow = (head * a.group + j) * a.tokens + t;
+    if (e < a.head_dim) {
+        uint2 u;
+        if (a.query_bf16) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * g, acc.y * g);
+            const __nv_bfloat162 hi = __floats2bfloat162_rn(acc.z * g, acc.w * g);
+            u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else {
+            u = make_uint2(pack_half2(acc.x * g, acc.y * g), pack_half2(acc.z * g, acc.w * g));
+        }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) = u;
+    }
+    if (e == 0) {
+        const float lse2 = ll == 0.0f ? -INFINITY : mm + log2f(ll) - kShift;
+        if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
+        if (w.lse2 != nullptr) w.lse2[head * a.rows + row] = lse2;
+    }
+}
+
+// 2^(score - lse2); 0 for a masked token, also of a row that saw nothing.
+__device__ __forceinline__ float weight_of(float score, float lse2) {
+    return score == -INFINITY ? 0.0f : ex2(score - lse2);
+}
+
+// Weights from the stored scores: a thread sums four tokens' columns over the (at most 16) rows of a head.
+__global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w) {
+    const size_t head = blockIdx.y + static_cast<size_t>(gridDim.y) * blockIdx.z;
+    const int n = static_cast<int>(head / a.kv_heads);
+    if (n >= a.batch) return;
+    const int len = kv_length(a.lengths, n, a.capacity);
+    const int64_t t = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
+    if (t >= len) return;
+    const float* sc = w.scores + head * 16 * static_cast<size_t>(a.capacity) + t;
+    float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int r = 0; r < a.rows; ++r) {
+        const float lse2 = w.lse2[head * a.rows + r];
+        const float4 x = *reinterpret_cast<const float4*>(sc + r * static_cast<size_t>(a.capacity));
+        v[0] += weight_of(x.x, lse2);
+        v[1] += weight_of(x.y, lse2);
+        v[2] += weight_of(x.z, lse2);
+        v[3] += weight_of(x.w, lse2);
+    }
+    float* o = a.weights + head * a.capacity + t;
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        if (t + i < len) o[i] = a.accumulate ? o[i] + v[i] : v[i];
+}
+
+// Weights of many query rows: the scores are computed again, 128 tokens of a head a CTA, 32 a warp, with the keys in
+// registers and the rows streamed past them 16 at a time; every token's sum stays in one lane's registers until the
+// end, so there are no atomics and the order of the sum is fixed.
+template <bool E4M3, int EP>
+__global__ void __launch_bounds__(kAttnThreads) k_kv_column_sums(KvAttnArgs a, const float* __restrict__ lse2s, int row_tiles,
+                                                                 int key_tiles) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c4 = lane & 3, r4 = lane >> 2;
+    const size_t head = blockIdx.x / key_tiles;
+    const int n = static_cast<int>(head / a.kv_heads), h = static_cast<int>(head % a.kv_heads);
+    const int len = kv_length(a.lengths, n, a.capacity), cnt = kv_count(a.counts, n, a.tokens);
+    const int tok = static_cast<int>(blockIdx.x % key_tiles) * kTile + warp * kWarpTokens;
+    if (tok >= len) return;
+    const uint8_t* const kbase = a.key + (head * a.capacity + tok) * a.head_dim;
+    const float kscale = a.key_scale[head * a.nblocks + (tok >> a.block_shift)] * code_unit<E4M3>();
+    float sum[4][2];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[j][0] = sum[j][1] = 0.0f;
+    uint4 k4[4][EP / 64];
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int kc = 0; kc < EP / 64; ++kc) {
+            const int r = j * 8 + r4, e = (kc * 4 + c4) * 16;
+            k4[j][kc] = tok + r < len && e < a.head_dim
+                            ? *reinterpret_cast<const uint4*>(kbase + static_cast<size_t>(r) * a.head_dim + e)
+                            : make_uint4(0, 0, 0, 0);
+        }
+    for (int rt = 0; rt < row_tiles; ++rt) {
+        // the last row of a tile sees the most
+        const int last = min(rt * 16 + 15, a.rows - 1);
+        if (a.causal && kv_limit(a, min(last, cnt * a.group - 1), len, cnt) <= tok) continue;
+        uint32_t q[EP / 4];
+        float f[2];
+        load_query<EP>(a, n, h, rt * 16, q, f);
+        const int row[2] = {rt * 16 + r4, rt * 16 + r4 + 8};
+        int lim[2];
+        float lse2[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            f[i] = f[i] * a.scale_log2 * kscale;
+            lim[i] = kv_limit(a, row[i], len, cnt);
+            lse2[i] = row[i] < a.rows ? lse2s[head * a.rows + row[i]] : 0.0f;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int kc = 0; kc < EP / 64; ++kc) {
+                const uint32_t kw[4] = {k4[j][kc].x, k4[j][kc].y, k4[j][kc].z, k4[j][kc].w};
+#pragma unroll
+                for (int step = 0; step < 4; ++step) {
+                    uint32_t b0, b1;
+                    codes_to_half<E4M3, 0>(kw[step], b0, b1);
+                    const uint32_t* qa = q + kc * 16 + step * 4;
+                    mma16816(s, qa[0], qa[1], qa[2], qa[3], b0, b1);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (tok + j * 8 + c4 * 2 + (i & 1) < lim[i >> 1])
+                    sum[j][i & 1] += ex2(s[i] * f[i >> 1] - lse2[i >> 1]);
+        }
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+#pragma unroll
+            for (int d = 4; d < 32; d <<= 1) sum[j][i] += __shfl_xor_sync(0xffffffffu, sum[j][i], d);
+            const int t = tok + j * 8 + c4 * 2 + i;
+            if (r4 == 0 && t < len) {
+                float* o = a.weights + head * a.capacity + t;
+                *o = a.accumulate ? *o + sum[j][i] : sum[j][i];
+            }
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Eviction
+// ---------------------------------------------------------------------------------------------------------------
+struct KvEvictArgs {
+    const uint8_t* src[2];
+    const float* src_scale[2];
+    uint8_t* dst[2];
+    float* dst_scale[2];
+    const int32_t* lengths;
+    const float* weights;
+    int32_t* kept;  // [batch * heads][budget]
+    int32_t* dst_lengths;
+    float* dst_weights;
+    int64_t src_cap, dst_cap;
+    int batch, heads, head_dim, block_shift, budget, recent, spans;
+};
+
+constexpr int kSelectThreads = 1024;
+
+// Order of the weights as unsigned integers: NaN above everything, -0 equal to 0.
+__device__ __forceinline__ uint32_t order_key(float f) {
+    if (f != f) return 0xffffffffu;
+    const uint32_t b = __float_as_uint(f + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+// Sum over the CTA and the part of it before this thread.
+__device__ __forceinline__ int block_scan(int v, int* warp_sums, int* all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int incl = v;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+    }
+    __syncthreads();  // earlier readers of warp_sums
+    if (lane == 31) warp_sums[warp] = incl;
+    __syncthreads();
+    int wsum = warp_sums[lane], winc = wsum;  // 32 warps
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+        const int o = __shfl_up_sync(0xffffffffu, winc, d);
+        if (lane >= d) winc += o;
+    }
+    *all = __shfl_sync(0xffffffffu, winc, 31);
+    return incl - v + __shfl_sync(0xffffffffu, winc - wsum, warp);
+}
+
+// Positions that stay, ascending: a radix selection of the threshold weight among the tokens before the recent ones
+// (digits of 11, 11 and 10 bits, a histogram in shared memory each), then one pass that writes the positions in
+// order, of those equal to the threshold the first ones. One head per CTA.
+__global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a) {
+    __shared__ int hist[2048];
+    __shared__ int warp_sums[32];
+    __shared__ uint32_t sh_digit;
+    __shared__ int sh_above;
+    const int tid = threadIdx.x;
+    const size_t head = blockIdx.x;
+    const int n = static_cast<int>(head / a.heads);
+    const int len = kv_length(a.lengths, n, a.src_cap);
+    const int count = min(len, a.budget);
+    const int late = min(len, a.recent);
+    const int old = len - late;   // tokens that compete
+    int need = count - late;      // places for them
+    const float* const w = a.weights + head * a.src_cap;
+    int32_t* const kept = a.kept + head * a.budget;
+    if (head % a.heads == 0 && tid == 0) a.dst_lengths[n] = count;
+    for (int i = count + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+    if (need == old) {
+        for (int i = tid; i < count; i += kSelectThreads) kept[i] = i;
+        return;
+    }
+    for (int i = tid; i < late; i += kSelectThreads) kept[need + i] = old + i;
+    if (need == 0) return;
+
+    const int places = need;
+    uint32_t prefix = 0, mask = 0;
+    const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = shifts[pass], size = 1 << bits[pass];
+        for (int i = tid; i < 2048; i += kSelectThreads) hist[i] = 0;
+        __syncthreads();
+        for (int i = tid; i < (old + 31) / 32 * 32; i += kSelectThreads) {
+            const uint32_t key = i < old ? order_key(w[i]) : 0u;
+            const bool in = i < old && (key & mask) == prefix;
+            const uint32_t digit = (key >> shift) & (size - 1);
+            const uint32_t live = __ballot_sync(0xffffffffu, in);
+            if (live == 0) continue;
+            const int leader = __ffs(live) - 1;
+            const uint32_t lead_digit = __shfl_sync(0xffffffffu, digit, leader);  // every lane takes part
+            // a warp whose keys agree (ties, such as tokens never attended to) adds once
+            if (__all_sync(0xffffffffu, !in || digit == lead_digit)) {
+                if ((tid & 31) == leader) atomicAdd(&hist[digit], __popc(live));
+            } else if (in) {
+                atomicAdd(&hist[digit], 1);
+            }
+        }
+        __syncthreads();
+        // the digit at which the count from above reaches the places that are left; two bins a thread, from the top
+        const int b0 = size - 1 - 2 * tid, b1 = b0 - 1;
+        const int h0 = b0 >= 0 ? hist[b0] : 0, h1 = b1 >= 0 ? hist[b1] : 0;
+        int all;
+        const int above = block_scan(h0 + h1, warp_sums, &all);
+        if (above < need && above + h0 >= need) {
+            sh_digit = b0;
+            sh_above = above;
+        } else if (above + h0 < need && above + h0 + h1 >= need) {
+            sh_digit = b1;
+            sh_above = above + h0;
+        }
+        __syncthreads();
+        prefix |= sh_digit << shift;
+        mask |= static_cast<uint32_t>(size - 1) << shift;
+        need -= sh_above;
+        __syncthreads();
+    }
+    // all above the threshold `prefix`, and the first `need` equal to it
+    int done = 0, ties = 0;
+    for (int i0 = 0; i0 < old && done < places; i0 += kSelectThreads) {
+        const int i = i0 + tid;
+        const uint32_t key = i < old ? order_key(w[i]) : 0u;
+        const bool more = i < old && key > prefix, tie = i < old && key == prefix;
+        int all;
+        const int before = block_scan((more ? 1 : 0) | (tie ? 0x10000 : 0), warp_sums, &all);
+        const int tie_at = ties + (before >> 16);
+        if (more || (tie && tie_at < need)) kept[done + (before & 0xffff) + min(tie_at, need) - min(ties, need)] = i;
+        const int now = ties + (all >> 16);
+        done += (all & 0xffff) + min(now, need) - min(ties, need);
+        ties = now;
+    }
+}
+
+// One block of dst (keys or values) per CTA: the kept tokens' values, their largest, the new scale, the codes.
+template <bool E4M3, int VPT>
+__global__ void __launch_bounds__(kAppendThreads) k_kv_gather(KvEvictArgs a) {
+    const int tid = threadIdx.x;
+    int64_t b = blockIdx.x;
+    const int i = static_cast<int>(b % a.spans);
+    b /= a.spans;
+    const int kv = static_cast<int>(b & 1);
+    const size_t head = static_cast<size_t>(b >> 1);
+    const int n = static_cast<int>(head / a.heads);
+    const int count = min(kv_length(a.lengths, n, a.src_cap), a.budget);
+    const int block = 1 << a.block_shift;
+    const int slot = i << a.block_shift;
+    const int live = min(block, count - slot);
+    const int32_t* const kept = a.kept + head * a.budget + slot;
+    if (kv == 0 && a.dst_weights != nullptr && tid < block) {
+        a.dst_weights[head * a.dst_cap + slot + tid] =
+            tid < live ? a.weights[head * a.src_cap + kept[tid]] : 0.0f;
+    }
+    if (live <= 0) return;
+    const int cpr = a.head_dim >> 4;
+    const uint8_t* const src = a.src[kv] + head * a.src_cap * a.head_dim;
+    const float* const src_scale = a.src_scale[kv] + head * (a.src_cap >> a.block_shift);
+    uint4 x[VPT];
+    float sc[VPT];
+    uint32_t most = 0;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int idx = v * kAppendThreads + tid;
+        x[v] = make_uint4(0, 0, 0, 0);
+        sc[v] = 0.0f;
+        if (idx < live * cpr) {
+            const int t = idx / cpr;
+            const int from = kept[t];
+            x[v] = reinterpret_cast<const uint4*>(src + static_cast<size_t>(from) * a.head_dim)[idx - t * cpr];
+            sc[v] = src_scale[from >> a.block_shift];
+            const uint32_t q[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float f[4];
+                decode4<E4M3>(q[j], f);
+#pragma unroll
+                for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(f[k] * sc[v]) & 0x7fffffffu);
+            }
+        }
+    }
+    __shared__ uint32_t part[kAppendThreads / 32];
+    most = __reduce_max_sync(0xffffffffu, most);
+    if ((tid & 31) == 0) part[tid >> 5] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, part[w]);
+    const float s = most >= 0x7f800000u ? kNan : scale_of<E4M3>(__uint_as_float(most));
+    if (tid == 0) a.dst_scale[kv][head * (a.dst_cap >> a.block_shift) + i] = s;
+    uint4* const dst = reinterpret_cast<uint4*>(a.dst[kv] + (head * a.dst_cap + slot) * a.head_dim);
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int idx = v * kAppendThreads + tid;
+        if (idx < block * cpr) {
+            uint32_t q[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                float f[4];
+                decode4<E4M3>(q[j], f);
+                q[j] = encode4<E4M3>(f[0] * sc[v], f[1] * sc[v], f[2] * sc[v], f[3] * sc[v], s);
+            }
+            dst[idx] = make_uint4(q[0], q[1], q[2], q[3]);
+        }
+    }
+}
+
+// dst_weights behind the blocks that k_kv_gather writes.
+__global__ void __launch_bounds__(256) k_kv_zero_tail(float* w, int64_t heads, int64_t cap, int64_t from) {
+    const int64_t tail = cap - from;
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < heads * tail;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.x)
+        w[i / tail * cap + from + i % tail] = 0.0f;
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Host side
+// ---------------------------------------------------------------------------------------------------------------
+bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+int log2_of(int64_t v) {
+    int s = 0;
+    while ((int64_t{1} << s) < v) ++s;
+    return s;
+}
+
+int check_cache(const dt_kv_cache* c, const char* name) {
+    const std::string who = std::string(name) + ": ";
+    if (c == nullptr) return set_error(DT_ERR_INVALID, who + "null cache");
+    if (c->code != DT_KV_INT8 && c->code != DT_KV_E4M3) return set_error(DT_ERR_INVALID, who + "unknown code type");
+    if (c->block != 32 && c->block != 64 && c->block != 128)
+        return set_error(DT_ERR_INVALID, who + "block must be 32, 64 or 128 tokens");
+    if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16 != 0)
+        return set_error(DT_ERR_INVALID, who + "head_dim must be a multiple of 16 up to 256");
+    if (c->batch < 0 || c->kv_heads < 1 || c->capacity < 0 || c->capacity % c->block != 0)
+        return set_error(DT_ERR_INVALID, who + "capacity must be a multiple of block, heads at least 1");
+    if (c->capacity > (int64_t{1} << 30) || c->batch > (int64_t{1} << 20) || c->kv_heads > (int64_t{1} << 16) ||
+        c->batch * c->kv_heads > (int64_t{1} << 24))
+        return set_error(DT_ERR_INVALID, who + "too many tokens, sequences or heads");
+    if (c->batch == 0 || c->capacity == 0) return DT_OK;
+    if (c->key == nullptr || c->value == nullptr || c->key_scale == nullptr || c->value_scale == nullptr)
+        return set_error(DT_ERR_INVALID, who + "null buffer");
+    if (!aligned16(c->key) || !aligned16(c->value)) return set_error(DT_ERR_INVALID, who + "codes must be 16-byte aligned");
+    return DT_OK;
+}
+
+bool rows_vectorised(const void* p, const int64_t* strides) {
+    return aligned16(p) && strides[0] % 8 == 0 && strides[1] % 8 == 0 && strides[2] % 8 == 0;
+}
+
+int grid_of(int64_t ctas, const char* what, unsigned* grid) {
+    if (ctas > INT32_MAX) return set_error(DT_ERR_INVALID, std::string(what) + ": too many blocks");
+    *grid = static_cast<unsigned>(ctas);
+    return DT_OK;
+}
+
+// f(constant) for the number of vectors a thread of a block kernel holds.
+template <typename F>
+void with_vpt(int64_t block, int64_t head_dim, F f) {
+    const int64_t vectors = block * head_dim / 16;
+    if (vectors <= kAppendThreads) f(std::integral_constant<int, 1>{});
+    else if (vectors <= 2 * kAppendThreads) f(std::integral_constant<int, 2>{});
+    else if (vectors <= 4 * kAppendThreads) f(std::integral_constant<int, 4>{});
+    else f(std::integral_constant<int, 8>{});
+}
+
+// f(constant) for the padded head size of the attention kernels.
+template <typename F>
+int with_head_dim(int64_t head_dim, F f) {
+    if (head_dim <= 64) return f(std::integral_constant<int, 64>{});
+    if (head_dim <= 128) return f(std::integral_constant<int, 128>{});
+    return f(std::integral_constant<int, 256>{});
+}
+
+int64_t padded_head(int64_t e) { return e <= 64 ? 64 : e <= 128 ? 128 : 256; }
+int attn_ctas_per_sm(int64_t e) { return e <= 64 ? 3 : e <= 128 ? 2 : 1; }
+
+// Stored scores against computing them again, where few rows ask for weights: see k_kv_weights.
+bool stores_scores(const dt_kv_cache* c, int64_t rows) {
+    return rows <= 16 && c->batch * c->kv_heads * 16 * c->capacity * 4 <= (int64_t{1} << 30);
+}
+
+struct AttnPlan {
+    int64_t rows, row_tiles;
+    int grid;
+    size_t out, stats, lse2, scores, bytes;  // offsets and the total
+};
+
+int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool weights, AttnPlan* p) {
+    int dev = 0, sms = 0;
+    int st = current_device(&dev, &sms);
+    if (st != DT_OK) return st;
+    const int64_t ep = padded_head(c->head_dim);
+    p->rows = query_heads / c->kv_heads * tokens;
+    p->row_tiles = (p->rows + 15) / 16;
+    p->grid = sms * attn_ctas_per_sm(c->head_dim);
+    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    p->out = 0;
+    p->stats = up(static_cast<size_t>(p->grid) * 2 * 16 * ep * 4);
+    p->lse2 = p->stats + up(static_cast<size_t>(p->grid) * 2 * 16 * 8);
+    p->scores = p->lse2 + (weights ? up(static_cast<size_t>(c->batch) * c->kv_heads * p->rows * 4) : 0);
+    p->bytes = p->scores;
+    if (weights && stores_scores(c, p->rows))
+        p->bytes += static_cast<size_t>(c->batch) * c->kv_heads * 16 * c->capacity * 4;
+    return DT_OK;
+}
+
+template <bool E4M3, int EP>
+int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, bool weights, cudaStream_t stream) {
+    using S = AttnShape<EP>;
+    // per device and cheap: the limit belongs to the kernel in the current context
+    cudaError_t e = cudaFuncSetAttribute(k_kv_attend<E4M3, EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
+    const int row_tiles = static_cast<int>(p.row_tiles);
+    k_kv_attend<E4M3, EP><<<p.grid, kAttnThreads, S::kSmem, stream>>>(a, w, row_tiles);
+    int st = check_launch("dt_kv_attention");
+    if (st != DT_OK) return st;
+    unsigned grid = 0;
+    st = grid_of(static_cast<int64_t>(a.batch) * a.kv_heads * row_tiles * 16, "dt_kv_attention", &grid);
+    if (st != DT_OK) return st;
+    k_kv_merge<EP><<<grid, std::max(32, EP / 4), 0, stream>>>(a, w, row_tiles, p.grid);
+    st = check_launch("dt_kv_attention");
+    if (st != DT_OK || !weights) return st;
+    const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
+    if (w.scores != nullptr) {
+        const unsigned y = static_cast<unsigned>(std::min<int64_t>(heads, 32768));
+        const dim3 g(static_cast<unsigned>((a.capacity + 1023) / 1024), y, static_cast<unsigned>((heads + y - 1) / y));
+        k_kv_weights<<<g, 256, 0, stream>>>(a, w);
+    } else {
+        const int key_tiles = static_cast<int>((a.capacity + kTile - 1) / kTile);
+        st = grid_of(heads * key_tiles, "dt_kv_attention", &grid);
+        if (st != DT_OK) return st;
+        k_kv_column_sums<E4M3, EP><<<grid, kAttnThreads, 0, stream>>>(a, w.lse2, row_tiles, key_tiles);
+    }
+    return check_launch("dt_kv_attention");
+}
+
+}  // namespace
+
+extern "C" {
+
+int dt_kv_append(const dt_kv_cache* cache, const void* key, const void* value, int64_t tokens,
+                 const int64_t* key_strides, const int64_t* value_strides, int dtype, const int32_t* lengths,
+                 const int32_t* counts, void* stream) {
+    int st = check_cache(cache, "dt_kv_append");
+    if (st != DT_OK) return st;
+    if (dtype != DT_BFLOAT16 && dtype != DT_FLOAT16)
+        return set_error(DT_ERR_INVALID, "dt_kv_append: keys and values must be bf16 or fp16");
+    if (tokens < 0 || tokens > (int64_t{1} << 30)) return set_error(DT_ERR_INVALID, "dt_kv_append: bad token count");
+    if (cache->batch == 0 || cache->capacity == 0 || tokens == 0) return DT_OK;
+    if (key == nullptr || value == nullptr || key_strides == nullptr || value_strides == nullptr || lengths == nullptr)
+        return set_error(DT_ERR_INVALID, "dt_kv_append: null argument");
+    KvAppendArgs a{};
+    a.codes[0] = static_cast<uint8_t*>(cache->key);
+    a.codes[1] = static_cast<uint8_t*>(cache->value);
+    a.scales[0] = cache->key_scale;
+    a.scales[1] = cache->value_scale;
+    a.src[0] = static_cast<const uint16_t*>(key);
+    a.src[1] = static_cast<const uint16_t*>(value);
+    std::copy_n(key_strides, 3, a.stride[0]);
+    std::copy_n(value_strides, 3, a.stride[1]);
+    a.vec[0] = rows_vectorised(key, key_strides);
+    a.vec[1] = rows_vectorised(value, value_strides);
+    a.lengths = lengths;
+    a.counts = counts;
+    a.capacity = cache->capacity;
+    a.heads = static_cast<int>(cache->kv_heads);
+    a.head_dim = static_cast<int>(cache->head_dim);
+    a.tokens = static_cast<int>(tokens);
+    a.block_shift = log2_of(cache->block);
+    // blocks that `tokens` tokens can touch, wherever the first falls
+    a.spans = static_cast<int>(std::min((tokens + 2 * cache->block - 2) / cache->block, cache->capacity / cache->block));
+    a.bf16 = dtype == DT_BFLOAT16;
+    unsigned grid = 0;
+    st = grid_of(cache->batch * cache->kv_heads * 2 * a.spans, "dt_kv_append", &grid);
+    if (st != DT_OK) return st;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    with_vpt(cache->block, cache->head_dim, [&](auto vpt) {
+        constexpr int V = decltype(vpt)::value;
+        if (cache->code == DT_KV_E4M3) k_kv_append<true, V><<<grid, kAppendThreads, 0, s>>>(a);
+        else k_kv_append<false, V><<<grid, kAppendThreads, 0, s>>>(a);
+    });
+    return check_launch("dt_kv_append");
+}
+
+int dt_kv_read(const dt_kv_cache* cache, const int32_t* lengths, const int32_t* first, int64_t first_all,
+               int64_t count, void* key, void* value, int dtype, void* stream) {
+    int st = check_cache(cache, "dt_kv_read");
+    if (st != DT_OK) return st;
+    if (dtype != DT_FLOAT32 && dtype != DT_BFLOAT16 && dtype != DT_FLOAT16)
+        return set_error(DT_ERR_INVALID, "dt_kv_read: unsupported dtype");
+    if (count < 0 || count > (int64_t{1} << 31)) return set_error(DT_ERR_INVALID, "dt_kv_read: bad token count");
+    if (cache->batch == 0 || count == 0 || (key == nullptr && value == nullptr)) return DT_OK;
+    if (lengths == nullptr) return set_error(DT_ERR_INVALID, "dt_kv_read: null lengths");
+    if (!aligned16(key) || !aligned16(value)) return set_error(DT_ERR_INVALID, "dt_kv_read: outputs must be 16-byte aligned");
+    KvReadArgs a{};
+    a.codes[0] = static_cast<const uint8_t*>(cache->key);
+    a.codes[1] = static_cast<const uint8_t*>(cache->value);
+    a.scales[0] = cache->key_scale;
+    a.scales[1] = cache->value_scale;
+    a.out[0] = key;
+    a.out[1] = value;
+    a.lengths = lengths;
+    a.first = first;
+    a.first_all = first_all;
+    a.count = count;
+    a.capacity = cache->capacity;
+    a.heads = static_cast<int>(cache->kv_heads);
+    a.head_dim = static_cast<int>(cache->head_dim);
+    a.block_shift = log2_of(cache->block);
+    a.dtype = dtype;
+    a.vectors = cache->batch * cache->kv_heads * count * (cache->head_dim / 16);
+    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.vectors + 255) / 256, 148 * 64)), 2);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (cache->code == DT_KV_E4M3) k_kv_read<true><<<grid, 256, 0, s>>>(a);
+    else k_kv_read<false><<<grid, 256, 0, s>>>(a);
+    return check_launch("dt_kv_read");
+}
+
+static int check_queries(const dt_kv_cache* cache, int64_t query_heads, int64_t tokens, const char* who) {
+    int st = check_cache(cache, who);
+    if (st != DT_OK) return st;
+    if (query_heads < cache->kv_heads || query_heads % cache->kv_heads != 0)
+        return set_error(DT_ERR_INVALID, std::string(who) + ": query heads must be a multiple of the key heads");
+    if (tokens < 0 || tokens > (int64_t{1} << 30) || query_heads > (int64_t{1} << 20) ||
+        query_heads / cache->kv_heads * tokens > (int64_t{1} << 30))
+        return set_error(DT_ERR_INVALID, std::string(who) + ": too many queries");
+    return DT_OK;
+}
+
+int dt_kv_attention_workspace(const dt_kv_cache* cache, int64_t query_heads, int64_t tokens, int with_weights,
+                              size_t* bytes) {
+    int st = check_queries(cache, query_heads, tokens, "dt_kv_attention_workspace");
+    if (st != DT_OK) return st;
+    if (bytes == nullptr) return set_error(DT_ERR_INVALID, "dt_kv_attention_workspace: null bytes");
+    *bytes = 0;
+    if (cache->batch == 0 || tokens == 0) return DT_OK;
+    AttnPlan p{};
+    st = attn_plan(cache, query_heads, tokens, with_weights != 0, &p);
+    if (st == DT_OK) *bytes = p.bytes;
+    return st;
+}
+
+int dt_kv_attention(const dt_kv_cache* cache, const void* query, int64_t query_heads, int64_t tokens,
+                    const int64_t* query_strides, int dtype, const int32_t* lengths, const int32_t* counts,
+                    float scale, int flags, void* out, float* lse, float* weights, void* workspace,
+                    size_t workspace_bytes, void* stream) {
+    int st = check_queries(cache, query_heads, tokens, "dt_kv_attention");
+    if (st != DT_OK) return st;
+    if (dtype != DT_BFLOAT16 && dtype != DT_FLOAT16)
+        return set_error(DT_ERR_INVALID, "dt_kv_attention: queries must be bf16 or fp16");
+    if ((flags & ~(DT_KV_CAUSAL | DT_KV_ACCUMULATE)) != 0) return set_error(DT_ERR_INVALID, "dt_kv_attention: unknown flag");
+    if (!std::isfinite(scale)) return set_error(DT_ERR_INVALID, "dt_kv_attention: scale must be finite");
+    if (cache->batch == 0 || tokens == 0) return DT_OK;
+    if (query == nullptr || query_strides == nullptr || lengths == nullptr || out == nullptr)
+        return set_error(DT_ERR_INVALID, "dt_kv_attention: null argument");
+    if ((reinterpret_cast<uintptr_t>(out) & 15) != 0 || !aligned16(workspace))
+        return set_error(DT_ERR_INVALID, "dt_kv_attention: out and workspace must be 16-byte aligned");
+    AttnPlan p{};
+    st = attn_plan(cache, query_heads, tokens, weights != nullptr, &p);
+    if (st != DT_OK) return st;
+    if (workspace == nullptr || workspace_bytes < p.bytes)
+        return set_error(DT_ERR_INVALID, "dt_kv_attention: workspace too small (dt_kv_attention_workspace)");
+    KvAttnArgs a{};
+    a.key = static_cast<const uint8_t*>(cache->key);
+    a.value = static_cast<const uint8_t*>(cache->value);
+    a.key_scale = cache->key_scale;
+    a.value_scale = cache->value_scale;
+    a.query = query;
+    a.lengths = lengths;
+    a.counts = counts;
+    a.out = out;
+    a.lse = lse;
+    a.weights = weights;
+    a.q_stride_n = query_strides[0];
+    a.q_stride_h = query_strides[1];
+    a.q_stride_t = query_strides[2];
+    a.batch = static_cast<int>(cache->batch);
+    a.kv_heads = static_cast<int>(cache->kv_heads);
+    a.head_dim = static_cast<int>(cache->head_dim);
+    a.group = static_cast<int>(query_heads / cache->kv_heads);
+    a.tokens = static_cast<int>(tokens);
+    a.rows = static_cast<int>(p.rows);
+    a.capacity = cache->capacity;
+    a.block_shift = log2_of(cache->block);
+    a.nblocks = static_cast<int>(cache->capacity >> a.block_shift);
+    a.scale_log2 = scale * kLog2e;
+    a.causal = (flags & DT_KV_CAUSAL) != 0;
+    a.query_bf16 = dtype == DT_BFLOAT16;
+    a.accumulate = (flags & DT_KV_ACCUMULATE) != 0;
+    a.q_vec = rows_vectorised(query, query_strides);
+    char* ws = static_cast<char*>(workspace);
+    KvPartials w{};
+    w.out = reinterpret_cast<float*>(ws + p.out);
+    w.stats = reinterpret_cast<float2*>(ws + p.stats);
+    w.lse2 = weights != nullptr ? reinterpret_cast<float*>(ws + p.lse2) : nullptr;
+    w.scores = p.bytes > p.scores ? reinterpret_cast<float*>(ws + p.scores) : nullptr;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    return with_head_dim(cache->head_dim, [&](auto ep) {
+        constexpr int EP = decltype(ep)::value;
+        return cache->code == DT_KV_E4M3 ? launch_attend<true, EP>(a, w, p, weights != nullptr, s)
+                                         : launch_attend<false, EP>(a, w, p, weights != nullptr, s);
+    });
+}
+
+int dt_kv_evict_workspace(const dt_kv_cache* src, int64_t budget, size_t* bytes) {
+    int st = check_cache(src, "dt_kv_evict_workspace");
+    if (st != DT_OK) return st;
+    if (bytes == nullptr || budget < 0 || budget > (int64_t{1} << 30))
+        return set_error(DT_ERR_INVALID, "dt_kv_evict_workspace: bad argument");
+    *bytes = static_cast<size_t>(src->batch) * src->kv_heads * budget * 4;
+    return DT_OK;
+}
+
+static bool overlap(const void* p, size_t np, const void* q, size_t nq) {
+    const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+    return a < b + nq && b < a + np;
+}
+
+int dt_kv_evict(const dt_kv_cache* src, const dt_kv_cache* dst, const int32_t* lengths, const float* weights,
+                int64_t budget, int64_t recent, int32_t* dst_lengths, float* dst_weights, int32_t* kept,
+                void* workspace, size_t workspace_bytes, void* stream) {
+    int st = check_cache(src, "dt_kv_evict");
+    if (st == DT_OK) st = check_cache(dst, "dt_kv_evict");
+    if (st != DT_OK) return st;
+    if (src->batch != dst->batch || src->kv_heads != dst->kv_heads || src->head_dim != dst->head_dim ||
+        src->block != dst->block || src->code != dst->code)
+        return set_error(DT_ERR_INVALID, "dt_kv_evict: the caches differ in batch, heads, head_dim, block or code");
+    if (budget < 0 || budget > dst->capacity) return set_error(DT_ERR_INVALID, "dt_kv_evict: budget exceeds dst's capacity");
+    if (recent < 0 || recent > budget) return set_error(DT_ERR_INVALID, "dt_kv_evict: recent must be 0..budget");
+    if (src->batch == 0) return DT_OK;
+    if (lengths == nullptr || weights == nullptr || dst_lengths == nullptr)
+        return set_error(DT_ERR_INVALID, "dt_kv_evict: null argument");
+    const size_t heads = static_cast<size_t>(src->batch) * src->kv_heads;
+    const void* const in[4] = {src->key, src->value, src->key_scale, src->value_scale};
+    const void* const to[4] = {dst->key, dst->value, dst->key_scale, dst->value_scale};
+    for (int i = 0; i < 4; ++i)
+        for (int j = 0; j < 4; ++j) {
+            const size_t unit_i = i < 2 ? src->head_dim * src->block : 4, unit_j = j < 2 ? dst->head_dim * dst->block : 4;
+            if (overlap(in[i], heads * (src->capacity / src->block) * unit_i, to[j],
+                        heads * (dst->capacity / dst->block) * unit_j))
+                return set_error(DT_ERR_INVALID, "dt_kv_evict: src and dst overlap");
+        }
+    const size_t n_src = heads * src->capacity * 4, n_dst = heads * dst->capacity * 4, n_len = src->batch * 4;
+    if (overlap(lengths, n_len, dst_lengths, n_len) || (dst_weights != nullptr && overlap(weights, n_src, dst_weights, n_dst)))
+        return set_error(DT_ERR_INVALID, "dt_kv_evict: lengths or weights overlap their outputs");
+    if (kept == nullptr && budget > 0) {
+        if (workspace == nullptr || workspace_bytes < heads * budget * 4)
+            return set_error(DT_ERR_INVALID, "dt_kv_evict: workspace too small (dt_kv_evict_workspace)");
+        kept = static_cast<int32_t*>(workspace);
+    }
+    KvEvictArgs a{};
+    a.src[0] = static_cast<const uint8_t*>(src->key);
+    a.src[1] = static_cast<const uint8_t*>(src->value);
+    a.src_scale[0] = src->key_scale;
+    a.src_scale[1] = src->value_scale;
+    a.dst[0] = static_cast<uint8_t*>(dst->key);
+    a.dst[1] = static_cast<uint8_t*>(dst->value);
+    a.dst_scale[0] = dst->key_scale;
+    a.dst_scale[1] = dst->value_scale;
+    a.lengths = lengths;
+    a.weights = weights;
+    a.kept = kept;
+    a.dst_lengths = dst_lengths;
+    a.dst_weights = dst_weights;
+    a.src_cap = src->capacity;
+    a.dst_cap = dst->capacity;
+    a.batch = static_cast<int>(src->batch);
+    a.heads = static_cast<int>(src->kv_heads);
+    a.head_dim = static_cast<int>(src->head_dim);
+    a.block_shift = log2_of(src->block);
+    a.budget = static_cast<int>(budget);
+    a.recent = static_cast<int>(recent);
+    a.spans = static_cast<int>((budget + src->block - 1) / src->block);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    unsigned grid = 0;
+    st = grid_of(static_cast<int64_t>(heads) * 2 * a.spans, "dt_kv_evict", &grid);
+    if (st != DT_OK) return st;
+    k_kv_select<<<static_cast<unsigned>(heads), kSelectThreads, 0, s>>>(a);
+    st = check_launch("dt_kv_evict");
+    if (st != DT_OK) return st;
+    if (grid > 0) {
+        with_vpt(src->block, src->head_dim, [&](auto vpt) {
+            constexpr int V = decltype(vpt)::value;
+            if (src->code == DT_KV_E4M3) k_kv_gather<true, V><<<grid, kAppendThreads, 0, s>>>(a);
+            else k_kv_gather<false, V><<<grid, kAppendThreads, 0, s>>>(a);
+        });
+        st = check_launch("dt_kv_evict");
+        if (st != DT_OK) return st;
+    }
+    const int64_t written = static_cast<int64_t>(a.spans) * src->block;
+    if (dst_weights != nullptr && written < dst->capacity) {
+        const int64_t tail = static_cast<int64_t>(heads) * (dst->capacity - written);
+        k_kv_zero_tail<<<static_cast<unsigned>(std::min<int64_t>((tail + 255) / 256, 148 * 16)), 256, 0, s>>>(
+            dst_weights, static_cast<int64_t>(heads), dst->capacity, written);
+        st = check_launch("dt_kv_evict");
+    }
+    return st;
+}
+
+}  // extern "C"

@@ -1,0 +1,128 @@
+// Device helpers of the 8-bit key/value cache (dt_kv.cu, dt_kv_prompt.cu).
+#pragma once
+
+#include <cstdint>
+
+#include <cuda_bf16.h>
+#include <cuda_fp16.h>
+#include <cuda_fp8.h>
+#include <cuda_runtime.h>
+
+#include "../../include/dtorch_b200.h"
+
+namespace dtb {
+
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLn2 = 0.6931471805599453f;
+
+// What the attention kernels read. Query row r of key head h is query r / group of the sequence and query head
+// h * group + r % group: rows in the order of the tokens, so the rows of a tile see nearly the same tokens.
+struct KvAttnArgs {
+    const uint8_t* key;
+    const uint8_t* value;
+    const float* key_scale;
+    const float* value_scale;
+    const void* query;
+    const int32_t* lengths;
+    const int32_t* counts;
+    void* out;
+    float* lse;
+    float* weights;
+    int64_t q_stride_n, q_stride_h, q_stride_t;
+    int batch, kv_heads, head_dim, group, tokens, rows;  // rows = group * tokens
+    int64_t capacity;
+    int block_shift;   // log2(tokens that share a scale)
+    int nblocks;       // capacity >> block_shift
+    float scale_log2;  // softmax scale * log2(e)
+    int causal;
+    int query_bf16;
+    int accumulate;
+    int q_vec;  // query rows can be read 16 bytes at a time
+};
+
+__device__ __forceinline__ int kv_length(const int32_t* lengths, int n, int64_t capacity) {
+    const int l = lengths[n];
+    return l < 0 ? 0 : (l > capacity ? static_cast<int>(capacity) : l);
+}
+
+__device__ __forceinline__ int kv_count(const int32_t* counts, int n, int tokens) {
+    if (counts == nullptr) return tokens;
+    const int c = counts[n];
+    return c < 0 ? 0 : (c > tokens ? tokens : c);
+}
+
+// How many tokens, from the first, query row `row` of a sequence sees.
+__device__ __forceinline__ int kv_limit(const KvAttnArgs& a, int row, int len, int cnt) {
+    const int t = row / a.group;
+    if (row >= a.rows || t >= cnt) return 0;
+    const int lim = a.causal ? len - cnt + t + 1 : len;
+    return lim < 0 ? 0 : lim;
+}
+
+__device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
+    uint32_t d;
+    asm("prmt.b32 %0, %1, %2, %3;" : "=r"(d) : "r"(a), "r"(b), "r"(sel));
+    return d;
+}
+
+__device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("sub.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+
+// Four codes of a word to two fp16 pairs; every code is exact in fp16. SPLIT 0: pairs (0,1) and (2,3); SPLIT 1: pairs
+// (0,2) and (1,3), the byte transposition that rows read through ldmatrix.trans need, at no further cost.
+// int8: 1024 + (code + 128) is the fp16 whose low byte is code + 128; subtracting 1152 leaves the code.
+// e4m3: exponent and mantissa land in fp16's fields when shifted by one, which gives code / 256 (fp16's bias is 15,
+// e4m3's 7; subnormals included); the factor 256 is left to the scale (code_unit). 0x7f (NaN) never occurs below a
+// sequence's length: the writers saturate and mark NaN in the scale.
+template <bool E4M3, int SPLIT>
+__device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    if constexpr (E4M3) {
+        const uint32_t a = prmt(w, 0u, SPLIT ? 0x2404 : 0x1404);  // bytes to the high halves of the fp16 pair
+        const uint32_t b = prmt(w, 0u, SPLIT ? 0x3414 : 0x3424);
+        lo = (a & 0x80008000u) | ((a >> 1) & 0x3f803f80u);
+        hi = (b & 0x80008000u) | ((b >> 1) & 0x3f803f80u);
+    } else {
+        const uint32_t u = w ^ 0x80808080u;
+        lo = hsub2(prmt(u, 0x64646464u, SPLIT ? 0x4240 : 0x4140), 0x64806480u);
+        hi = hsub2(prmt(u, 0x64646464u, SPLIT ? 0x4341 : 0x4342), 0x64806480u);
+    }
+}
+
+// What the fp16 values of codes_to_half are short of.
+template <bool E4M3>
+__device__ __forceinline__ constexpr float code_unit() {
+    return E4M3 ? 256.0f : 1.0f;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    uint32_t d;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+    return d;
+}
+
+// Two 16-bit floats of a word as fp32.
+__device__ __forceinline__ float2 unpack16(uint32_t w, bool bf16) {
+    if (bf16) return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Power of two that brings a row whose largest |element| is `amax` into fp16's range, and its inverse. bf16 and fp16
+// elements stay exact above 2^-38 of the row's largest, below that the error is under 2^-39 of it: the products are
+// those of the model's type, and one fp16 path serves both types.
+__device__ __forceinline__ void row_power(float amax, float& mul, float& inv) {
+    int ex = static_cast<int>(__float_as_uint(amax) >> 23) - 127;
+    ex = ex < -100 ? -100 : ex;
+    mul = __uint_as_float(static_cast<uint32_t>(127 + 13 - ex) << 23);
+    inv = __uint_as_float(static_cast<uint32_t>(127 - 13 + ex) << 23);
+}
+
+}  // namespace dtb

@@ -2,6 +2,7 @@
 // threads or on the GPU releases the GIL.
 #include <torch/extension.h>
 
+#include "kv_cache.h"
 #include "placement.h"
 #include "redistribute.h"
 #include "thread_group.h"
@@ -131,6 +132,45 @@ PYBIND11_MODULE(_host, m) {
         auto& ks = KernelStreamManager::Global().Get(globalDeviceId);
         return py::make_tuple(reinterpret_cast<uintptr_t>(ks.Stream().stream()), ks.CudaDevice());
     }, "(cudaStream_t as int, CUDA device) of the kernel stream the executor runs a device's collectives on");
+
+    // argument errors of the cache's operators under Python's own names
+    py::register_local_exception_translator([](std::exception_ptr p) {
+        try {
+            if (p) std::rethrow_exception(p);
+        } catch (const c10::ValueError& e) {
+            PyErr_SetString(PyExc_ValueError, e.what_without_backtrace());
+        } catch (const c10::TypeError& e) {
+            PyErr_SetString(PyExc_TypeError, e.what_without_backtrace());
+        }
+    });
+    py::class_<QuantizedKVCache>(m, "QuantizedKVCache")
+        .def(py::init<torch::Tensor, torch::Tensor, torch::Tensor, torch::Tensor>())
+        .def_static("empty",
+                    [](int64_t batch, int64_t kvHeads, int64_t capacity, int64_t headDim, py::object dtype, int64_t block,
+                       py::object device) {
+                        return QuantizedKVCache::Empty(batch, kvHeads, capacity, headDim,
+                                                       torch::python::detail::py_object_to_dtype(dtype), block,
+                                                       torch::python::detail::py_object_to_device(device));
+                    })
+        .def_readonly("key", &QuantizedKVCache::key)
+        .def_readonly("value", &QuantizedKVCache::value)
+        .def_readonly("key_scale", &QuantizedKVCache::keyScale)
+        .def_readonly("value_scale", &QuantizedKVCache::valueScale)
+        .def_property_readonly("batch", [](const QuantizedKVCache& c) { return c.abi.batch; })
+        .def_property_readonly("kv_heads", [](const QuantizedKVCache& c) { return c.abi.kv_heads; })
+        .def_property_readonly("capacity", [](const QuantizedKVCache& c) { return c.abi.capacity; })
+        .def_property_readonly("head_dim", [](const QuantizedKVCache& c) { return c.abi.head_dim; })
+        .def_property_readonly("block", [](const QuantizedKVCache& c) { return c.abi.block; });
+    m.def("kv_cache_append", &KVCacheAppend, py::call_guard<py::gil_scoped_release>());
+    m.def("kv_cache_read",
+          [](const QuantizedKVCache& c, const torch::Tensor& lengths, const std::optional<torch::Tensor>& first,
+             int64_t firstAll, int64_t count, py::object dtype) {
+              const auto st = torch::python::detail::py_object_to_dtype(dtype);
+              py::gil_scoped_release nogil;
+              return KVCacheRead(c, lengths, first, firstAll, count, st);
+          });
+    m.def("kv_cache_attention", &KVCacheAttention, py::call_guard<py::gil_scoped_release>());
+    m.def("kv_cache_evict", &KVCacheEvict, py::call_guard<py::gil_scoped_release>());
 
     // placement algebra (host logic; testable without a GPU)
     m.def("shard_sizes", &ShardSizes);

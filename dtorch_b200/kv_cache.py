@@ -1,0 +1,118 @@
+"""Keys and values of decoder attention held in 8 bits, and the operators that write, read, attend to and evict them.
+
+The cache is (N, H, capacity, E) codes, int8 or float8_e4m3fn, with one float32 scale for `block` consecutive tokens
+of a head: a value is code * scale. A scale is the largest |value| of its block / 127 (int8) or / 448 (e4m3), rounded
+up to the next bfloat16; a code is the exact quotient to nearest, ties to even. A block that a non-finite value
+enters reads as NaN.
+
+A cache is storage only. How many tokens each sequence holds is the caller's int32 tensor `lengths` (N,), on the cache's
+device, and the operators read it there: nothing is copied to the host, and a decode step can be captured in a CUDA
+graph and replayed while the lengths grow::
+
+    cache = QuantizedKVCache(batch, kv_heads, capacity, head_dim, dtype=torch.int8, block=64, device="cuda")
+    kv_cache_append(cache, k, v, lengths)             # behind what the sequences hold
+    lengths += k.shape[2]
+    out = kv_cache_attention(q, cache, lengths, weights=seen)   # q: the last tokens; seen: what each token got, added up
+    cache, lengths, seen, _ = kv_cache_evict(cache, lengths, seen, budget=4096, recent=512)
+
+Lengths below 0 count as 0 and those above the capacity as the capacity; slots behind a length are never read. The
+operators run on the current stream of the cache's device, whichever device is current. There is no backward pass.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional, Tuple, Union
+
+import torch
+
+from . import _host
+
+
+class QuantizedKVCache:
+    """An 8-bit key/value cache of `batch` sequences, zero-filled. `capacity`, in tokens, is a multiple of `block` (32, 64
+    or 128 tokens that share a scale); `head_dim` a multiple of 16 up to 256; `dtype` torch.int8 or
+    torch.float8_e4m3fn. Attributes: key, value, key_scale, value_scale (the tensors), batch, kv_heads, capacity,
+    head_dim, block, dtype, device."""
+
+    __slots__ = ("_c", "key", "value", "key_scale", "value_scale", "batch", "kv_heads", "capacity", "head_dim", "block",
+                 "dtype", "device")
+
+    def __init__(self, batch: int, kv_heads: int, capacity: int, head_dim: int, dtype: torch.dtype = torch.int8,
+                 block: int = 64, device: Union[str, torch.device] = "cuda"):
+        self._adopt(_host.QuantizedKVCache.empty(batch, kv_heads, capacity, head_dim, dtype, block, torch.device(device)))
+
+    @classmethod
+    def from_tensors(cls, key: torch.Tensor, value: torch.Tensor, key_scale: torch.Tensor,
+                     value_scale: torch.Tensor) -> "QuantizedKVCache":
+        """A cache over existing contiguous tensors, which it shares: codes (N, H, capacity, E) and scales
+        (N, H, capacity / block). Codes are taken as the operators write them (no float8 NaN below a length)."""
+        c = cls.__new__(cls)
+        c._adopt(_host.QuantizedKVCache(key, value, key_scale, value_scale))
+        return c
+
+    def _adopt(self, c) -> None:
+        self._c = c
+        for name in ("key", "value", "key_scale", "value_scale", "batch", "kv_heads", "capacity", "head_dim", "block"):
+            setattr(self, name, getattr(c, name))
+        self.dtype, self.device = self.key.dtype, self.key.device
+
+    def __repr__(self) -> str:
+        return (f"QuantizedKVCache(batch={self.batch}, kv_heads={self.kv_heads}, capacity={self.capacity}, "
+                f"head_dim={self.head_dim}, dtype={self.dtype}, block={self.block}, device={str(self.device)!r})")
+
+
+def kv_cache_append(cache: QuantizedKVCache, key: torch.Tensor, value: torch.Tensor, lengths: torch.Tensor,
+                    counts: Optional[torch.Tensor] = None) -> None:
+    """Write new keys and values (N, H, T, E), bfloat16 or float16, behind the lengths[n] tokens that each sequence holds
+    (the first counts[n] <= T of them where `counts` is given: a padded batch). The scale of a block that is still
+    filling grows with its tokens; when it does, the codes of its earlier tokens are rounded again to the new scale.
+    Tokens that would fall behind the capacity are not written. `lengths` is left to the caller, who advances it."""
+    _host.kv_cache_append(cache._c, key, value, lengths, counts)
+
+
+def kv_cache_read(cache: QuantizedKVCache, lengths: torch.Tensor, first: Union[int, torch.Tensor] = 0,
+                  count: Optional[int] = None, dtype: torch.dtype = torch.bfloat16) -> Tuple[torch.Tensor, torch.Tensor]:
+    """(key, value) of the tokens first .. first + count of every sequence as values, (N, H, count, E); zeros outside
+    0 .. lengths[n]. `first` is a number or an int32 tensor (N,); `count` defaults to the rest of the capacity (for a
+    tensor `first`: to the capacity). float32 is exact, bfloat16 and float16 are rounded once."""
+    if isinstance(first, torch.Tensor):
+        return _host.kv_cache_read(cache._c, lengths, first, 0, cache.capacity if count is None else count, dtype)
+    if first < 0:
+        raise ValueError("kv_cache_read: first must not be negative")
+    if count is None:
+        count = max(cache.capacity - first, 0)
+    return _host.kv_cache_read(cache._c, lengths, None, first, count, dtype)
+
+
+def kv_cache_attention(query: torch.Tensor, cache: QuantizedKVCache, lengths: torch.Tensor,
+                       counts: Optional[torch.Tensor] = None, is_causal: bool = True, scale: Optional[float] = None,
+                       weights: Optional[torch.Tensor] = None, accumulate: bool = True, return_lse: bool = False):
+    """Softmax attention of query (N, Hq, T, E), bfloat16 or float16, over the lengths[n] cached tokens of each sequence:
+    (N, Hq, T, E) in query's type. Hq is a multiple of the cache's heads, and head j reads key head
+    j // (Hq // H). The queries are the last T (counts[n] where `counts` is given) of the lengths[n] tokens, which
+    were appended before: with `is_causal` query i sees the first lengths[n] - T + i + 1. Queries that see nothing, and
+    those behind counts[n], give zeros. `scale` defaults to 1 / sqrt(E).
+
+    `weights`, a float32 tensor (N, H, capacity), takes the sum of each cached token's softmax weights over the
+    queries and the query heads of its key head, for the tokens below lengths[n] (what kv_cache_evict goes by): added,
+    or written where `accumulate` is False. A slot that a new token takes keeps what it had: set it to 0 first, or
+    start from zeros. With `return_lse` also the log-sum-exp of the scaled scores, float32 (N, Hq, T), -inf for a
+    query that sees nothing. The same inputs give the same bits."""
+    s = 1.0 / math.sqrt(cache.head_dim) if scale is None else scale
+    out, lse = _host.kv_cache_attention(query, cache._c, lengths, counts, is_causal, s, weights, accumulate, return_lse)
+    return (out, lse) if return_lse else out
+
+
+def kv_cache_evict(cache: QuantizedKVCache, lengths: torch.Tensor, weights: torch.Tensor, budget: int, recent: int = 0,
+                   out: Optional[QuantizedKVCache] = None):
+    """Cut every sequence back to at most `budget` tokens: in each head the last `recent` stay, and of the others those
+    with the largest `weights` (N, H, capacity), ties to the lowest position; they keep their order. The kept tokens go
+    to the front of `out`, a cache that shares no memory with `cache` (default: a new one of the budget rounded up to
+    blocks), in blocks that are scaled anew. Returns (out, lengths, weights, kept): the new cache's lengths (N,) and
+    weights (N, H, out.capacity), 0 behind the kept tokens, and the kept positions (N, H, budget), -1 behind the last."""
+    if out is None:
+        most = max(-(-budget // cache.block), 1) * cache.block
+        out = QuantizedKVCache(cache.batch, cache.kv_heads, most, cache.head_dim, cache.dtype, cache.block, cache.device)
+    new_lengths, new_weights, kept = _host.kv_cache_evict(cache._c, lengths, weights, budget, recent, out._c)
+    return out, new_lengths, new_weights, kept

@@ -302,6 +302,95 @@ int dt_local_all_gather(int n, const void* const* ins, void* out, size_t outer, 
 int dt_local_all_to_all(int n, const void* const* ins, void* const* outs, int ndim, const int64_t* in_shape,
                         int src_dim, int dst_dim, const int64_t* src_lens, size_t elem_bytes, void* stream);
 
+/* ---- 8-bit key/value cache ------------------------------------------------------------------------------- */
+/* Keys and values of decoder attention held in 8 bits, and the attention that reads them: what a serving program
+ * keeps next to the context-parallel attention (each device holds its heads after the Ulysses swap). No counterpart
+ * in the reference, whose caches hold the model's own type.
+ *
+ * Layout: key and value are (batch, kv_heads, capacity, head_dim) codes, contiguous, 16-byte aligned; key_scale and
+ * value_scale are (batch, kv_heads, capacity / block) fp32, one scale for `block` consecutive tokens of a head. A
+ * value is code * scale. A block's scale is the largest |value| of its tokens / 127 (int8) or / 448 (e4m3), rounded
+ * up to the next bfloat16, so code * scale needs at most 15 bits and every rounding of a code is exactly defined: to
+ * nearest, ties to even, of the exact quotient. A block that a non-finite value enters has the scale NaN and reads as
+ * NaN.
+ *
+ * All entry points run on the current device and stream, allocate nothing, and can be captured in a CUDA graph.
+ * `lengths`, `counts` and `first` are device arrays of `batch` int32. Lengths are taken as 0 where they are negative
+ * and as the capacity where they are larger. Slots behind a sequence's length are never read as values: they may
+ * hold anything. head_dim: a multiple of 16, up to 256; block: 32, 64 or 128; capacity: a multiple of block. */
+
+typedef enum dt_kv_code {
+    DT_KV_INT8 = 0, /* -127..127 */
+    DT_KV_E4M3 = 1  /* 4 exponent and 3 mantissa bits, no infinities, up to 448 */
+} dt_kv_code;
+
+#define DT_KV_CAUSAL 0x1     /* query i of a sequence sees the tokens up to its own */
+#define DT_KV_ACCUMULATE 0x2 /* add to `weights` instead of writing them */
+
+typedef struct dt_kv_cache {
+    void* key;
+    void* value;
+    float* key_scale;
+    float* value_scale;
+    int64_t batch;
+    int64_t kv_heads;
+    int64_t capacity; /* tokens a sequence can hold */
+    int64_t head_dim;
+    int64_t block; /* tokens that share a scale */
+    int code;      /* dt_kv_code */
+} dt_kv_cache;
+
+/* Write `tokens` new tokens of every sequence behind the lengths[n] tokens that it holds (counts[n] of them where
+ * counts is not NULL). key and value are (batch, kv_heads, tokens, head_dim) in `dtype` (DT_BFLOAT16, DT_FLOAT16),
+ * the last dimension contiguous, the strides of the others in elements in key_strides / value_strides (3 each). The
+ * scale of a block that is filling grows with the new tokens and never shrinks; when it grows, the codes of the
+ * block's earlier tokens are rounded again to the new scale. Tokens that would fall behind the capacity are not
+ * written. `lengths` is not changed: the caller advances it. */
+int dt_kv_append(const dt_kv_cache* cache, const void* key, const void* value, int64_t tokens,
+                 const int64_t* key_strides, const int64_t* value_strides, int dtype, const int32_t* lengths,
+                 const int32_t* counts, void* stream);
+
+/* key and value of the tokens [first[n], first[n] + count) of every sequence (first_all for all where first is NULL)
+ * as (batch, kv_heads, count, head_dim) in `dtype` (fp32 is exact, the others are rounded once), zeros outside
+ * [0, lengths[n]). Either output may be NULL. */
+int dt_kv_read(const dt_kv_cache* cache, const int32_t* lengths, const int32_t* first, int64_t first_all,
+               int64_t count, void* key, void* value, int dtype, void* stream);
+
+/* Bytes of workspace dt_kv_attention needs for these arguments on the current device (with_weights: weights are
+ * asked for). 16-byte aligned; two calls that may run at the same time need a workspace each. */
+int dt_kv_attention_workspace(const dt_kv_cache* cache, int64_t query_heads, int64_t tokens, int with_weights,
+                              size_t* bytes);
+
+/* Softmax attention of `tokens` queries of every sequence over its lengths[n] cached tokens. query is (batch,
+ * query_heads, tokens, head_dim) in `dtype` (DT_BFLOAT16, DT_FLOAT16), the last dimension contiguous, other strides
+ * in elements in query_strides (3); query_heads is a multiple of kv_heads, and head j reads key head j / (query_heads /
+ * kv_heads). out is (batch, query_heads, tokens, head_dim) in the same type, contiguous. The queries are the last
+ * counts[n] (tokens where counts is NULL) of the lengths[n] tokens: with DT_KV_CAUSAL query i sees the first
+ * lengths[n] - counts[n] + i + 1 of them. A query that sees nothing, and queries behind counts[n], give 0 and a
+ * log-sum-exp of -infinity. lse (NULL: not wanted) is (batch, query_heads, tokens) fp32, natural logarithm, of the
+ * scaled scores. weights (NULL: not wanted) is (batch, kv_heads, capacity) fp32: the sum of each cached token's
+ * softmax weights over the queries and the query heads of its key head, written (DT_KV_ACCUMULATE: added) for the
+ * tokens below lengths[n]; slots behind are left as they were. Sums are fp32 in a fixed order: the same inputs give
+ * the same bits. */
+int dt_kv_attention(const dt_kv_cache* cache, const void* query, int64_t query_heads, int64_t tokens,
+                    const int64_t* query_strides, int dtype, const int32_t* lengths, const int32_t* counts,
+                    float scale, int flags, void* out, float* lse, float* weights, void* workspace,
+                    size_t workspace_bytes, void* stream);
+
+/* Bytes of workspace dt_kv_evict needs. */
+int dt_kv_evict_workspace(const dt_kv_cache* src, int64_t budget, size_t* bytes);
+
+/* Copy at most `budget` tokens of every head of src to the front of dst (another cache of the same batch, heads,
+ * head_dim, block and code whose memory does not overlap src's): the last `recent` (<= budget) of its lengths[n]
+ * tokens and, of the others, those with the largest weights (ties: the lowest position; NaN counts as the largest),
+ * in their order. Blocks of dst get scales of their own; the slots behind the last kept token of a block become 0.
+ * weights is (batch, kv_heads, src capacity), dst_weights (NULL: not wanted) (batch, kv_heads, dst capacity): the kept
+ * tokens' weights, 0 behind. dst_lengths[n] = min(lengths[n], budget). kept (NULL: not wanted) is (batch, kv_heads,
+ * budget) int32: positions in src, -1 behind the last. */
+int dt_kv_evict(const dt_kv_cache* src, const dt_kv_cache* dst, const int32_t* lengths, const float* weights,
+                int64_t budget, int64_t recent, int32_t* dst_lengths, float* dst_weights, int32_t* kept,
+                void* workspace, size_t workspace_bytes, void* stream);
+
 /* ---- instrumentation -------------------------------------------------------------------------------------- */
 
 /* Number of kernels this library has launched on the calling process since load (all threads). */
