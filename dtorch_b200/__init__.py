@@ -16,7 +16,8 @@ _DTENSOR_NAMES = ("DeviceMesh", "Placement", "Shard", "Replicate", "Partial", "i
                   "get_placements_from_dict",
                   "cuda_device_of", "clear", "redistribute_many", "reduce", "set_pool_bytes")
 
-_KV_CACHE_NAMES = ("QuantizedKVCache", "kv_cache_append", "kv_cache_read", "kv_cache_attention", "kv_cache_evict")
+_KV_CACHE_NAMES = ("QuantizedKVCache", "kv_cache_append", "kv_cache_read", "kv_cache_attention", "kv_cache_evict",
+                   "DistributedKVCache")
 
 
 def __getattr__(name):

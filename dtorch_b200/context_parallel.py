@@ -26,6 +26,11 @@ devices' chunks, and merges the partial outputs by their log-sum-exp (softmax ov
 The result equals the one-pass attention up to floating-point rounding. It is off by default: on B200 the
 split (attention kernels that also return the log-sum-exp, the fp32 merge, more launches) cost more than the
 all-gather it hides at every shape measured (2 GPUs, bf16, sequence 1K-16K, 16-64 heads).
+
+`kv_cache`, a DistributedKVCache, makes the call a step of decoding: key and value are the new tokens', which are
+appended to the cache in 8 bits, and the queries, the last tokens, attend over all that it holds, each device for its
+heads. A prompt comes sequence-sharded (Shard(2) along the Ulysses dim) and takes the fused swap to the cache's
+Shard(1) and back; single tokens come head-sharded already and need no swap.
 """
 
 from __future__ import annotations
@@ -36,6 +41,7 @@ import torch
 import torch.nn.functional as F
 
 from .dtensor import DTensor, Replicate, Shard, _host, redistribute_many
+from .kv_cache import DistributedKVCache
 
 
 def _dim_index(tensor: DTensor, dim: Optional[Union[int, str]]) -> Optional[int]:
@@ -187,12 +193,31 @@ def _ulysses_overlapped(query: DTensor, key: DTensor, value: DTensor, u: int, gr
     return DTensor(out_locals, mesh, seq, tuple(query.shape[:3]) + (value.shape[3],))
 
 
+def _attention_with_cache(query: DTensor, key: DTensor, value: DTensor, kv_cache: DistributedKVCache, u: Optional[int],
+                          is_causal: bool, scale: Optional[float]) -> DTensor:
+    placements = list(query.placements)
+    swap = u is not None and placements[u] == Shard(2)
+    if swap:
+        head = list(placements)
+        head[u] = Shard(1)
+        if query.shape == key.shape == value.shape:
+            query, key, value = redistribute_many([query, key, value], head)
+        else:
+            query = query.redistribute(placements=head)
+            key, value = redistribute_many([key, value], head)
+    kv_cache.append(key, value)
+    out = kv_cache.attend(query, is_causal=is_causal, scale=scale)
+    return out.redistribute(placements=placements) if swap else out
+
+
 def scaled_dot_product_attention_with_cp(query: DTensor, key: DTensor, value: DTensor, dropout_p: float = 0.0,
                                          is_causal: bool = False, scale: Optional[float] = None,
                                          ulysses_cp_dim: Optional[Union[int, str]] = None,
                                          ring_cp_dim: Optional[Union[int, str]] = None,
-                                         ring_overlap: bool = False, ulysses_overlap_groups: int = 1) -> DTensor:
-    """`ulysses_overlap_groups` > 1 pipelines a pure-Ulysses call over that many head groups (batch 1, q/k/v of
+                                         ring_overlap: bool = False, ulysses_overlap_groups: int = 1,
+                                         kv_cache: Optional[DistributedKVCache] = None) -> DTensor:
+    """With `kv_cache` the new keys and values are appended to it and the queries attend over what it then holds, with
+    `is_causal` each up to its own token; no dropout, ring dim or overlap. `ulysses_overlap_groups` > 1 pipelines a pure-Ulysses call over that many head groups (batch 1, q/k/v of
     one shape, heads divisible by groups * Ulysses size): swaps of one group overlap attention of another."""
     u = _dim_index(query, ulysses_cp_dim)
     r = _dim_index(query, ring_cp_dim)
@@ -200,6 +225,16 @@ def scaled_dot_product_attention_with_cp(query: DTensor, key: DTensor, value: DT
         raise ValueError("ring_overlap needs a ring dim, is_causal=False and dropout_p=0")
     if key.placements != query.placements or value.placements != query.placements:
         raise RuntimeError("query, key and value have different placements")
+    if kv_cache is not None:
+        if dropout_p > 0.0 or r is not None or ring_overlap or ulysses_overlap_groups > 1:
+            raise ValueError("kv_cache goes with neither dropout nor a ring dim nor overlap")
+        if u is not None and query.placements[u] not in (Shard(1), Shard(2)):
+            raise ValueError("with kv_cache the Ulysses dim shards the sequence (Shard(2)) or the heads (Shard(1))")
+        n = query.device_mesh.shape[u] if u is not None else 1
+        if query.shape[1] % n or key.shape[1] % n:
+            raise ValueError(f"attention heads ({query.shape[1]}, {key.shape[1]}) cannot be divided evenly by the "
+                             f"Ulysses size {n}")
+        return _attention_with_cache(query, key, value, kv_cache, u, is_causal, scale)
     old_placements = list(query.placements)
     if not is_causal:
         plain = [Shard(p.get_shard_index()) if p.is_shard() and p.has_sub_split_coordinates() else p

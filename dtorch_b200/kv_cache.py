@@ -22,11 +22,12 @@ operators run on the current stream of the cache's device, whichever device is c
 from __future__ import annotations
 
 import math
-from typing import Optional, Tuple, Union
+from typing import Dict, Optional, Sequence, Tuple, Union
 
 import torch
 
 from . import _host
+from .dtensor import DeviceMesh, DTensor, Placement, cuda_device_of
 
 
 class QuantizedKVCache:
@@ -116,3 +117,86 @@ def kv_cache_evict(cache: QuantizedKVCache, lengths: torch.Tensor, weights: torc
         out = QuantizedKVCache(cache.batch, cache.kv_heads, most, cache.head_dim, cache.dtype, cache.block, cache.device)
     new_lengths, new_weights, kept = _host.kv_cache_evict(cache._c, lengths, weights, budget, recent, out._c)
     return out, new_lengths, new_weights, kept
+
+
+class DistributedKVCache:
+    """The 8-bit cache of a decoder on a device mesh: every device holds a QuantizedKVCache of its part of (batch,
+    kv_heads, capacity, head_dim) under `placements`, where a mesh dim may shard the batch (Shard(0)) or the heads
+    (Shard(1): the placement after the Ulysses swap), evenly, or replicate. It keeps the lengths and, with
+    `track_weights`, what evict goes by. scaled_dot_product_attention_with_cp(..., kv_cache=cache) appends and attends.
+
+    Attributes: locals (QuantizedKVCache of each device id), lengths and weights (tensors of each device id),
+    max_length (no sequence holds more tokens; known without asking the devices)."""
+
+    def __init__(self, device_mesh: DeviceMesh, placements: Sequence[Placement], batch: int, kv_heads: int, capacity: int,
+                 head_dim: int, dtype: torch.dtype = torch.int8, block: int = 64, track_weights: bool = False):
+        self.device_mesh = device_mesh
+        shape, ids = list(device_mesh.shape), device_mesh.ids
+        names = _host.normalize([repr(p) for p in placements], shape, ids, 4)
+        self.placements = [Placement(p) for p in names]
+        self.shape = (batch, kv_heads, capacity, head_dim)
+        parts = [1, 1]
+        for size, p in zip(shape, self.placements):
+            if p.is_shard() and not p.has_sub_split_coordinates() and p.get_shard_index() in (0, 1):
+                parts[p.get_shard_index()] *= size
+            elif not p.is_replicate():
+                raise ValueError(f"DistributedKVCache: a mesh dim shards the batch or the heads or replicates, not {p}")
+        if batch % parts[0] or kv_heads % parts[1]:
+            raise ValueError(f"DistributedKVCache: batch {batch} and heads {kv_heads} do not divide evenly into "
+                             f"{parts[0]} and {parts[1]} parts")
+        self.max_length = 0
+        self.locals: Dict[int, QuantizedKVCache] = {}
+        self.lengths: Dict[int, torch.Tensor] = {}
+        self.weights: Dict[int, torch.Tensor] = {}
+        for gid, s in _host.compute_local_shapes(list(self.shape), shape, ids, names).items():
+            dev = torch.device("cuda", cuda_device_of(gid))
+            self.locals[gid] = QuantizedKVCache(s[0], s[1], capacity, head_dim, dtype, block, dev)
+            self.lengths[gid] = torch.zeros(s[0], dtype=torch.int32, device=dev)
+            if track_weights:
+                self.weights[gid] = torch.zeros(s[:3], device=dev)
+
+    def _check(self, t: DTensor, name: str) -> None:
+        if t.device_mesh != self.device_mesh or t.placements != self.placements:
+            raise ValueError(f"DistributedKVCache: {name} is {t.placements} on {t.device_mesh}, the cache "
+                             f"{self.placements} on {self.device_mesh}")
+
+    def append(self, key: DTensor, value: DTensor) -> None:
+        """Append T tokens (batch, kv_heads, T, head_dim) to every sequence."""
+        self._check(key, "key")
+        self._check(value, "value")
+        if key.shape != value.shape or len(key.shape) != 4 or key.shape[:2] + key.shape[3:] != \
+                self.shape[:2] + self.shape[3:]:
+            raise ValueError(f"DistributedKVCache: key {key.shape} and value {value.shape} do not fit {self.shape}")
+        tokens = key.shape[2]
+        if self.max_length + tokens > self.shape[2]:
+            raise ValueError(f"DistributedKVCache: {tokens} more tokens than {self.max_length} do not fit the capacity "
+                             f"of {self.shape[2]}; evict first")
+        for gid, cache in self.locals.items():
+            kv_cache_append(cache, key.local(gid), value.local(gid), self.lengths[gid])
+            with torch.cuda.device(cache.device):
+                self.lengths[gid] += tokens
+        self.max_length += tokens
+
+    def attend(self, query: DTensor, is_causal: bool = True, scale: Optional[float] = None) -> DTensor:
+        """Attention of the last T tokens' queries (batch, query_heads, T, head_dim), as kv_cache_attention; adds to the
+        weights where they are tracked."""
+        self._check(query, "query")
+        if len(query.shape) != 4 or query.shape[0] != self.shape[0] or query.shape[3] != self.shape[3] or \
+                query.shape[1] % self.shape[1]:
+            raise ValueError(f"DistributedKVCache: query {query.shape} does not fit {self.shape}")
+        out = {gid: kv_cache_attention(query.local(gid), cache, self.lengths[gid], is_causal=is_causal, scale=scale,
+                                       weights=self.weights.get(gid)) for gid, cache in self.locals.items()}
+        return DTensor(out, self.device_mesh, query.placements, query.shape)
+
+    def evict(self, budget: int, recent: int = 0) -> None:
+        """kv_cache_evict on every device, by the tracked weights; the capacity stays."""
+        if not self.weights:
+            raise ValueError("DistributedKVCache: evict needs track_weights=True")
+        if not 0 <= recent <= budget <= self.shape[2]:
+            raise ValueError("DistributedKVCache: 0 <= recent <= budget <= capacity")
+        for gid, cache in self.locals.items():
+            into = QuantizedKVCache(cache.batch, cache.kv_heads, cache.capacity, cache.head_dim, cache.dtype, cache.block,
+                                    cache.device)
+            self.locals[gid], self.lengths[gid], self.weights[gid], _ = kv_cache_evict(
+                cache, self.lengths[gid], self.weights[gid], budget, recent, out=into)
+        self.max_length = min(self.max_length, budget)

@@ -532,3 +532,62 @@ def test_nothing_to_do():
     assert dt.kv_cache_attention(q, none, ints([])).shape == (0, 4, 3, 32)
     w = torch.empty((0, 2, 64), device="cuda")
     assert dt.kv_cache_evict(none, ints([]), w, 10)[3].shape == (0, 2, 10)
+
+
+@pytest.fixture(params=["same", "peer"])
+def mode(request, monkeypatch):
+    if request.param == "same":
+        monkeypatch.setenv("DTORCH_DTENSOR_IN_SAME_DEVICE", "1")
+    else:
+        if torch.cuda.device_count() < 2:
+            pytest.skip("peer mode needs 2 GPUs")
+        monkeypatch.delenv("DTORCH_DTENSOR_IN_SAME_DEVICE", raising=False)
+    monkeypatch.setenv("DTORCH_COMM_TIMEOUT_SECOND", "30")
+    dt.clear()
+    yield request.param
+    dt.clear()
+
+
+@pytest.mark.parametrize("group", [1, 3])
+def test_context_parallel_attention_with_a_cache(mode, group):
+    """A sequence-sharded prompt, a head-sharded token, an eviction and another token through
+    scaled_dot_product_attention_with_cp, against one device's cache."""
+    n, h, e, cap = 2, 4, 64, 256
+    mesh = dt.init_device_mesh("cuda", (2,), mesh_dim_names=["cp"])
+    gen = torch.Generator().manual_seed(23)
+    cache = dt.DistributedKVCache(mesh, [dt.Shard(1)], n, h, cap, e, block=32, track_weights=True)
+    one = dt.QuantizedKVCache(n, h, cap, e, block=32)
+    lengths, seen = ints([0, 0]), torch.zeros((n, h, cap), device="cuda")
+
+    def step(t, place):
+        q = torch.randn((n, h * group, t, e), generator=gen).to(BF16)
+        k, v = tokens(gen, n, h, t, e, BF16), tokens(gen, n, h, t, e, BF16)
+        dq, dk, dv = (dt.DTensor.from_torch(x, mesh, [place]) for x in (q, k, v))
+        out = dt.scaled_dot_product_attention_with_cp(dq, dk, dv, is_causal=True, ulysses_cp_dim="cp", kv_cache=cache)
+        assert out.placements == [place] and out.shape == q.shape
+        nonlocal lengths
+        dt.kv_cache_append(one, k.cuda(), v.cuda(), lengths)
+        lengths = lengths + t
+        want = dt.kv_cache_attention(q.cuda(), one, lengths, weights=seen)
+        torch.cuda.synchronize()
+        # how the tiles are shared out depends on the number of heads: sums differ in their order
+        assert torch.allclose(out.to_torch().float(), want.float().cpu(), rtol=2.0 ** -7, atol=2.0 ** -9)
+        for gid in mesh.ids:
+            part = seen[:, gid * 2:gid * 2 + 2].cpu()
+            assert torch.allclose(cache.weights[gid].cpu(), part, rtol=1e-5, atol=1e-8)
+
+    step(101, dt.Shard(2))
+    step(1, dt.Shard(1))
+    cache.evict(64, 16)
+    assert cache.max_length == 64
+    for gid in mesh.ids:
+        assert cache.locals[gid].capacity == cap and cache.lengths[gid].tolist() == [64, 64]
+    # the same choice on one device: the distributed weights
+    w = torch.cat([cache.weights[g].cpu() for g in mesh.ids], 1)
+    both = [torch.cat([getattr(cache.locals[g], k).cpu() for g in mesh.ids], 1).cuda()
+            for k in ("key", "value", "key_scale", "value_scale")]
+    one, lengths, seen = dt.QuantizedKVCache.from_tensors(*both), ints([64, 64]), w.cuda()
+    step(1, dt.Shard(1))
+    step(6, dt.Shard(2))
+    with pytest.raises(ValueError, match="evict"):
+        step(250, dt.Shard(1))

@@ -171,3 +171,26 @@ def test_oracle_rounds_as_torch_does():
         s = ko.scale_of(a, dtype)
         assert torch.equal(s, s.to(BF16).double()) and (s * ko.LIMIT[dtype] >= a).all()
         assert (s * ko.LIMIT[dtype] <= a * (1 + 2.0 ** -7)).all()
+
+
+def test_distributed_cache_refuses():
+    mesh = dt.init_device_mesh("cuda", (2,))
+    for placements, shape in (([dt.Shard(2)], (2, 2)), ([dt.Shard(3)], (2, 2)), ([dt.Partial()], (2, 2)),
+                              ([dt.Shard(1, 3)], (2, 4)), ([dt.Shard(1)], (2, 3)), ([dt.Shard(0)], (3, 2))):
+        with pytest.raises(ValueError):
+            dt.DistributedKVCache(mesh, placements, shape[0], shape[1], 64, 32)
+
+
+def test_attention_with_cp_refuses_what_the_cache_does_not_serve():
+    mesh = dt.init_device_mesh("cuda", (2,))
+    x = dt.DTensor({0: rows(h=2), 1: rows(h=2)}, mesh, [dt.Shard(1)], (2, 4, 3, 64))
+    s0 = dt.DTensor({0: rows(n=1), 1: rows(n=1)}, mesh, [dt.Shard(0)], (2, 2, 3, 64))
+    odd = dt.DTensor({0: rows(h=2), 1: rows(h=1)}, mesh, [dt.Shard(1)], (2, 3, 3, 64))
+    fake = object()  # never reached
+    for kw in (dict(dropout_p=0.1), dict(ring_cp_dim=0), dict(ulysses_overlap_groups=2)):
+        with pytest.raises(ValueError, match="kv_cache"):
+            dt.scaled_dot_product_attention_with_cp(x, x, x, kv_cache=fake, **{"ulysses_cp_dim": 0, **kw})
+    with pytest.raises(ValueError, match="Shard"):
+        dt.scaled_dot_product_attention_with_cp(s0, s0, s0, kv_cache=fake, ulysses_cp_dim=0)
+    with pytest.raises(ValueError, match="divided"):
+        dt.scaled_dot_product_attention_with_cp(odd, odd, odd, kv_cache=fake, ulysses_cp_dim=0)
