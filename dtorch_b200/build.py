@@ -38,7 +38,7 @@ def _newer(target: str, sources) -> bool:
     return any(os.path.getmtime(s) > t for s in sources)
 
 
-CAPI_SRCS = ["dt_comm.cu", "dt_kv.cu"]
+CAPI_SRCS = ["dt_comm.cu", "dt_kv.cu", "dt_kv_prompt.cu"]
 
 
 def build_capi(force: bool = False, verbose: bool = False) -> str:

@@ -8,6 +8,7 @@
 
 #include "dt_internal.h"
 #include "dt_kv.cuh"
+#include "dt_kv_prompt.h"
 
 using namespace dtb;
 
@@ -1099,8 +1100,12 @@ bool stores_scores(const dt_kv_cache* c, int64_t rows) {
     return rows <= 16 && c->batch * c->kv_heads * 16 * c->capacity * 4 <= (int64_t{1} << 30);
 }
 
+// Many rows of a head take the tensor-core kernel.
+bool many_rows(const dt_kv_cache* c, int64_t rows) { return rows > 32 && c->head_dim <= 128; }
+
 struct AttnPlan {
     int64_t rows, row_tiles;
+    bool many_rows;
     int grid;
     size_t out, stats, lse2, scores, bytes;  // offsets and the total
 };
@@ -1112,6 +1117,7 @@ int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool we
     const int64_t ep = padded_head(c->head_dim);
     p->rows = query_heads / c->kv_heads * tokens;
     p->row_tiles = (p->rows + 15) / 16;
+    p->many_rows = many_rows(c, p->rows);
     p->grid = sms * attn_ctas_per_sm(c->head_dim);
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     p->out = 0;
@@ -1131,14 +1137,19 @@ int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, b
     cudaError_t e = cudaFuncSetAttribute(k_kv_attend<E4M3, EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
     const int row_tiles = static_cast<int>(p.row_tiles);
-    k_kv_attend<E4M3, EP><<<p.grid, kAttnThreads, S::kSmem, stream>>>(a, w, row_tiles);
-    int st = check_launch("dt_kv_attention");
-    if (st != DT_OK) return st;
+    int st = DT_OK;
     unsigned grid = 0;
-    st = grid_of(static_cast<int64_t>(a.batch) * a.kv_heads * row_tiles * 16, "dt_kv_attention", &grid);
-    if (st != DT_OK) return st;
-    k_kv_merge<EP><<<grid, std::max(32, EP / 4), 0, stream>>>(a, w, row_tiles, p.grid);
-    st = check_launch("dt_kv_attention");
+    if (p.many_rows) {
+        st = kv_prompt_attention(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, w.lse2, stream);
+    } else {
+        k_kv_attend<E4M3, EP><<<p.grid, kAttnThreads, S::kSmem, stream>>>(a, w, row_tiles);
+        st = check_launch("dt_kv_attention");
+        if (st != DT_OK) return st;
+        st = grid_of(static_cast<int64_t>(a.batch) * a.kv_heads * row_tiles * 16, "dt_kv_attention", &grid);
+        if (st != DT_OK) return st;
+        k_kv_merge<EP><<<grid, std::max(32, EP / 4), 0, stream>>>(a, w, row_tiles, p.grid);
+        st = check_launch("dt_kv_attention");
+    }
     if (st != DT_OK || !weights) return st;
     const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
     if (w.scores != nullptr) {
