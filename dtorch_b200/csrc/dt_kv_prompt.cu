@@ -13,14 +13,16 @@ using namespace dtb;
 namespace {
 
 // 256 query rows of a key head (two tiles of 128) against tiles of 128 tokens, one CTA per SM:
-//   warps 0-3, 4-7   softmax of row tile 0, 1: a thread owns a row. It reads the row's scores from TMEM, writes its
-//                    weights back as fp16 over the same columns, and one thread issues the tile's next products:
-//                    O += P V (P from TMEM) and S = Q K^T for the next tokens. While one row tile is in its softmax,
-//                    the tensor core works for the other.
-//   warps 8-11       read codes from global memory into registers a tile ahead, turn them into fp16 (exact) and store
-//                    them as tcgen05 operands (128-byte swizzle), two stages of keys and two of values.
-// TMEM, 512 columns: S of both row tiles (128 each, P in the first half of each), O of both (EP each). The products of
-// one row tile are issued by one thread and run in order, so a completed S also says that the O += P V before it is done.
+//   warps 0-3, 4-7   softmax of row tile 0, 1: a thread owns a row. It reads the row's scores from TMEM and writes its
+//                    weights back as fp16 over the same columns, in two halves, each of which it reports.
+//   warps 8-11       copy codes to shared memory a tile ahead (cp.async, every thread its own 16 bytes, so no barrier),
+//                    turn them into fp16 (exact) and store them as tcgen05 operands (128-byte swizzle), two stages of
+//                    keys and two of values.
+//   warp 12          issues every product: O += P V (P from TMEM, the first half while the second is still made), then
+//                    S = Q K^T of the next tokens, for one row tile and then the other, so that one is in its softmax
+//                    while the tensor core works for the other.
+// TMEM, 512 columns: S of both row tiles (128 each, P in the first half of each), O of both (EP each). Products run in
+// the order of their issue, so a completed S also says that the O += P V before it is done.
 //
 // A softmax row keeps a reference instead of its exact maximum: it moves (and O is scaled, in TMEM) only when the
 // maximum has grown by more than 2^3, so weights stay below 2^3 and the scaling is rare. Block scales: a key scale is
@@ -29,7 +31,11 @@ namespace {
 // largest normal).
 constexpr int kRowTile = 128;
 constexpr int kTokTile = 128;
-constexpr int kPromptThreads = 384;
+constexpr int kPromptThreads = 512;
+// A softmax row holds 128 scores; the block is launched with 128 registers a thread and shares them out anew.
+constexpr int kSoftmaxRegs = 200, kConvertRegs = 72, kIssueRegs = 40;
+static_assert(256 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kIssueRegs <= kPromptThreads * 128,
+              "a sum above the launch's waits forever");
 constexpr float kGrowth = 3.0f;
 constexpr float kPromptShift = 12.0f;
 constexpr int kScaleRing = 4;
@@ -43,13 +49,16 @@ struct PromptShape {
     static constexpr int kQuery = 0;                           // two row tiles
     static constexpr int kKeys = 2 * kOperand;                 // two stages
     static constexpr int kValues = 4 * kOperand;               // two stages
-    static constexpr int kScales = 6 * kOperand;               // [ring][keys, values][4]
+    static constexpr int kCodes = 6 * kOperand;                // a tile's codes of keys and of values, on their way
+    static constexpr int kCodeBytes = 128 * EP;
+    static constexpr int kScales = kCodes + 2 * kCodeBytes;    // [ring][keys, values][4]
     static constexpr int kBars = kScales + kScaleRing * 2 * 4 * 4;
     static constexpr int kSmem = kBars + 256 + 1024;           // barriers, TMEM address, flag, maxima; alignment of the base
     static constexpr int kTmemCols = EP == 64 ? 512 : 512;
 };
 
-enum Bar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kBarCount = 10 };
+// kPReady: [row tile][half]
+enum Bar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kBarCount = 14 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -95,6 +104,15 @@ __device__ __forceinline__ void tc_commit(uint32_t bar) {
 __device__ __forceinline__ uint64_t operand_desc(uint32_t addr, uint32_t leading, uint32_t stride) {
     return static_cast<uint64_t>((addr & 0x3ffff) >> 4) | (static_cast<uint64_t>(leading >> 4) << 16) |
            (static_cast<uint64_t>(stride >> 4) << 32) | (1ull << 46) | (2ull << 61);
+}
+
+// One lane of a converged warp. tcgen05.mma takes its operands from uniform registers: issued behind this in a branch
+// that the whole warp takes it needs few instructions; behind `if (thread == 0)` every operand is moved over first (eight
+// products 800 cycles, measured, against the 512 that the tensor core takes).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 
 // fp16 operands, fp32 accumulator, M = 128; bit 16: B is MN-major.
@@ -148,9 +166,6 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Barrier of one warpgroup.
-__device__ __forceinline__ void group_sync(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
-
 // Byte offset of 16-byte chunk `c` (8 fp16) of row `r` in an operand of 128-byte panels.
 __device__ __forceinline__ uint32_t operand_offset(int r, int c) {
     return (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
@@ -195,35 +210,100 @@ __device__ __forceinline__ float stage_query(const KvAttnArgs& a, const uint16_t
     return inv;
 }
 
-// Codes of a tile of 128 tokens: this thread's vectors, EP / 16 of them (16 codes each).
+// Place of vector `v` (16 codes) of thread `tid` in a tile of 128 tokens. Eight lanes take four neighbouring vectors of
+// two rows: their halves, 16 bytes of fp16 each, then fall into eight different 16-byte columns of the swizzled panel.
 template <int EP>
-__device__ __forceinline__ void load_codes(const uint8_t* base, int tok, int len, int head_dim, int tid, uint4* w) {
+__device__ __forceinline__ void tile_place(int v, int tid, int& r, int& c) {
+    r = (v / (EP / 64)) * 32 + (tid >> 2);
+    c = (v % (EP / 64)) * 4 + (tid & 3);
+}
+
+// Codes of a tile of 128 tokens to shared memory: 16 codes a copy, EP / 16 copies a thread, each thread its own.
+template <int EP>
+__device__ __forceinline__ void fetch_codes(uint32_t smem, const uint8_t* base, int tok, int len, int head_dim, int tid) {
 #pragma unroll
     for (int v = 0; v < EP / 16; ++v) {
-        const int idx = v * 128 + tid, r = idx / (EP / 16), c = idx % (EP / 16);
-        w[v] = tok + r < len && c * 16 < head_dim
-                   ? __ldg(reinterpret_cast<const uint4*>(base + static_cast<size_t>(tok + r) * head_dim + c * 16))
-                   : make_uint4(0, 0, 0, 0);
+        int r, c;
+        tile_place<EP>(v, tid, r, c);
+        const bool live = tok + r < len && c * 16 < head_dim;
+        const uint8_t* const p = live ? base + static_cast<size_t>(tok + r) * head_dim + c * 16 : base;
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem + (v * 128 + tid) * 16), "l"(p),
+                     "r"(live ? 16 : 0)
+                     : "memory");
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+}
+
+// The thread's own codes as fp16 operand rows.
+template <bool E4M3, int EP>
+__device__ __forceinline__ void store_operand(uint8_t* smem, const uint8_t* codes, int tid) {
+#pragma unroll
+    for (int v = 0; v < EP / 16; ++v) {
+        int r, c;
+        tile_place<EP>(v, tid, r, c);
+        const uint4 w = *reinterpret_cast<const uint4*>(codes + (v * 128 + tid) * 16);
+        uint4 lo, hi;
+        codes_to_half<E4M3, 0>(w.x, lo.x, lo.y);
+        codes_to_half<E4M3, 0>(w.y, lo.z, lo.w);
+        codes_to_half<E4M3, 0>(w.z, hi.x, hi.y);
+        codes_to_half<E4M3, 0>(w.w, hi.z, hi.w);
+        *reinterpret_cast<uint4*>(smem + operand_offset(r, 2 * c)) = lo;
+        *reinterpret_cast<uint4*>(smem + operand_offset(r, 2 * c + 1)) = hi;
     }
 }
 
-// The same as fp16 operand rows.
-template <bool E4M3, int EP>
-__device__ __forceinline__ void store_operand(uint8_t* smem, int tid, const uint4* w) {
+// Pairs of fp32 in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// 32 scores of a row (span `c` of a tile) to weights: their sum in fp32, and times the value factor as 16 fp16 pairs.
+// MASKED: columns from `live` on count nothing, whatever the scales there are.
+template <bool MASKED>
+__device__ __forceinline__ float weights_of(const uint32_t* s, float f, float vf, float down, int live, uint32_t* p) {
+    float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
-    for (int v = 0; v < EP / 16; ++v) {
-        const int idx = v * 128 + tid, r = idx / (EP / 16), c = idx % (EP / 16);
-        uint4 lo, hi;
-        codes_to_half<E4M3, 0>(w[v].x, lo.x, lo.y);
-        codes_to_half<E4M3, 0>(w[v].y, lo.z, lo.w);
-        codes_to_half<E4M3, 0>(w[v].z, hi.x, hi.y);
-        codes_to_half<E4M3, 0>(w[v].w, hi.z, hi.w);
-        // eight lanes write a row of both panels: the second panel's lanes take their odd chunk first, so that no two
-        // of the eight meet in a bank
-        const bool swap = (c >> 2) & 1;
-        *reinterpret_cast<uint4*>(smem + operand_offset(r, 2 * c + (swap ? 1 : 0))) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(smem + operand_offset(r, 2 * c + (swap ? 0 : 1))) = swap ? lo : hi;
+    for (int i = 0; i < 32; i += 2) {
+        float2 x = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(f, f),
+                        make_float2(-down, -down));
+        x.x = ex2(x.x);
+        x.y = ex2(x.y);
+        if (MASKED) {
+            if (i >= live) x.x = 0.0f;
+            if (i + 1 >= live) x.y = 0.0f;
+        }
+        sum = add2(sum, x);
+        float2 v = mul2(x, make_float2(vf, vf));
+        if (MASKED) {
+            if (i >= live) v.x = 0.0f;
+            if (i + 1 >= live) v.y = 0.0f;
+        }
+        p[i >> 1] = pack_half2(v.x, v.y);
     }
+    return sum.x + sum.y;
 }
 
 template <bool E4M3, int EP>
@@ -236,8 +316,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
     float* const scales = reinterpret_cast<float*>(smem + S::kScales);
     volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + kBarCount * 8);
     volatile uint32_t* const dead = tmem_slot + 1;
-    volatile float* const vmax_slot = reinterpret_cast<volatile float*>(tmem_slot + 2);  // [12]
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile float* const vmax_slot = reinterpret_cast<volatile float*>(tmem_slot + 2);  // [16]
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     // the row tiles that see the most tokens first
     const size_t head = blockIdx.x % (static_cast<unsigned>(a.batch) * a.kv_heads);
@@ -255,10 +335,12 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
             mbar_init(bars + (kKFull + i) * 8, 128);
-            mbar_init(bars + (kKEmpty + i) * 8, 2);
+            mbar_init(bars + (kKEmpty + i) * 8, 1);
             mbar_init(bars + (kVFull + i) * 8, 128);
-            mbar_init(bars + (kVEmpty + i) * 8, 2);
+            mbar_init(bars + (kVEmpty + i) * 8, 1);
             mbar_init(bars + (kSFull + i) * 8, 1);
+            mbar_init(bars + (kPReady + i) * 8, 4);
+            mbar_init(bars + (kPReady + 2 + i) * 8, 4);
         }
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
@@ -276,24 +358,97 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
     if (lane == 0) vmax_slot[warp] = vmax;
+    // the row tiles' queries, a row a thread
+    float inv = 0.0f;
+    if (warp < 8) {
+        const int row = row0 + tid;
+        const uint16_t* qp = nullptr;
+        if (row < a.rows) {
+            const int t = row / a.group, jj = row - t * a.group;
+            qp = static_cast<const uint16_t*>(a.query) + n * a.q_stride_n +
+                 static_cast<int64_t>(h * a.group + jj) * a.q_stride_h + t * a.q_stride_t;
+        }
+        inv = stage_query<EP>(a, qp, smem + S::kQuery + (tid >> 7) * S::kOperand, tid & 127,
+                              a.scale_log2 < 0.0f ? -1.0f : 1.0f);
+        async_proxy_fence();
+    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    const uint32_t tmem = *tmem_slot;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
 
-    if (warp >= 8) {
+    const int row_groups = row0 + kRowTile < a.rows ? 2 : 1;  // row tiles that hold rows
+    constexpr uint32_t kScoreInstr = instr_desc(kTokTile, false), kOutInstr = instr_desc(EP, true);
+
+    if (warp >= 12) {
+        // ---- products ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
+        if (warp == 12 && tiles > 0) {
+            const auto scores = [&](int g, int j) {
+                const uint64_t q_desc = operand_desc(base + S::kQuery + g * S::kOperand, 16, 1024);
+                const uint64_t k_desc = operand_desc(base + S::kKeys + (j & 1) * S::kOperand, 16, 1024);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < EP / 16; ++k) {
+                        const uint32_t off = ((k >> 2) * S::kPanelBytes + (k & 3) * 32) >> 4;
+                        mma_ss(tmem + g * 128, q_desc + off, k_desc + off, kScoreInstr, k > 0);
+                    }
+                    tc_commit(bars + (kSFull + g) * 8);
+                    if (g + 1 == row_groups) tc_commit(bars + (kKEmpty + (j & 1)) * 8);
+                }
+                __syncwarp();
+            };
+            const auto outputs = [&](int g, int j, int half) {
+                const uint64_t v_desc = operand_desc(base + S::kValues + (j & 1) * S::kOperand, S::kPanelBytes, 1024);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < kTokTile / 32; ++k) {
+                        const int kk = half * (kTokTile / 32) + k;
+                        mma_ts(tmem + 256 + g * EP, tmem + g * 128 + kk * 8, v_desc + kk * (2048 >> 4), kOutInstr,
+                               j > 0 || kk > 0);
+                    }
+                    if (half == 1 && g + 1 == row_groups) tc_commit(bars + (kVEmpty + (j & 1)) * 8);
+                    if (half == 1 && j + 1 == tiles) tc_commit(bars + (kSFull + g) * 8);
+                }
+                __syncwarp();
+            };
+            const auto await = [&](int bar, int parity) {
+                mbar_wait(bars + bar * 8, parity, dead);
+                __syncwarp();
+                tc_fence_after();
+            };
+            await(kKFull, 0);
+            for (int g = 0; g < row_groups; ++g) scores(g, 0);
+            for (int j = 0; j < tiles; ++j) {
+                const bool more = j + 1 < tiles;
+                await(kVFull + (j & 1), (j >> 1) & 1);
+                if (more) await(kKFull + ((j + 1) & 1), ((j + 1) >> 1) & 1);
+                for (int g = 0; g < row_groups; ++g) {
+                    await(kPReady + g * 2, j & 1);
+                    outputs(g, j, 0);
+                    await(kPReady + g * 2 + 1, j & 1);
+                    outputs(g, j, 1);
+                    if (more) scores(g, j + 1);
+                }
+            }
+        }
+    } else if (warp >= 8) {
         // ---- keys and values to fp16 operands ----
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
         const int t = tid - 256;
         const uint8_t* const kbase = a.key + head * a.capacity * a.head_dim;
         const uint8_t* const vbase = a.value + head * a.capacity * a.head_dim;
-        uint4 kw[EP / 16], vw[EP / 16];
+        uint8_t* const kcodes = smem + S::kCodes;
+        uint8_t* const vcodes = kcodes + S::kCodeBytes;
         if (tiles > 0) {
-            load_codes<EP>(kbase, 0, len, a.head_dim, t, kw);
-            load_codes<EP>(vbase, 0, len, a.head_dim, t, vw);
+            fetch_codes<EP>(smem_addr(kcodes), kbase, 0, len, a.head_dim, t);
+            fetch_codes<EP>(smem_addr(vcodes), vbase, 0, len, a.head_dim, t);
         }
         for (int j = 0; j < tiles; ++j) {
             const int st = j & 1;
             const uint32_t free_parity = ((j >> 1) & 1) ^ 1;
+            // behind the last tile nothing is fetched: every copy is of tokens < len or of no bytes
+            const int next = j + 1 < tiles ? (j + 1) * kTokTile : len;
             float sc = 0.0f;
             if (t < 8) {  // the scales of the tile's four spans of 32 tokens; 0 behind the length
                 const int tok = j * kTokTile + (t & 3) * 32;
@@ -301,26 +456,28 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
             }
             mbar_wait(bars + (kKEmpty + st) * 8, free_parity, dead);
             if (t < 8) scales[(j % kScaleRing) * 8 + t] = sc;
-            store_operand<E4M3, EP>(smem + S::kKeys + st * S::kOperand, t, kw);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            store_operand<E4M3, EP>(smem + S::kKeys + st * S::kOperand, kcodes, t);
             async_proxy_fence();
             mbar_arrive(bars + (kKFull + st) * 8);
-            if (j + 1 < tiles) load_codes<EP>(kbase, (j + 1) * kTokTile, len, a.head_dim, t, kw);
+            fetch_codes<EP>(smem_addr(kcodes), kbase, next, len, a.head_dim, t);
             mbar_wait(bars + (kVEmpty + st) * 8, free_parity, dead);
-            store_operand<E4M3, EP>(smem + S::kValues + st * S::kOperand, t, vw);
+            asm volatile("cp.async.wait_group 1;" ::: "memory");
+            store_operand<E4M3, EP>(smem + S::kValues + st * S::kOperand, vcodes, t);
             async_proxy_fence();
             mbar_arrive(bars + (kVFull + st) * 8);
-            if (j + 1 < tiles) load_codes<EP>(vbase, (j + 1) * kTokTile, len, a.head_dim, t, vw);
+            fetch_codes<EP>(smem_addr(vcodes), vbase, next, len, a.head_dim, t);
         }
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         // ---- softmax of a row tile ----
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         const int g = warp >> 2;            // row tile of the two
         const int r = tid & 127;            // row of the tile = TMEM lane
         const int row = row0 + g * kRowTile + r;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         const uint32_t s_col = tmem + g * 128, o_col = tmem + 256 + g * EP;
-        const uint32_t query = base + S::kQuery + g * S::kOperand;
-        const uint32_t s_full = bars + (kSFull + g) * 8;
-        constexpr uint32_t kScoreInstr = instr_desc(kTokTile, false), kOutInstr = instr_desc(EP, true);
+        const uint32_t s_full = bars + (kSFull + g) * 8, p_ready = bars + (kPReady + g * 2) * 8;
 
         float vtop = 0.0f;
 #pragma unroll
@@ -331,36 +488,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
         const float v_down = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23) * exp2f(kPromptShift);
         const float v_up = __uint_as_float(static_cast<uint32_t>(127 + ve) << 23) * (code_unit<E4M3>() * exp2f(-kPromptShift));
 
-        const uint16_t* qp = nullptr;
-        if (row < a.rows) {
-            const int t = row / a.group, jj = row - t * a.group;
-            qp = static_cast<const uint16_t*>(a.query) + n * a.q_stride_n +
-                 static_cast<int64_t>(h * a.group + jj) * a.q_stride_h + t * a.q_stride_t;
-        }
-        const float inv = stage_query<EP>(a, qp, smem + S::kQuery + g * S::kOperand, r, a.scale_log2 < 0.0f ? -1.0f : 1.0f);
         const float factor = inv * fabsf(a.scale_log2) * code_unit<E4M3>();
         const int lim = kv_limit(a, row, len, cnt);
-        async_proxy_fence();
-        group_sync(1 + g);
-
-        const auto issue_scores = [&](int j) {
-            const uint32_t keys = base + S::kKeys + (j & 1) * S::kOperand;
-            mbar_wait(bars + (kKFull + (j & 1)) * 8, (j >> 1) & 1, dead);
-            tc_fence_after();
-#pragma unroll
-            for (int k = 0; k < EP / 16; ++k) {
-                const uint32_t off = (k >> 2) * S::kPanelBytes + (k & 3) * 32;
-                mma_ss(s_col, operand_desc(query + off, 16, 1024), operand_desc(keys + off, 16, 1024), kScoreInstr, k > 0);
-            }
-            tc_commit(bars + (kKEmpty + (j & 1)) * 8);
-        };
-        if (r == 0 && tiles > 0) {
-            issue_scores(0);
-            tc_commit(s_full);
-        }
-
         float ref = -INFINITY, l = 0.0f;
-        for (int j = 0; j < tiles; ++j) {
+        const int steps = g < row_groups ? tiles : 0;
+        for (int j = 0; j < steps; ++j) {
             mbar_wait(s_full, j & 1, dead);
             __syncwarp();
             tc_fence_after();
@@ -376,14 +508,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
                 for (int c = 0; c < 128; ++c)
                     if (tok + c >= lim) s[c] = 0xff800000u;
             }
+            float mx[8];  // two chains for each span of 32 columns
+#pragma unroll
+            for (int c = 0; c < 8; ++c) mx[c] = __uint_as_float(s[c * 16]);
+#pragma unroll
+            for (int i = 1; i < 16; ++i)
+#pragma unroll
+                for (int c = 0; c < 8; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(s[c * 16 + i]));
             float top = -INFINITY;
 #pragma unroll
             for (int c = 0; c < 4; ++c) {
-                float mx = -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, __uint_as_float(s[c * 32 + i]));
-                // a masked score stays so where the scale is 0
-                if (mx != -INFINITY) top = fmaxf(top, mx * (factor * sc[c]));
+                const float m = fmaxf(mx[2 * c], mx[2 * c + 1]);
+                if (m != -INFINITY) top = fmaxf(top, m * (factor * sc[c]));  // masked stays masked where the scale is 0
             }
             const bool grow = top > ref + kGrowth;  // also the first: ref is -infinity
             if (__any_sync(0xffffffffu, grow)) {
@@ -408,45 +544,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
             for (int c = 0; c < 4; ++c) {
                 uint32_t p[16];
                 const float f = factor * sc[c], vf = sc[4 + c] * v_down;
-                float sum = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 32; i += 2) {
-                    const int k = c * 32 + i;
-                    float x = ex2(fmaf(__uint_as_float(s[k]), f, -down));
-                    float y = ex2(fmaf(__uint_as_float(s[k + 1]), f, -down));
-                    if (ragged) {
-                        if (tok + k >= lim) x = 0.0f;
-                        if (tok + k + 1 >= lim) y = 0.0f;
-                    }
-                    sum += x + y;
-                    float px = x * vf, py = y * vf;
-                    if (ragged) {
-                        if (tok + k >= lim) px = 0.0f;
-                        if (tok + k + 1 >= lim) py = 0.0f;
-                    }
-                    p[i >> 1] = pack_half2(px, py);
-                }
-                l += sum;
+                if (ragged) l += weights_of<true>(s + c * 32, f, vf, down, lim - tok - c * 32, p);
+                else l += weights_of<false>(s + c * 32, f, vf, down, 32, p);
                 tmem_store16(s_col + lanes + c * 16, p);
-            }
-            tmem_wait_store();
-            tc_fence_before();
-            group_sync(1 + g);
-            if (r == 0) {
-                tc_fence_after();
-                const uint32_t values = base + S::kValues + (j & 1) * S::kOperand;
-                mbar_wait(bars + (kVFull + (j & 1)) * 8, (j >> 1) & 1, dead);
-                tc_fence_after();
-#pragma unroll
-                for (int k = 0; k < kTokTile / 16; ++k)
-                    mma_ts(o_col, s_col + k * 8, operand_desc(values + k * 2048, S::kPanelBytes, 1024), kOutInstr,
-                           j > 0 || k > 0);
-                tc_commit(bars + (kVEmpty + (j & 1)) * 8);
-                if (j + 1 < tiles) issue_scores(j + 1);
-                tc_commit(s_full);
+                if (c & 1) {
+                    tmem_wait_store();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(p_ready + (c >> 1) * 8);
+                }
             }
         }
-        if (tiles > 0) {
+        if (steps > 0) {
             mbar_wait(s_full, tiles & 1, dead);
             __syncwarp();
             tc_fence_after();
@@ -458,7 +567,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
 #pragma unroll
         for (int c = 0; c < EP; c += 32) {
             uint32_t o[32];
-            if (tiles > 0) {
+            if (steps > 0) {
                 tmem_load32(o_col + lanes + c, o);
                 tmem_wait_load();
             }
@@ -468,8 +577,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     // a row that saw nothing: its O may be anything where no tile was computed
-                    const float x = tiles > 0 && l != 0.0f ? __uint_as_float(o[i + 2 * k]) * inv_l : 0.0f;
-                    const float y = tiles > 0 && l != 0.0f ? __uint_as_float(o[i + 2 * k + 1]) * inv_l : 0.0f;
+                    const float x = steps > 0 && l != 0.0f ? __uint_as_float(o[i + 2 * k]) * inv_l : 0.0f;
+                    const float y = steps > 0 && l != 0.0f ? __uint_as_float(o[i + 2 * k + 1]) * inv_l : 0.0f;
                     if (a.query_bf16) {
                         const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
                         q[k] = *reinterpret_cast<const uint32_t*>(&b);
