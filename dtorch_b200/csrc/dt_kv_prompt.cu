@@ -13,14 +13,15 @@ using namespace dtb;
 namespace {
 
 // 256 query rows of a key head (two tiles of 128) against tiles of 128 tokens, one CTA per SM:
-//   warps 0-3, 4-7   softmax of row tile 0, 1: a thread owns a row. It reads the row's scores from TMEM and writes its
-//                    weights back as fp16 over the same columns, in two halves, each of which it reports.
-//   warps 8-11       copy codes to shared memory a tile ahead (cp.async, every thread its own 16 bytes, so no barrier),
+//   warps 0-15       softmax: two warpgroups for each row tile, one for each half of the 128 columns; two threads share
+//                    a row. They read their scores from TMEM, agree on the row's reference, and write their weights
+//                    back as fp16 over columns that have been read, each half reported by itself.
+//   warps 16-19      copy codes to shared memory a tile ahead (cp.async, every thread its own 16 bytes, so no barrier),
 //                    turn them into fp16 (exact) and store them as tcgen05 operands (128-byte swizzle), two stages of
 //                    keys and two of values.
-//   warp 12          issues every product: O += P V (P from TMEM, the first half while the second is still made), then
-//                    S = Q K^T of the next tokens, for one row tile and then the other, so that one is in its softmax
-//                    while the tensor core works for the other.
+//   warp 20          issues every product: O += P V (P from TMEM, the halves as they come), then S = Q K^T of the next
+//                    tokens, for one row tile and then the other, so that one is in its softmax while the tensor core
+//                    works for the other.
 // TMEM, 512 columns: S of both row tiles (128 each, P in the first half of each), O of both (EP each). Products run in
 // the order of their issue, so a completed S also says that the O += P V before it is done.
 //
@@ -31,10 +32,11 @@ namespace {
 // largest normal).
 constexpr int kRowTile = 128;
 constexpr int kTokTile = 128;
-constexpr int kPromptThreads = 512;
-// A softmax row holds 128 scores; the block is launched with 128 registers a thread and shares them out anew.
-constexpr int kSoftmaxRegs = 200, kConvertRegs = 72, kIssueRegs = 40;
-static_assert(256 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kIssueRegs <= kPromptThreads * 128,
+constexpr int kPromptThreads = 768;
+constexpr int kConvertWarp = 16, kIssueWarp = 20;
+// A softmax thread holds 64 scores; the block is launched with 80 registers a thread and shares them out anew.
+constexpr int kSoftmaxRegs = 96, kConvertRegs = 64, kIssueRegs = 32;
+static_assert(512 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kIssueRegs <= kPromptThreads * 80,
               "a sum above the launch's waits forever");
 constexpr float kGrowth = 3.0f;
 constexpr float kPromptShift = 12.0f;
@@ -53,12 +55,14 @@ struct PromptShape {
     static constexpr int kCodeBytes = 128 * EP;
     static constexpr int kScales = kCodes + 2 * kCodeBytes;    // [ring][keys, values][4]
     static constexpr int kBars = kScales + kScaleRing * 2 * 4 * 4;
-    static constexpr int kSmem = kBars + 256 + 1024;           // barriers, TMEM address, flag, maxima; alignment of the base
-    static constexpr int kTmemCols = EP == 64 ? 512 : 512;
+    static constexpr int kTops = kBars + 256;                  // bfloat16 [parity][row tile][half][row]
+    static constexpr int kSmem = kTops + 2 * 2 * 2 * 128 * 2;  // barriers, TMEM address, flag, maxima before it
+    static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
+    static constexpr int kTmemCols = 512;
 };
 
 // kPReady: [row tile][half]
-enum Bar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kBarCount = 14 };
+enum Bar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kQReady = 14, kBarCount = 15 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -163,7 +167,15 @@ __device__ __forceinline__ void tmem_store16(uint32_t addr, const uint32_t* r) {
         : "memory");
 }
 
-__device__ __forceinline__ void tmem_wait_load() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+#define DT_RW4(a, i) "+r"((a)[i]), "+r"((a)[(i) + 1]), "+r"((a)[(i) + 2]), "+r"((a)[(i) + 3])
+
+// Wait for the loads issued so far; the registers of the last are named, so that nothing uses them before.
+__device__ __forceinline__ void tmem_wait_load32(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : DT_RW4(r, 0), DT_RW4(r, 4), DT_RW4(r, 8), DT_RW4(r, 12), DT_RW4(r, 16), DT_RW4(r, 20), DT_RW4(r, 24),
+                   DT_RW4(r, 28)::"memory");
+}
+
 __device__ __forceinline__ void tmem_wait_store() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Byte offset of 16-byte chunk `c` (8 fp16) of row `r` in an operand of 128-byte panels.
@@ -171,22 +183,35 @@ __device__ __forceinline__ uint32_t operand_offset(int r, int c) {
     return (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// One query row to fp16 in the operand at `smem` (row `r`), scaled by a power of two; returns its inverse. `sign`
-// carries the sign of the softmax scale, so that the score factor is not negative.
+// The least bfloat16 that is not below x (its upper 16 bits), and back.
+__device__ __forceinline__ uint16_t round_up16(float x) {
+    const uint32_t b = __float_as_uint(x);
+    return static_cast<uint16_t>(((b >> 31) != 0 || b == 0x7f800000u ? b : b + 0xffffu) >> 16);
+}
+__device__ __forceinline__ float from16(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
+
+// Barrier of two warps.
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+
+// Half a query row to fp16 in the operand at `smem` (row `r`), scaled by a power of two that it agrees on with the other
+// half (`mine`, `other`: one warp of each half at the barrier `id`); returns its inverse. `sign` carries the sign of the
+// softmax scale, so that the score factor is not negative.
 template <int EP>
-__device__ __forceinline__ float stage_query(const KvAttnArgs& a, const uint16_t* p, uint8_t* smem, int r, float sign) {
-    uint32_t x[EP / 2];
+__device__ __forceinline__ float stage_query(const KvAttnArgs& a, const uint16_t* p, uint8_t* smem, int r, int half,
+                                             volatile uint16_t* mine, volatile uint16_t* other, int id, float sign) {
+    uint32_t x[EP / 4];
     float amax = 0.0f;
 #pragma unroll
-    for (int c = 0; c < EP / 8; ++c) {
-        const bool live = p != nullptr && c * 8 < a.head_dim;
+    for (int c = 0; c < EP / 16; ++c) {
+        const int e = half * (EP / 2) + c * 8;
+        const bool live = p != nullptr && e < a.head_dim;
         if (live && a.q_vec) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p + c * 8);
+            const uint4 u = *reinterpret_cast<const uint4*>(p + e);
             x[c * 4] = u.x, x[c * 4 + 1] = u.y, x[c * 4 + 2] = u.z, x[c * 4 + 3] = u.w;
         } else {
 #pragma unroll
             for (int j = 0; j < 4; ++j)
-                x[c * 4 + j] = live ? p[c * 8 + 2 * j] | (static_cast<uint32_t>(p[c * 8 + 2 * j + 1]) << 16) : 0u;
+                x[c * 4 + j] = live ? p[e + 2 * j] | (static_cast<uint32_t>(p[e + 2 * j + 1]) << 16) : 0u;
         }
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -194,18 +219,20 @@ __device__ __forceinline__ float stage_query(const KvAttnArgs& a, const uint16_t
             amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
         }
     }
+    *mine = round_up16(amax);
+    pair_sync(id);
     float mul, inv;
-    row_power(amax, mul, inv);
+    row_power(fmaxf(from16(*mine), from16(*other)), mul, inv);
     mul *= sign;
 #pragma unroll
-    for (int c = 0; c < EP / 8; ++c) {
+    for (int c = 0; c < EP / 16; ++c) {
         uint32_t h[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const float2 f = unpack16(x[c * 4 + j], a.query_bf16);
             h[j] = pack_half2(f.x * mul, f.y * mul);
         }
-        *reinterpret_cast<uint4*>(smem + operand_offset(r, c)) = make_uint4(h[0], h[1], h[2], h[3]);
+        *reinterpret_cast<uint4*>(smem + operand_offset(r, half * (EP / 16) + c)) = make_uint4(h[0], h[1], h[2], h[3]);
     }
     return inv;
 }
@@ -252,71 +279,94 @@ __device__ __forceinline__ void store_operand(uint8_t* smem, const uint8_t* code
     }
 }
 
-// Pairs of fp32 in one instruction.
-__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
-        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+// Pairs of fp32 in one 64-bit register: one instruction for two elements.
+using Pair = unsigned long long;
+
+__device__ __forceinline__ Pair pair_of(float x, float y) {
+    Pair d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(x), "f"(y));
     return d;
 }
 
-__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-        "mul.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ void unpair(Pair p, float& x, float& y) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p));
+}
+
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
     return d;
 }
 
-__device__ __forceinline__ float2 add2(float2 a, float2 b) {
-    float2 d;
-    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
-        "add.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
-        : "=f"(d.x), "=f"(d.y)
-        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
 
-// 32 scores of a row (span `c` of a tile) to weights: their sum in fp32, and times the value factor as 16 fp16 pairs.
-// MASKED: columns from `live` on count nothing, whatever the scales there are.
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// In the place that the program gives it: an exponential occupies its unit for 8 cycles, in which the warp can issue
+// the arithmetic of other columns.
+__device__ __forceinline__ void ex2_here(float& x) { asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x)); }
+
+// 32 scores of a row to weights: 16 fp16 pairs, times the value factor; adds their sum in fp32 (without the value
+// factor). Columns 2 i and 2 i + 1 go through three stages, a few columns apart, so that the exponentials of some run
+// beside the arithmetic of others. MASKED: columns from `live` on count nothing, whatever the scales there are.
 template <bool MASKED>
-__device__ __forceinline__ float weights_of(const uint32_t* s, float f, float vf, float down, int live, uint32_t* p) {
-    float2 sum = make_float2(0.0f, 0.0f);
+__device__ __forceinline__ void weigh(const uint32_t* s, float f, float vf, float down, int live, uint32_t* p, Pair* sum) {
+    constexpr int kAhead = 2, kBehind = 4;
+    const Pair f2 = pair_of(f, f), vf2 = pair_of(vf, vf), down2 = pair_of(-down, -down);
+    Pair x[16];
 #pragma unroll
-    for (int i = 0; i < 32; i += 2) {
-        float2 x = fma2(make_float2(__uint_as_float(s[i]), __uint_as_float(s[i + 1])), make_float2(f, f),
-                        make_float2(-down, -down));
-        x.x = ex2(x.x);
-        x.y = ex2(x.y);
-        if (MASKED) {
-            if (i >= live) x.x = 0.0f;
-            if (i + 1 >= live) x.y = 0.0f;
+    for (int i = -kAhead; i < 16 + kBehind; ++i) {
+        const int k = i + kAhead;
+        if (k < 16) x[k] = fma2(pair_of(__uint_as_float(s[2 * k]), __uint_as_float(s[2 * k + 1])), f2, down2);
+        if (i >= 0 && i < 16) {
+            float a, b;
+            unpair(x[i], a, b);
+            ex2_here(a);
+            ex2_here(b);
+            x[i] = pair_of(a, b);
         }
-        sum = add2(sum, x);
-        float2 v = mul2(x, make_float2(vf, vf));
-        if (MASKED) {
-            if (i >= live) v.x = 0.0f;
-            if (i + 1 >= live) v.y = 0.0f;
+        const int d = i - kBehind;
+        if (d >= 0) {
+            float a, b;
+            if (MASKED) {
+                unpair(x[d], a, b);
+                x[d] = pair_of(2 * d >= live ? 0.0f : a, 2 * d + 1 >= live ? 0.0f : b);
+            }
+            sum[d & 1] = add2(sum[d & 1], x[d]);
+            unpair(mul2(x[d], vf2), a, b);
+            if (MASKED) {
+                if (2 * d >= live) a = 0.0f;
+                if (2 * d + 1 >= live) b = 0.0f;
+            }
+            p[d] = pack_half2(a, b);
         }
-        p[i >> 1] = pack_half2(v.x, v.y);
     }
-    return sum.x + sum.y;
 }
 
 template <bool E4M3, int EP>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, float* lse2_out, int row_tiles) {
     using S = PromptShape<EP>;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* const smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t{1023});
+    extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_addr(smem);
     const uint32_t bars = base + S::kBars;
     float* const scales = reinterpret_cast<float*>(smem + S::kScales);
     volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + kBarCount * 8);
     volatile uint32_t* const dead = tmem_slot + 1;
-    volatile float* const vmax_slot = reinterpret_cast<volatile float*>(tmem_slot + 2);  // [16]
+    volatile float* const vmax_slot = reinterpret_cast<volatile float*>(tmem_slot + 2);  // [24]
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
     // the row tiles that see the most tokens first
@@ -342,10 +392,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
             mbar_init(bars + (kPReady + i) * 8, 4);
             mbar_init(bars + (kPReady + 2 + i) * 8, 4);
         }
+        mbar_init(bars + kQReady * 8, kConvertWarp);
         *dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 8) {
+    if (warp == kConvertWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(const_cast<uint32_t*>(tmem_slot))),
                      "n"(S::kTmemCols)
                      : "memory");
@@ -358,20 +409,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
 #pragma unroll
     for (int d = 16; d > 0; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
     if (lane == 0) vmax_slot[warp] = vmax;
-    // the row tiles' queries, a row a thread
-    float inv = 0.0f;
-    if (warp < 8) {
-        const int row = row0 + tid;
-        const uint16_t* qp = nullptr;
-        if (row < a.rows) {
-            const int t = row / a.group, jj = row - t * a.group;
-            qp = static_cast<const uint16_t*>(a.query) + n * a.q_stride_n +
-                 static_cast<int64_t>(h * a.group + jj) * a.q_stride_h + t * a.q_stride_t;
-        }
-        inv = stage_query<EP>(a, qp, smem + S::kQuery + (tid >> 7) * S::kOperand, tid & 127,
-                              a.scale_log2 < 0.0f ? -1.0f : 1.0f);
-        async_proxy_fence();
-    }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
@@ -380,10 +417,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
     const int row_groups = row0 + kRowTile < a.rows ? 2 : 1;  // row tiles that hold rows
     constexpr uint32_t kScoreInstr = instr_desc(kTokTile, false), kOutInstr = instr_desc(EP, true);
 
-    if (warp >= 12) {
+    if (warp >= kIssueWarp) {
         // ---- products ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        if (warp == 12 && tiles > 0) {
+        if (warp == kIssueWarp && tiles > 0) {
             const auto scores = [&](int g, int j) {
                 const uint64_t q_desc = operand_desc(base + S::kQuery + g * S::kOperand, 16, 1024);
                 const uint64_t k_desc = operand_desc(base + S::kKeys + (j & 1) * S::kOperand, 16, 1024);
@@ -404,7 +441,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
 #pragma unroll
                     for (int k = 0; k < kTokTile / 32; ++k) {
                         const int kk = half * (kTokTile / 32) + k;
-                        mma_ts(tmem + 256 + g * EP, tmem + g * 128 + kk * 8, v_desc + kk * (2048 >> 4), kOutInstr,
+                        mma_ts(tmem + 256 + g * EP, tmem + g * 128 + (kk >> 1) * 32 + (kk & 1) * 8, v_desc + kk * (2048 >> 4), kOutInstr,
                                j > 0 || kk > 0);
                     }
                     if (half == 1 && g + 1 == row_groups) tc_commit(bars + (kVEmpty + (j & 1)) * 8);
@@ -417,6 +454,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
                 __syncwarp();
                 tc_fence_after();
             };
+            await(kQReady, 0);
             await(kKFull, 0);
             for (int g = 0; g < row_groups; ++g) scores(g, 0);
             for (int j = 0; j < tiles; ++j) {
@@ -432,10 +470,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
                 }
             }
         }
-    } else if (warp >= 8) {
+    } else if (warp >= kConvertWarp) {
         // ---- keys and values to fp16 operands ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
-        const int t = tid - 256;
+        const int t = tid - kConvertWarp * 32;
         const uint8_t* const kbase = a.key + head * a.capacity * a.head_dim;
         const uint8_t* const vbase = a.value + head * a.capacity * a.head_dim;
         uint8_t* const kcodes = smem + S::kCodes;
@@ -472,13 +510,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
     } else {
         // ---- softmax of a row tile ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
-        const int g = warp >> 2;            // row tile of the two
-        const int r = tid & 127;            // row of the tile = TMEM lane
-        const int row = row0 + g * kRowTile + r;
+        // row tile, half of the columns, row, and the barrier and places shared with the row's other thread
+        const int g = warp >> 3, half = (warp >> 2) & 1, r = tid & 127, row = row0 + g * kRowTile + r;
+        const int pair = 1 + g * 4 + (warp & 3);
+        volatile uint16_t* const tops = reinterpret_cast<volatile uint16_t*>(smem + S::kTops) + g * 256 + r;  // + parity * 512
+        float factor;
+        {
+            const uint16_t* qp = nullptr;
+            if (row < a.rows) {
+                const int t = row / a.group, jj = row - t * a.group;
+                qp = static_cast<const uint16_t*>(a.query) + n * a.q_stride_n +
+                     static_cast<int64_t>(h * a.group + jj) * a.q_stride_h + t * a.q_stride_t;
+            }
+            // the places of odd tiles: the first tile's are written before the other thread has read these
+            const float inv = stage_query<EP>(a, qp, smem + S::kQuery + g * S::kOperand, r, half, tops + 512 + half * 128,
+                                              tops + 512 + (half ^ 1) * 128, pair, a.scale_log2 < 0.0f ? -1.0f : 1.0f);
+            factor = inv * fabsf(a.scale_log2) * code_unit<E4M3>();
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + kQReady * 8);
+        }
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
-        const uint32_t s_col = tmem + g * 128, o_col = tmem + 256 + g * EP;
-        const uint32_t s_full = bars + (kSFull + g) * 8, p_ready = bars + (kPReady + g * 2) * 8;
-
+        // this thread's columns of S; a span's weights lie over its own scores
+        const uint32_t s_col = (tmem + g * 128 + half * 64) | lanes, o_col = (tmem + 256 + g * EP + half * (EP / 2)) | lanes;
+        const uint32_t s_full = bars + (kSFull + g) * 8, p_ready = bars + (kPReady + g * 2 + half) * 8;
         float vtop = 0.0f;
 #pragma unroll
         for (int i = 0; i < kPromptThreads / 32; ++i) vtop = fmaxf(vtop, vmax_slot[i]);
@@ -488,7 +543,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
         const float v_down = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23) * exp2f(kPromptShift);
         const float v_up = __uint_as_float(static_cast<uint32_t>(127 + ve) << 23) * (code_unit<E4M3>() * exp2f(-kPromptShift));
 
-        const float factor = inv * fabsf(a.scale_log2) * code_unit<E4M3>();
         const int lim = kv_limit(a, row, len, cnt);
         float ref = -INFINITY, l = 0.0f;
         const int steps = g < row_groups ? tiles : 0;
@@ -496,80 +550,106 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
             mbar_wait(s_full, j & 1, dead);
             __syncwarp();
             tc_fence_after();
-            uint32_t s[128];
-#pragma unroll
-            for (int c = 0; c < 4; ++c) tmem_load32(s_col + lanes + c * 32, s + c * 32);
-            const float* const sc = scales + (j % kScaleRing) * 8;
-            tmem_wait_load();
-            const int tok = j * kTokTile;
-            const bool ragged = __any_sync(0xffffffffu, tok + kTokTile > lim);
-            if (ragged) {
-#pragma unroll
-                for (int c = 0; c < 128; ++c)
-                    if (tok + c >= lim) s[c] = 0xff800000u;
-            }
-            float mx[8];  // two chains for each span of 32 columns
-#pragma unroll
-            for (int c = 0; c < 8; ++c) mx[c] = __uint_as_float(s[c * 16]);
-#pragma unroll
-            for (int i = 1; i < 16; ++i)
-#pragma unroll
-                for (int c = 0; c < 8; ++c) mx[c] = fmaxf(mx[c], __uint_as_float(s[c * 16 + i]));
+            const float* const sc = scales + (j % kScaleRing) * 8 + half * 2;
+            const int live = lim - j * kTokTile - half * 64;  // of these columns
+            const bool ragged = __any_sync(0xffffffffu, live < 64);
+            uint32_t s[32];
             float top = -INFINITY;
+            // span 0 is loaded again for its weights: 32 scores fewer to hold meanwhile
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                const float m = fmaxf(mx[2 * c], mx[2 * c + 1]);
+            for (int c = 0; c < 2; ++c) {
+                tmem_load32(s_col + c * 32, s);
+                tmem_wait_load32(s);
+                uint32_t* const x = s;
+                if (ragged) {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i)
+                        if (c * 32 + i >= live) x[i] = 0xff800000u;
+                }
+                float mx[2] = {fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])),
+                               fmaxf(__uint_as_float(x[2]), __uint_as_float(x[3]))};
+#pragma unroll
+                for (int i = 4; i < 32; i += 4) {
+                    mx[0] = max3(mx[0], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
+                    mx[1] = max3(mx[1], __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
+                }
+                const float m = fmaxf(mx[0], mx[1]);
                 if (m != -INFINITY) top = fmaxf(top, m * (factor * sc[c]));  // masked stays masked where the scale is 0
             }
+            // the row's largest, of both halves, as bfloat16 rounded up: a reference need not be exact. The next use of
+            // these places is two tiles on, behind the other thread's barrier of the next.
+            const uint16_t top16 = round_up16(top);
+            tops[(j & 1) * 512 + half * 128] = top16;
+            pair_sync(pair);
+            top = fmaxf(from16(top16), from16(tops[(j & 1) * 512 + (half ^ 1) * 128]));
             const bool grow = top > ref + kGrowth;  // also the first: ref is -infinity
-            if (__any_sync(0xffffffffu, grow)) {
+            if (__any_sync(0xffffffffu, grow)) {    // the same for both warps of the pair
                 const float now = grow ? top : ref;
                 const float alpha = grow ? ex2(ref - now) : 1.0f;
                 ref = now;
                 l *= alpha;
                 if (j > 0) {
-#pragma unroll
-                    for (int c = 0; c < EP; c += 32) {
+#pragma unroll 1
+                    for (int c = 0; c < EP / 2; c += 32) {
+                        const uint32_t col = o_col + c;
                         uint32_t o[32];
-                        tmem_load32(o_col + lanes + c, o);
-                        tmem_wait_load();
+                        tmem_load32(col, o);
+                        tmem_wait_load32(o);
 #pragma unroll
                         for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tmem_store32(o_col + lanes + c, o);
+                        tmem_store32(col, o);
                     }
+                    tmem_wait_store();
+                    tc_fence_before();
+                    pair_sync(pair);  // the first half's weights release a product that adds to all of O
+                    tc_fence_after();
                 }
             }
             const float down = ref == -INFINITY ? 0.0f : ref;
+            Pair sum[2] = {0, 0};
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 1; c >= 0; --c) {
                 uint32_t p[16];
                 const float f = factor * sc[c], vf = sc[4 + c] * v_down;
-                if (ragged) l += weights_of<true>(s + c * 32, f, vf, down, lim - tok - c * 32, p);
-                else l += weights_of<false>(s + c * 32, f, vf, down, 32, p);
-                tmem_store16(s_col + lanes + c * 16, p);
-                if (c & 1) {
-                    tmem_wait_store();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(p_ready + (c >> 1) * 8);
+                if (c == 0) {
+                    tmem_load32(s_col, s);
+                    tmem_wait_load32(s);
                 }
+                if (ragged) weigh<true>(s, f, vf, down, live - c * 32, p, sum);
+                else weigh<false>(s, f, vf, down, 32, p, sum);
+                tmem_store16(s_col + c * 32, p);
             }
+            tmem_wait_store();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(p_ready);
+            float sum_a, sum_b;
+            unpair(add2(sum[0], sum[1]), sum_a, sum_b);
+            l += sum_a + sum_b;
         }
         if (steps > 0) {
             mbar_wait(s_full, tiles & 1, dead);
             __syncwarp();
             tc_fence_after();
         }
+        // the row's sum; the operands' memory is free once the last product is done (or holds none)
+        volatile float* const sums = reinterpret_cast<volatile float*>(smem + S::kKeys) + g * 256 + r;
+        if (steps > 0) {
+            sums[half * 128] = l;
+            pair_sync(pair);
+            l += sums[(half ^ 1) * 128];
+        }
         const float inv_l = *dead ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : v_up / l;
         const int t = row < a.rows ? row / a.group : 0, jj = row - t * a.group;
         const size_t orow = (head * a.group + jj) * a.tokens + t;
         uint16_t* const out = static_cast<uint16_t*>(a.out) + orow * a.head_dim;
-#pragma unroll
-        for (int c = 0; c < EP; c += 32) {
+#pragma unroll 1
+        for (int c0 = 0; c0 < EP / 2; c0 += 32) {
+            const int c = half * (EP / 2) + c0;  // element of the row
             uint32_t o[32];
             if (steps > 0) {
-                tmem_load32(o_col + lanes + c, o);
-                tmem_wait_load();
+                tmem_load32(o_col + c0, o);
+                tmem_wait_load32(o);
             }
 #pragma unroll
             for (int i = 0; i < 32; i += 8) {
@@ -590,7 +670,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
                     *reinterpret_cast<uint4*>(out + c + i) = make_uint4(q[0], q[1], q[2], q[3]);
             }
         }
-        if (row < a.rows) {
+        if (row < a.rows && half == 0) {
             const float lse2 = l == 0.0f ? -INFINITY : ref + log2f(l);
             if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
             if (lse2_out != nullptr) lse2_out[head * a.rows + row] = lse2;
@@ -598,7 +678,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
         tc_fence_before();
     }
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kConvertWarp) {
         tc_fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(S::kTmemCols) : "memory");
     }
