@@ -1106,7 +1106,8 @@ bool many_rows(const dt_kv_cache* c, int64_t rows) { return rows > 32 && c->head
 struct AttnPlan {
     int64_t rows, row_tiles;
     bool many_rows;
-    int grid;
+    KvPromptPlan prompt;  // of many rows
+    int grid;             // of few
     size_t out, stats, lse2, scores, bytes;  // offsets and the total
 };
 
@@ -1121,8 +1122,13 @@ int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool we
     p->grid = sms * attn_ctas_per_sm(c->head_dim);
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     p->out = 0;
-    p->stats = up(static_cast<size_t>(p->grid) * 2 * 16 * ep * 4);
-    p->lse2 = p->stats + up(static_cast<size_t>(p->grid) * 2 * 16 * 8);
+    if (p->many_rows) {
+        p->prompt = kv_prompt_plan(c->batch, p->rows, c->head_dim, sms);
+        p->lse2 = p->prompt.bytes;
+    } else {
+        p->stats = up(static_cast<size_t>(p->grid) * 2 * 16 * ep * 4);
+        p->lse2 = p->stats + up(static_cast<size_t>(p->grid) * 2 * 16 * 8);
+    }
     p->scores = p->lse2 + (weights ? up(static_cast<size_t>(c->batch) * c->kv_heads * p->rows * 4) : 0);
     p->bytes = p->scores;
     if (weights && stores_scores(c, p->rows))
@@ -1131,7 +1137,8 @@ int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool we
 }
 
 template <bool E4M3, int EP>
-int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, bool weights, cudaStream_t stream) {
+int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, void* workspace, bool weights,
+                  cudaStream_t stream) {
     using S = AttnShape<EP>;
     // per device and cheap: the limit belongs to the kernel in the current context
     cudaError_t e = cudaFuncSetAttribute(k_kv_attend<E4M3, EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
@@ -1140,7 +1147,7 @@ int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, b
     int st = DT_OK;
     unsigned grid = 0;
     if (p.many_rows) {
-        st = kv_prompt_attention(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, w.lse2, stream);
+        st = kv_prompt_attention(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.prompt, workspace, w.lse2, stream);
     } else {
         k_kv_attend<E4M3, EP><<<p.grid, kAttnThreads, S::kSmem, stream>>>(a, w, row_tiles);
         st = check_launch("dt_kv_attention");
@@ -1328,8 +1335,8 @@ int dt_kv_attention(const dt_kv_cache* cache, const void* query, int64_t query_h
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_head_dim(cache->head_dim, [&](auto ep) {
         constexpr int EP = decltype(ep)::value;
-        return cache->code == DT_KV_E4M3 ? launch_attend<true, EP>(a, w, p, weights != nullptr, s)
-                                         : launch_attend<false, EP>(a, w, p, weights != nullptr, s);
+        return cache->code == DT_KV_E4M3 ? launch_attend<true, EP>(a, w, p, workspace, weights != nullptr, s)
+                                         : launch_attend<false, EP>(a, w, p, workspace, weights != nullptr, s);
     });
 }
 

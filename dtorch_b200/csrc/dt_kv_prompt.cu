@@ -12,16 +12,18 @@ using namespace dtb;
 
 namespace {
 
-// 256 query rows of a key head (two tiles of 128) against tiles of 128 tokens, one CTA per SM:
+// 256 query rows of a key head (two tiles of 128) against tiles of 128 tokens, one CTA per SM. The tiles of all
+// (sequence, key head, 256 rows) items stand in one list, of which every CTA takes an equal stretch, whatever the lengths
+// and however few the rows: a stretch may end one item and begin the next. An item inside one stretch is finished
+// there; the others leave their parts in the workspace, and k_kv_prompt_merge joins them in the order of the list.
 //   warps 0-15       softmax: two warpgroups for each row tile, one for each half of the 128 columns; two threads share
 //                    a row. They read their scores from TMEM, agree on the row's reference, and write their weights
-//                    back as fp16 over columns that have been read, each half reported by itself.
+//                    back as fp16 over columns that have been read.
 //   warps 16-19      copy codes to shared memory a tile ahead (cp.async, every thread its own 16 bytes, so no barrier),
 //                    turn them into fp16 (exact) and store them as tcgen05 operands (128-byte swizzle), two stages of
 //                    keys and two of values.
-//   warp 20          issues every product: O += P V (P from TMEM, the halves as they come), then S = Q K^T of the next
-//                    tokens, for one row tile and then the other, so that one is in its softmax while the tensor core
-//                    works for the other.
+//   warp 20          issues every product: O += P V (P from TMEM), then S = Q K^T of the next tokens, for one row tile
+//                    and then the other, so that one is in its softmax while the tensor core works for the other.
 // TMEM, 512 columns: S of both row tiles (128 each, P in the first half of each), O of both (EP each). Products run in
 // the order of their issue, so a completed S also says that the O += P V before it is done.
 //
@@ -35,7 +37,7 @@ constexpr int kTokTile = 128;
 constexpr int kPromptThreads = 768;
 constexpr int kConvertWarp = 16, kIssueWarp = 20;
 // A softmax thread holds 64 scores; the block is launched with 80 registers a thread and shares them out anew.
-constexpr int kSoftmaxRegs = 96, kConvertRegs = 64, kIssueRegs = 32;
+constexpr int kSoftmaxRegs = 96, kConvertRegs = 48, kIssueRegs = 48;
 static_assert(512 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kIssueRegs <= kPromptThreads * 80,
               "a sum above the launch's waits forever");
 constexpr float kGrowth = 3.0f;
@@ -55,14 +57,13 @@ struct PromptShape {
     static constexpr int kCodeBytes = 128 * EP;
     static constexpr int kScales = kCodes + 2 * kCodeBytes;    // [ring][keys, values][4]
     static constexpr int kBars = kScales + kScaleRing * 2 * 4 * 4;
-    static constexpr int kTops = kBars + 256;                  // bfloat16 [parity][row tile][half][row]
-    static constexpr int kSmem = kTops + 2 * 2 * 2 * 128 * 2;  // barriers, TMEM address, flag, maxima before it
+    static constexpr int kTops = kBars + 256;                  // 8 bytes a row: bfloat16 [parity][half], or float [half]
+    static constexpr int kSmem = kTops + 2 * 128 * 8;
     static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
     static constexpr int kTmemCols = 512;
 };
 
-// kPReady: [row tile][half]
-enum Bar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kQReady = 14, kBarCount = 15 };
+enum Bar { kKFull = 0, kKEmpty = 2, kVFull = 4, kVEmpty = 6, kSFull = 8, kPReady = 10, kQReady = 12, kBarCount = 13 };
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return static_cast<uint32_t>(__cvta_generic_to_shared(p)); }
 
@@ -237,26 +238,33 @@ __device__ __forceinline__ float stage_query(const KvAttnArgs& a, const uint16_t
     return inv;
 }
 
-// Place of vector `v` (16 codes) of thread `tid` in a tile of 128 tokens. Eight lanes take four neighbouring vectors of
-// two rows: their halves, 16 bytes of fp16 each, then fall into eight different 16-byte columns of the swizzled panel.
-template <int EP>
-__device__ __forceinline__ void tile_place(int v, int tid, int& r, int& c) {
-    r = (v / (EP / 64)) * 32 + (tid >> 2);
-    c = (v % (EP / 64)) * 4 + (tid & 3);
-}
+// A tile of 128 tokens is moved as vectors of 16 codes, EP / 16 a thread. Thread `tid` has column c = tid % 4 and row
+// r = tid / 4; its vector v stands (v / panels) * 32 rows and (v % panels) * 4 columns further. So eight lanes take four
+// neighbouring vectors of two rows, whose halves, 16 bytes of fp16 each, fall into eight different 16-byte columns of
+// the swizzled panel; and every address is one of the thread's plus a constant.
 
-// Codes of a tile of 128 tokens to shared memory: 16 codes a copy, EP / 16 copies a thread, each thread its own.
+// Codes of a tile to shared memory, each thread its own.
 template <int EP>
 __device__ __forceinline__ void fetch_codes(uint32_t smem, const uint8_t* base, int tok, int len, int head_dim, int tid) {
+    constexpr int kPanels = EP / 64;
+    const int r = tid >> 2, c = tid & 3;
+    const uint32_t dst = smem + tid * 16;
+    if (head_dim == EP && tok + kTokTile <= len) {
+        const uint8_t* const p = base + static_cast<size_t>(tok + r) * EP + c * 16;
 #pragma unroll
-    for (int v = 0; v < EP / 16; ++v) {
-        int r, c;
-        tile_place<EP>(v, tid, r, c);
-        const bool live = tok + r < len && c * 16 < head_dim;
-        const uint8_t* const p = live ? base + static_cast<size_t>(tok + r) * head_dim + c * 16 : base;
-        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem + (v * 128 + tid) * 16), "l"(p),
-                     "r"(live ? 16 : 0)
-                     : "memory");
+        for (int v = 0; v < EP / 16; ++v)
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst + v * 2048),
+                         "l"(p + (v / kPanels) * 32 * EP + (v % kPanels) * 64)
+                         : "memory");
+    } else {
+#pragma unroll 1
+        for (int v = 0; v < EP / 16; ++v) {
+            const int row = tok + r + (v / kPanels) * 32, e = (c + (v % kPanels) * 4) * 16;
+            const bool live = row < len && e < head_dim;
+            const uint8_t* const p = live ? base + static_cast<size_t>(row) * head_dim + e : base;
+            asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst + v * 2048), "l"(p), "r"(live ? 16 : 0)
+                         : "memory");
+        }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
 }
@@ -264,18 +272,23 @@ __device__ __forceinline__ void fetch_codes(uint32_t smem, const uint8_t* base, 
 // The thread's own codes as fp16 operand rows.
 template <bool E4M3, int EP>
 __device__ __forceinline__ void store_operand(uint8_t* smem, const uint8_t* codes, int tid) {
+    constexpr int kPanels = EP / 64;
+    const int r = tid >> 2, c = tid & 3;
+    const uint8_t* const src = codes + tid * 16;
+    uint8_t* const dst_lo = smem + operand_offset(r, 2 * c);
+    uint8_t* const dst_hi = smem + operand_offset(r, 2 * c + 1);
 #pragma unroll
     for (int v = 0; v < EP / 16; ++v) {
-        int r, c;
-        tile_place<EP>(v, tid, r, c);
-        const uint4 w = *reinterpret_cast<const uint4*>(codes + (v * 128 + tid) * 16);
+        const uint4 w = *reinterpret_cast<const uint4*>(src + v * 2048);
         uint4 lo, hi;
         codes_to_half<E4M3, 0>(w.x, lo.x, lo.y);
         codes_to_half<E4M3, 0>(w.y, lo.z, lo.w);
         codes_to_half<E4M3, 0>(w.z, hi.x, hi.y);
         codes_to_half<E4M3, 0>(w.w, hi.z, hi.w);
-        *reinterpret_cast<uint4*>(smem + operand_offset(r, 2 * c)) = lo;
-        *reinterpret_cast<uint4*>(smem + operand_offset(r, 2 * c + 1)) = hi;
+        constexpr int kRows = 32 * 128;
+        const int off = (v / kPanels) * kRows + (v % kPanels) * (128 * 128);
+        *reinterpret_cast<uint4*>(dst_lo + off) = lo;
+        *reinterpret_cast<uint4*>(dst_hi + off) = hi;
     }
 }
 
@@ -357,8 +370,139 @@ __device__ __forceinline__ void weigh(const uint32_t* s, float f, float vf, floa
     }
 }
 
+constexpr int kItemRows = 2 * kRowTile;
+constexpr int kLeastTiles = 2;  // a stretch is not shorter: each part costs its queries' staging and a join
+
+// Tiles of 128 tokens that the rows of item `rt` of a sequence see; at least one, so that rows that see nothing are
+// written too. Rows are in the order of the tokens: the last live one sees the most.
+__device__ __forceinline__ int item_tiles(const KvAttnArgs& a, int rt, int len, int cnt) {
+    const int last = min(min((rt + 1) * kItemRows, a.rows), cnt * a.group) - 1;
+    const int most = last < rt * kItemRows ? 0 : kv_limit(a, last, len, cnt);
+    return max(1, (most + kTokTile - 1) / kTokTile);
+}
+
+// Where a CTA's stretch of the list begins: an item, and a tile of it.
+struct PromptStart {
+    int n, h, rt, tile;
+};
+
+struct PromptList {
+    int64_t total;  // tiles
+    int64_t each;   // of every stretch but the last
+};
+
+// x / y, in 32 bits where both fit: 64-bit division takes over a hundred instructions.
+__device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
+    if (((x | y) >> 32) == 0) return static_cast<uint32_t>(x) / static_cast<uint32_t>(y);
+    return x / y;
+}
+
+// Lays out the list, in one block. prefix[n][rt]: tiles of a head's items before item rt of sequence n, and of all of
+// them at prefix[n][row_tiles]; base[n]: tiles of the sequences before n.
+__global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptList* list, PromptStart* starts,
+                                                         int64_t* prefix, int64_t* base, int row_tiles, int ctas) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    for (int n = warp; n < a.batch; n += 32) {
+        const int len = kv_length(a.lengths, n, a.capacity), cnt = kv_count(a.counts, n, a.tokens);
+        int64_t* const out = prefix + static_cast<int64_t>(n) * (row_tiles + 1);
+        int64_t done = 0;
+        for (int r0 = 0; r0 < row_tiles; r0 += 32) {
+            const int rt = r0 + lane;
+            const int64_t mine = rt < row_tiles ? item_tiles(a, rt, len, cnt) : 0;
+            int64_t incl = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += o;
+            }
+            if (rt < row_tiles) out[rt] = done + incl - mine;
+            done += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) out[row_tiles] = done;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        int64_t done = 0;
+        for (int n0 = 0; n0 < a.batch; n0 += 32) {
+            const int n = n0 + lane;
+            const int64_t mine = n < a.batch ? prefix[static_cast<int64_t>(n) * (row_tiles + 1) + row_tiles] * a.kv_heads : 0;
+            int64_t incl = mine;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += o;
+            }
+            if (n < a.batch) base[n] = done + incl - mine;
+            done += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        if (lane == 0) {
+            base[a.batch] = done;
+            *list = PromptList{done, max(quotient(done + ctas - 1, ctas), static_cast<int64_t>(kLeastTiles))};
+        }
+    }
+    __syncthreads();
+    const PromptList l = *list;
+    for (int b = threadIdx.x; b < ctas; b += 1024) {
+        int64_t x = l.each * b;
+        if (x >= l.total) continue;
+        const auto find = [](const int64_t* p, int n, int64_t v) {  // the last i < n with p[i] <= v
+            int lo = 0, hi = n;
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (p[mid] <= v) lo = mid;
+                else hi = mid;
+            }
+            return lo;
+        };
+        PromptStart s;
+        s.n = find(base, a.batch, x);
+        x -= base[s.n];
+        const int64_t* const p = prefix + static_cast<int64_t>(s.n) * (row_tiles + 1);
+        s.h = static_cast<int>(quotient(x, p[row_tiles]));
+        x -= s.h * p[row_tiles];
+        s.rt = find(p, row_tiles, x);
+        s.tile = static_cast<int>(x - p[s.rt]);
+        starts[b] = s;
+    }
+}
+
+struct PromptParts {
+    float* out;             // [slot][256][EP], unnormalised
+    float2* stats;          // [slot][256]: reference (log2), sum
+    const PromptList* list;
+    const PromptStart* starts;
+    const int64_t* prefix;
+    float* lse2;            // [batch * kv_heads][rows], or null
+};
+
+// An item of the list, from one of its tiles on.
+struct PromptItem {
+    int n, h, rt, tile, tiles;
+
+    __device__ __forceinline__ PromptItem(const PromptParts& w, int row_tiles, const PromptStart& s)
+        : n(s.n), h(s.h), rt(s.rt), tile(s.tile) {
+        measure(w, row_tiles);
+    }
+    __device__ __forceinline__ void measure(const PromptParts& w, int row_tiles) {
+        const int64_t* const p = w.prefix + static_cast<int64_t>(n) * (row_tiles + 1) + rt;
+        tiles = static_cast<int>(p[1] - p[0]);
+    }
+    // The next item, whole.
+    __device__ __forceinline__ void next(const PromptParts& w, int row_tiles, int kv_heads) {
+        tile = 0;
+        if (++rt == row_tiles) {
+            rt = 0;
+            if (++h == kv_heads) {
+                h = 0;
+                ++n;
+            }
+        }
+        measure(w, row_tiles);
+    }
+};
+
 template <bool E4M3, int EP>
-__global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, float* lse2_out, int row_tiles) {
+__global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, PromptParts w, int row_tiles) {
     using S = PromptShape<EP>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_addr(smem);
@@ -366,21 +510,13 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
     float* const scales = reinterpret_cast<float*>(smem + S::kScales);
     volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + kBarCount * 8);
     volatile uint32_t* const dead = tmem_slot + 1;
-    volatile float* const vmax_slot = reinterpret_cast<volatile float*>(tmem_slot + 2);  // [24]
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
 
-    // the row tiles that see the most tokens first
-    const size_t head = blockIdx.x % (static_cast<unsigned>(a.batch) * a.kv_heads);
-    const int rt = row_tiles - 1 - static_cast<int>(blockIdx.x / (static_cast<unsigned>(a.batch) * a.kv_heads));
-    const int n = static_cast<int>(head / a.kv_heads), h = static_cast<int>(head % a.kv_heads);
-    const int len = kv_length(a.lengths, n, a.capacity), cnt = kv_count(a.counts, n, a.tokens);
-    const int row0 = rt * 2 * kRowTile;
-    // rows are in the order of the tokens: the last live one sees the most
-    const int last = min(min(row0 + 2 * kRowTile, a.rows), cnt * a.group) - 1;
-    const int most = last < row0 ? 0 : kv_limit(a, last, len, cnt);
-    const int tiles = (most + kTokTile - 1) / kTokTile;
-    const float* const ks = a.key_scale + head * a.nblocks;
-    const float* const vs = a.value_scale + head * a.nblocks;
+    const PromptList list = *w.list;
+    const int64_t x_begin = list.each * blockIdx.x;
+    if (x_begin >= list.total) return;
+    const int count = static_cast<int>(min(list.each, list.total - x_begin));  // tiles of this CTA
+    const PromptStart start = w.starts[blockIdx.x];
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -389,8 +525,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
             mbar_init(bars + (kVFull + i) * 8, 128);
             mbar_init(bars + (kVEmpty + i) * 8, 1);
             mbar_init(bars + (kSFull + i) * 8, 1);
-            mbar_init(bars + (kPReady + i) * 8, 4);
-            mbar_init(bars + (kPReady + 2 + i) * 8, 4);
+            mbar_init(bars + (kPReady + i) * 8, 8);
         }
         mbar_init(bars + kQReady * 8, kConvertWarp);
         *dead = 0;
@@ -402,28 +537,26 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
-    // a power of two that no value scale of these tokens exceeds
-    float vmax = 0.0f;
-    const int nb = (most + (1 << a.block_shift) - 1) >> a.block_shift;
-    for (int i = tid; i < nb; i += kPromptThreads) vmax = fmaxf(vmax, vs[i]);
-#pragma unroll
-    for (int d = 16; d > 0; d >>= 1) vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, d));
-    if (lane == 0) vmax_slot[warp] = vmax;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
-
-    const int row_groups = row0 + kRowTile < a.rows ? 2 : 1;  // row tiles that hold rows
     constexpr uint32_t kScoreInstr = instr_desc(kTokTile, false), kOutInstr = instr_desc(EP, true);
 
+    // Every role walks the same items. Stages and phases go by running counts over all of them.
     if (warp >= kIssueWarp) {
         // ---- products ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kIssueRegs));
-        if (warp == kIssueWarp && tiles > 0) {
-            const auto scores = [&](int g, int j) {
+        if (warp == kIssueWarp) {
+            const auto await = [&](int bar, uint32_t count) {
+                mbar_wait(bars + bar * 8, count & 1, dead);
+                __syncwarp();
+                tc_fence_after();
+            };
+            // c: tiles of this CTA before the one in question
+            const auto scores = [&](int g, uint32_t c, bool last_group) {
                 const uint64_t q_desc = operand_desc(base + S::kQuery + g * S::kOperand, 16, 1024);
-                const uint64_t k_desc = operand_desc(base + S::kKeys + (j & 1) * S::kOperand, 16, 1024);
+                const uint64_t k_desc = operand_desc(base + S::kKeys + (c & 1) * S::kOperand, 16, 1024);
                 if (elect_one()) {
 #pragma unroll
                     for (int k = 0; k < EP / 16; ++k) {
@@ -431,249 +564,304 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
                         mma_ss(tmem + g * 128, q_desc + off, k_desc + off, kScoreInstr, k > 0);
                     }
                     tc_commit(bars + (kSFull + g) * 8);
-                    if (g + 1 == row_groups) tc_commit(bars + (kKEmpty + (j & 1)) * 8);
+                    if (last_group) tc_commit(bars + (kKEmpty + (c & 1)) * 8);
                 }
                 __syncwarp();
             };
-            const auto outputs = [&](int g, int j, int half) {
-                const uint64_t v_desc = operand_desc(base + S::kValues + (j & 1) * S::kOperand, S::kPanelBytes, 1024);
+            const auto outputs = [&](int g, uint32_t c, bool first_tile, bool last_tile, bool last_group) {
+                const uint64_t v_desc = operand_desc(base + S::kValues + (c & 1) * S::kOperand, S::kPanelBytes, 1024);
                 if (elect_one()) {
 #pragma unroll
-                    for (int k = 0; k < kTokTile / 32; ++k) {
-                        const int kk = half * (kTokTile / 32) + k;
-                        mma_ts(tmem + 256 + g * EP, tmem + g * 128 + (kk >> 1) * 32 + (kk & 1) * 8, v_desc + kk * (2048 >> 4), kOutInstr,
-                               j > 0 || kk > 0);
+                    for (int k = 0; k < kTokTile / 16; ++k)
+                        mma_ts(tmem + 256 + g * EP, tmem + g * 128 + (k >> 1) * 32 + (k & 1) * 8, v_desc + k * (2048 >> 4),
+                               kOutInstr, !first_tile || k > 0);
+                    if (last_group) tc_commit(bars + (kVEmpty + (c & 1)) * 8);
+                    if (last_tile) tc_commit(bars + (kSFull + g) * 8);
+                }
+                __syncwarp();
+            };
+            uint32_t c = 0, items = 0, c_group1 = 0;  // tiles, items, and tiles of row tile 1 so far
+            PromptItem pos(w, row_tiles, start);
+            for (int left = count;;) {
+                const int steps = min(pos.tiles - pos.tile, left);
+                const int groups = pos.rt * kItemRows + kRowTile < a.rows ? 2 : 1;
+                await(kQReady, items);
+                await(kKFull + (c & 1), c >> 1);
+                scores(0, c, groups == 1);
+                if (groups == 2) scores(1, c, true);
+                for (int j = 0; j < steps; ++j, ++c) {
+                    const bool more = j + 1 < steps;
+                    await(kVFull + (c & 1), c >> 1);
+                    if (more) await(kKFull + ((c + 1) & 1), (c + 1) >> 1);
+#pragma unroll
+                    for (int g = 0; g < 2; ++g) {
+                        if (g < groups) {
+                            const uint32_t mine = g == 0 ? c : c_group1;
+                            await(kPReady + g, mine);
+                            outputs(g, c, j == 0, !more, g + 1 == groups);
+                            if (more) scores(g, c + 1, g + 1 == groups);
+                        }
                     }
-                    if (half == 1 && g + 1 == row_groups) tc_commit(bars + (kVEmpty + (j & 1)) * 8);
-                    if (half == 1 && j + 1 == tiles) tc_commit(bars + (kSFull + g) * 8);
+                    c_group1 += groups - 1;
                 }
-                __syncwarp();
-            };
-            const auto await = [&](int bar, int parity) {
-                mbar_wait(bars + bar * 8, parity, dead);
-                __syncwarp();
-                tc_fence_after();
-            };
-            await(kQReady, 0);
-            await(kKFull, 0);
-            for (int g = 0; g < row_groups; ++g) scores(g, 0);
-            for (int j = 0; j < tiles; ++j) {
-                const bool more = j + 1 < tiles;
-                await(kVFull + (j & 1), (j >> 1) & 1);
-                if (more) await(kKFull + ((j + 1) & 1), ((j + 1) >> 1) & 1);
-                for (int g = 0; g < row_groups; ++g) {
-                    await(kPReady + g * 2, j & 1);
-                    outputs(g, j, 0);
-                    await(kPReady + g * 2 + 1, j & 1);
-                    outputs(g, j, 1);
-                    if (more) scores(g, j + 1);
-                }
+                ++items;
+                left -= steps;
+                if (left == 0) break;
+                pos.next(w, row_tiles, a.kv_heads);
             }
         }
     } else if (warp >= kConvertWarp) {
         // ---- keys and values to fp16 operands ----
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kConvertRegs));
         const int t = tid - kConvertWarp * 32;
-        const uint8_t* const kbase = a.key + head * a.capacity * a.head_dim;
-        const uint8_t* const vbase = a.value + head * a.capacity * a.head_dim;
         uint8_t* const kcodes = smem + S::kCodes;
         uint8_t* const vcodes = kcodes + S::kCodeBytes;
-        if (tiles > 0) {
-            fetch_codes<EP>(smem_addr(kcodes), kbase, 0, len, a.head_dim, t);
-            fetch_codes<EP>(smem_addr(vcodes), vbase, 0, len, a.head_dim, t);
-        }
-        for (int j = 0; j < tiles; ++j) {
-            const int st = j & 1;
-            const uint32_t free_parity = ((j >> 1) & 1) ^ 1;
-            // behind the last tile nothing is fetched: every copy is of tokens < len or of no bytes
-            const int next = j + 1 < tiles ? (j + 1) * kTokTile : len;
-            float sc = 0.0f;
-            if (t < 8) {  // the scales of the tile's four spans of 32 tokens; 0 behind the length
-                const int tok = j * kTokTile + (t & 3) * 32;
-                if (tok < len) sc = (t < 4 ? ks : vs)[tok >> a.block_shift];
+        uint32_t c = 0;
+        PromptItem pos(w, row_tiles, start);
+        for (int left = count;;) {
+            const int steps = min(pos.tiles - pos.tile, left);
+            const size_t head = static_cast<size_t>(pos.n) * a.kv_heads + pos.h;
+            const int len = kv_length(a.lengths, pos.n, a.capacity);
+            const uint8_t* const kbase = a.key + head * a.capacity * a.head_dim;
+            const uint8_t* const vbase = a.value + head * a.capacity * a.head_dim;
+            const float* const sbase = (t < 4 ? a.key_scale : a.value_scale) + head * a.nblocks;
+            fetch_codes<EP>(smem_addr(kcodes), kbase, pos.tile * kTokTile, len, a.head_dim, t);
+            fetch_codes<EP>(smem_addr(vcodes), vbase, pos.tile * kTokTile, len, a.head_dim, t);
+            for (int j = 0; j < steps; ++j, ++c) {
+                const int st = c & 1;
+                const uint32_t free_parity = ((c >> 1) & 1) ^ 1;
+                const int tok0 = (pos.tile + j) * kTokTile;
+                // behind the last tile nothing is fetched: every copy is of tokens < len or of no bytes
+                const int next = j + 1 < steps ? tok0 + kTokTile : len;
+                float sc = 0.0f;
+                if (t < 8) {  // the scales of the tile's four spans of 32 tokens; 0 behind the length
+                    const int tok = tok0 + (t & 3) * 32;
+                    if (tok < len) sc = sbase[tok >> a.block_shift];
+                }
+                mbar_wait(bars + (kKEmpty + st) * 8, free_parity, dead);
+                if (t < 8) scales[(c % kScaleRing) * 8 + t] = sc;
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                store_operand<E4M3, EP>(smem + S::kKeys + st * S::kOperand, kcodes, t);
+                async_proxy_fence();
+                mbar_arrive(bars + (kKFull + st) * 8);
+                fetch_codes<EP>(smem_addr(kcodes), kbase, next, len, a.head_dim, t);
+                mbar_wait(bars + (kVEmpty + st) * 8, free_parity, dead);
+                asm volatile("cp.async.wait_group 1;" ::: "memory");
+                store_operand<E4M3, EP>(smem + S::kValues + st * S::kOperand, vcodes, t);
+                async_proxy_fence();
+                mbar_arrive(bars + (kVFull + st) * 8);
+                fetch_codes<EP>(smem_addr(vcodes), vbase, next, len, a.head_dim, t);
             }
-            mbar_wait(bars + (kKEmpty + st) * 8, free_parity, dead);
-            if (t < 8) scales[(j % kScaleRing) * 8 + t] = sc;
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            store_operand<E4M3, EP>(smem + S::kKeys + st * S::kOperand, kcodes, t);
-            async_proxy_fence();
-            mbar_arrive(bars + (kKFull + st) * 8);
-            fetch_codes<EP>(smem_addr(kcodes), kbase, next, len, a.head_dim, t);
-            mbar_wait(bars + (kVEmpty + st) * 8, free_parity, dead);
-            asm volatile("cp.async.wait_group 1;" ::: "memory");
-            store_operand<E4M3, EP>(smem + S::kValues + st * S::kOperand, vcodes, t);
-            async_proxy_fence();
-            mbar_arrive(bars + (kVFull + st) * 8);
-            fetch_codes<EP>(smem_addr(vcodes), vbase, next, len, a.head_dim, t);
+            asm volatile("cp.async.wait_group 0;" ::: "memory");
+            left -= steps;
+            if (left == 0) break;
+            pos.next(w, row_tiles, a.kv_heads);
         }
-        asm volatile("cp.async.wait_group 0;" ::: "memory");
     } else {
         // ---- softmax of a row tile ----
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
         // row tile, half of the columns, row, and the barrier and places shared with the row's other thread
-        const int g = warp >> 3, half = (warp >> 2) & 1, r = tid & 127, row = row0 + g * kRowTile + r;
+        const int g = warp >> 3, half = (warp >> 2) & 1, r = tid & 127;
         const int pair = 1 + g * 4 + (warp & 3);
-        volatile uint16_t* const tops = reinterpret_cast<volatile uint16_t*>(smem + S::kTops) + g * 256 + r;  // + parity * 512
-        float factor;
-        {
-            const uint16_t* qp = nullptr;
-            if (row < a.rows) {
-                const int t = row / a.group, jj = row - t * a.group;
-                qp = static_cast<const uint16_t*>(a.query) + n * a.q_stride_n +
-                     static_cast<int64_t>(h * a.group + jj) * a.q_stride_h + t * a.q_stride_t;
-            }
-            // the places of odd tiles: the first tile's are written before the other thread has read these
-            const float inv = stage_query<EP>(a, qp, smem + S::kQuery + g * S::kOperand, r, half, tops + 512 + half * 128,
-                                              tops + 512 + (half ^ 1) * 128, pair, a.scale_log2 < 0.0f ? -1.0f : 1.0f);
-            factor = inv * fabsf(a.scale_log2) * code_unit<E4M3>();
-            async_proxy_fence();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bars + kQReady * 8);
-        }
+        volatile uint16_t* const tops = reinterpret_cast<volatile uint16_t*>(smem + S::kTops) + (g * 128 + r) * 4;
+        volatile float* const sums = reinterpret_cast<volatile float*>(tops);
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         // this thread's columns of S; a span's weights lie over its own scores
         const uint32_t s_col = (tmem + g * 128 + half * 64) | lanes, o_col = (tmem + 256 + g * EP + half * (EP / 2)) | lanes;
-        const uint32_t s_full = bars + (kSFull + g) * 8, p_ready = bars + (kPReady + g * 2 + half) * 8;
-        float vtop = 0.0f;
+        const uint32_t s_full = bars + (kSFull + g) * 8, p_ready = bars + (kPReady + g) * 8;
+        uint32_t c = 0, phase = 0, items = 0;  // tiles, completions of S and items so far
+        PromptItem pos(w, row_tiles, start);
+        for (int left = count; left > 0; left > 0 ? pos.next(w, row_tiles, a.kv_heads) : (void)0) {
+            const int item_steps = min(pos.tiles - pos.tile, left);
+            const int len = kv_length(a.lengths, pos.n, a.capacity), cnt = kv_count(a.counts, pos.n, a.tokens);
+            const size_t head = static_cast<size_t>(pos.n) * a.kv_heads + pos.h;
+            const int row = pos.rt * kItemRows + g * kRowTile + r;
+            const bool live_group = pos.rt * kItemRows + g * kRowTile < a.rows;
+            float factor;
+            {
+                const uint16_t* qp = nullptr;
+                const int t = row / a.group, jj = row - t * a.group;
+                if (row < a.rows)
+                    qp = static_cast<const uint16_t*>(a.query) + pos.n * a.q_stride_n +
+                         static_cast<int64_t>(pos.h * a.group + jj) * a.q_stride_h + t * a.q_stride_t;
+                // in the places of odd tiles: the first tile's are written before the other thread has read these
+                const float inv = stage_query<EP>(a, qp, smem + S::kQuery + g * S::kOperand, r, half, tops + 2 + half,
+                                                  tops + 2 + (half ^ 1), pair, a.scale_log2 < 0.0f ? -1.0f : 1.0f);
+                factor = inv * fabsf(a.scale_log2) * code_unit<E4M3>();
+                tc_fence_before();  // the reads of O of the item before
+                async_proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(bars + kQReady * 8);
+            }
+            // a power of two that no value scale of these tiles exceeds
+            float vtop = 0.0f;
+            {
+                const float* const vs = a.value_scale + head * a.nblocks;
+                const int first = (pos.tile * kTokTile) >> a.block_shift;
+                const int end = min((pos.tile + item_steps) * kTokTile, len);
+                for (int i = first + lane; i < (end + (1 << a.block_shift) - 1) >> a.block_shift; i += 32)
+                    vtop = fmaxf(vtop, vs[i]);
 #pragma unroll
-        for (int i = 0; i < kPromptThreads / 32; ++i) vtop = fmaxf(vtop, vmax_slot[i]);
-        // 2^-e and 2^e with vtop < 2^e
-        int ve = static_cast<int>(__float_as_uint(vtop) >> 23) - 126;
-        ve = ve < -100 ? -100 : ve > 126 ? 126 : ve;
-        const float v_down = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23) * exp2f(kPromptShift);
-        const float v_up = __uint_as_float(static_cast<uint32_t>(127 + ve) << 23) * (code_unit<E4M3>() * exp2f(-kPromptShift));
+                for (int d = 16; d > 0; d >>= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
+            }
+            int ve = static_cast<int>(__float_as_uint(vtop) >> 23) - 126;  // vtop < 2^ve
+            ve = ve < -100 ? -100 : ve > 126 ? 126 : ve;
+            const float v_down = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23) * exp2f(kPromptShift);
+            int live = kv_limit(a, row, len, cnt) - pos.tile * kTokTile - half * 64;  // of this thread's columns
 
-        const int lim = kv_limit(a, row, len, cnt);
-        float ref = -INFINITY, l = 0.0f;
-        const int steps = g < row_groups ? tiles : 0;
-        for (int j = 0; j < steps; ++j) {
-            mbar_wait(s_full, j & 1, dead);
-            __syncwarp();
-            tc_fence_after();
-            const float* const sc = scales + (j % kScaleRing) * 8 + half * 2;
-            const int live = lim - j * kTokTile - half * 64;  // of these columns
-            const bool ragged = __any_sync(0xffffffffu, live < 64);
-            uint32_t s[32];
-            float top = -INFINITY;
-            // span 0 is loaded again for its weights: 32 scores fewer to hold meanwhile
-#pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                tmem_load32(s_col + c * 32, s);
+            float ref = -INFINITY, l = 0.0f;
+            const int steps = live_group ? item_steps : 0;
+            for (int j = 0; j < steps; ++j) {
+                mbar_wait(s_full, phase & 1, dead);
+                ++phase;
+                __syncwarp();
+                tc_fence_after();
+                const float* const sc = scales + ((c + j) % kScaleRing) * 8 + half * 2;
+                const bool ragged = __any_sync(0xffffffffu, live < 64);
+                uint32_t s[32], s0[32];
+                float top = -INFINITY;
+                // span 0 is loaded again for its weights: 32 scores fewer to hold meanwhile
+                tmem_load32(s_col, s0);
+                tmem_load32(s_col + 32, s);
+                tmem_wait_load32(s0);
                 tmem_wait_load32(s);
-                uint32_t* const x = s;
-                if (ragged) {
 #pragma unroll
-                    for (int i = 0; i < 32; ++i)
-                        if (c * 32 + i >= live) x[i] = 0xff800000u;
-                }
-                float mx[2] = {fmaxf(__uint_as_float(x[0]), __uint_as_float(x[1])),
-                               fmaxf(__uint_as_float(x[2]), __uint_as_float(x[3]))};
+                for (int k = 0; k < 2; ++k) {
+                    uint32_t* const v = k == 0 ? s0 : s;
+                    if (ragged) {
 #pragma unroll
-                for (int i = 4; i < 32; i += 4) {
-                    mx[0] = max3(mx[0], __uint_as_float(x[i]), __uint_as_float(x[i + 1]));
-                    mx[1] = max3(mx[1], __uint_as_float(x[i + 2]), __uint_as_float(x[i + 3]));
-                }
-                const float m = fmaxf(mx[0], mx[1]);
-                if (m != -INFINITY) top = fmaxf(top, m * (factor * sc[c]));  // masked stays masked where the scale is 0
-            }
-            // the row's largest, of both halves, as bfloat16 rounded up: a reference need not be exact. The next use of
-            // these places is two tiles on, behind the other thread's barrier of the next.
-            const uint16_t top16 = round_up16(top);
-            tops[(j & 1) * 512 + half * 128] = top16;
-            pair_sync(pair);
-            top = fmaxf(from16(top16), from16(tops[(j & 1) * 512 + (half ^ 1) * 128]));
-            const bool grow = top > ref + kGrowth;  // also the first: ref is -infinity
-            if (__any_sync(0xffffffffu, grow)) {    // the same for both warps of the pair
-                const float now = grow ? top : ref;
-                const float alpha = grow ? ex2(ref - now) : 1.0f;
-                ref = now;
-                l *= alpha;
-                if (j > 0) {
-#pragma unroll 1
-                    for (int c = 0; c < EP / 2; c += 32) {
-                        const uint32_t col = o_col + c;
-                        uint32_t o[32];
-                        tmem_load32(col, o);
-                        tmem_wait_load32(o);
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
-                        tmem_store32(col, o);
+                        for (int i = 0; i < 32; ++i)
+                            if (k * 32 + i >= live) v[i] = 0xff800000u;
                     }
-                    tmem_wait_store();
-                    tc_fence_before();
-                    pair_sync(pair);  // the first half's weights release a product that adds to all of O
-                    tc_fence_after();
-                }
-            }
-            const float down = ref == -INFINITY ? 0.0f : ref;
-            Pair sum[2] = {0, 0};
+                    float mx[2] = {fmaxf(__uint_as_float(v[0]), __uint_as_float(v[1])),
+                                   fmaxf(__uint_as_float(v[2]), __uint_as_float(v[3]))};
 #pragma unroll
-            for (int c = 1; c >= 0; --c) {
-                uint32_t p[16];
-                const float f = factor * sc[c], vf = sc[4 + c] * v_down;
-                if (c == 0) {
-                    tmem_load32(s_col, s);
-                    tmem_wait_load32(s);
+                    for (int i = 4; i < 32; i += 4) {
+                        mx[0] = max3(mx[0], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                        mx[1] = max3(mx[1], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
+                    }
+                    const float m = fmaxf(mx[0], mx[1]);
+                    if (m != -INFINITY) top = fmaxf(top, m * (factor * sc[k]));  // masked stays so where the scale is 0
                 }
-                if (ragged) weigh<true>(s, f, vf, down, live - c * 32, p, sum);
-                else weigh<false>(s, f, vf, down, 32, p, sum);
-                tmem_store16(s_col + c * 32, p);
+                // the row's largest, of both halves, as bfloat16 rounded up: a reference need not be exact. The next use
+                // of these places is two tiles on, behind the other thread's barrier of the next.
+                const uint16_t top16 = round_up16(top);
+                tops[(j & 1) * 2 + half] = top16;
+                pair_sync(pair);
+                top = fmaxf(from16(top16), from16(tops[(j & 1) * 2 + (half ^ 1)]));
+                const bool grow = top > ref + kGrowth;  // also the first: ref is -infinity
+                if (__any_sync(0xffffffffu, grow)) {    // the same for both warps of the pair
+                    const float now = grow ? top : ref;
+                    const float alpha = grow ? ex2(ref - now) : 1.0f;
+                    ref = now;
+                    l *= alpha;
+                    if (j > 0) {
+#pragma unroll 1
+                        for (int k = 0; k < EP / 2; k += 32) {
+                            uint32_t o[32];
+                            tmem_load32(o_col + k, o);
+                            tmem_wait_load32(o);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * alpha);
+                            tmem_store32(o_col + k, o);
+                        }
+                    }
+                }
+                const float down = ref == -INFINITY ? 0.0f : ref;
+                Pair sum[2] = {0, 0};
+#pragma unroll
+                for (int k = 1; k >= 0; --k) {
+                    uint32_t p[16];
+                    const float f = factor * sc[k], vf = sc[4 + k] * v_down;
+                    if (k == 0) {
+                        tmem_load32(s_col, s);
+                        tmem_wait_load32(s);
+                    }
+                    if (ragged) weigh<true>(s, f, vf, down, live - k * 32, p, sum);
+                    else weigh<false>(s, f, vf, down, 32, p, sum);
+                    tmem_store16(s_col + k * 32, p);
+                }
+                tmem_wait_store();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(p_ready);
+                float sum_a, sum_b;
+                unpair(add2(sum[0], sum[1]), sum_a, sum_b);
+                l += sum_a + sum_b;
+                live -= kTokTile;
             }
-            tmem_wait_store();
-            tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(p_ready);
-            float sum_a, sum_b;
-            unpair(add2(sum[0], sum[1]), sum_a, sum_b);
-            l += sum_a + sum_b;
-        }
-        if (steps > 0) {
-            mbar_wait(s_full, tiles & 1, dead);
+            c += item_steps;
+            left -= item_steps;
+            ++items;
+            if (steps == 0) {  // no rows here: keep pace with the other row tile, whose warps report their queries too
+                mbar_wait(bars + kQReady * 8, (items - 1) & 1, dead);
+                __syncwarp();
+                continue;
+            }
+            mbar_wait(s_full, phase & 1, dead);
+            ++phase;
             __syncwarp();
             tc_fence_after();
-        }
-        // the row's sum; the operands' memory is free once the last product is done (or holds none)
-        volatile float* const sums = reinterpret_cast<volatile float*>(smem + S::kKeys) + g * 256 + r;
-        if (steps > 0) {
-            sums[half * 128] = l;
+            pair_sync(pair);  // the other thread has read the last tile's top
+            sums[half] = l;
             pair_sync(pair);
-            l += sums[(half ^ 1) * 128];
-        }
-        const float inv_l = *dead ? __int_as_float(0x7fc00000) : l == 0.0f ? 0.0f : v_up / l;
-        const int t = row < a.rows ? row / a.group : 0, jj = row - t * a.group;
-        const size_t orow = (head * a.group + jj) * a.tokens + t;
-        uint16_t* const out = static_cast<uint16_t*>(a.out) + orow * a.head_dim;
+            l += sums[half ^ 1];
+            pair_sync(pair);  // and both have read the sums, whose places take the next queries' tops
+            if (*dead) l = __int_as_float(0x7fc00000);
+            const float v_up = code_unit<E4M3>() / v_down;  // powers of two
+            if (item_steps < pos.tiles) {
+                // an item that other CTAs work on too: one that began before this stretch, or goes on behind it
+                const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (pos.tile > 0 ? 0 : 1);
+                const size_t at = slot * kItemRows + g * kRowTile + r;
+                float4* const out = reinterpret_cast<float4*>(w.out + at * EP + half * (EP / 2));
 #pragma unroll 1
-        for (int c0 = 0; c0 < EP / 2; c0 += 32) {
-            const int c = half * (EP / 2) + c0;  // element of the row
-            uint32_t o[32];
-            if (steps > 0) {
-                tmem_load32(o_col + c0, o);
-                tmem_wait_load32(o);
-            }
+                for (int k = 0; k < EP / 2; k += 32) {
+                    uint32_t o[32];
+                    tmem_load32(o_col + k, o);
+                    tmem_wait_load32(o);
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-                uint32_t q[4];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    // a row that saw nothing: its O may be anything where no tile was computed
-                    const float x = steps > 0 && l != 0.0f ? __uint_as_float(o[i + 2 * k]) * inv_l : 0.0f;
-                    const float y = steps > 0 && l != 0.0f ? __uint_as_float(o[i + 2 * k + 1]) * inv_l : 0.0f;
-                    if (a.query_bf16) {
-                        const __nv_bfloat162 b = __floats2bfloat162_rn(x, y);
-                        q[k] = *reinterpret_cast<const uint32_t*>(&b);
-                    } else {
-                        q[k] = pack_half2(x, y);
-                    }
+                    for (int i = 0; i < 32; i += 4)
+                        out[(k + i) / 4] = make_float4(__uint_as_float(o[i]) * v_up, __uint_as_float(o[i + 1]) * v_up,
+                                                       __uint_as_float(o[i + 2]) * v_up, __uint_as_float(o[i + 3]) * v_up);
                 }
-                if (row < a.rows && c + i < a.head_dim)
-                    *reinterpret_cast<uint4*>(out + c + i) = make_uint4(q[0], q[1], q[2], q[3]);
+                if (half == 0) w.stats[at] = make_float2(ref, l);
+                continue;
             }
-        }
-        if (row < a.rows && half == 0) {
-            const float lse2 = l == 0.0f ? -INFINITY : ref + log2f(l);
-            if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
-            if (lse2_out != nullptr) lse2_out[head * a.rows + row] = lse2;
+            const float inv_l = v_up / l;
+            int at_end = row;
+            asm volatile("" : "+r"(at_end));  // worked out again: not held through the loop
+            const int t = at_end / a.group, jj = at_end - t * a.group;
+            const size_t orow = (head * a.group + jj) * a.tokens + t;
+            uint16_t* const out = static_cast<uint16_t*>(a.out) + orow * a.head_dim;
+#pragma unroll 1
+            for (int k0 = 0; k0 < EP / 2; k0 += 32) {
+                const int k = half * (EP / 2) + k0;  // element of the row
+                uint32_t o[32];
+                tmem_load32(o_col + k0, o);
+                tmem_wait_load32(o);
+#pragma unroll
+                for (int i = 0; i < 32; i += 8) {
+                    uint32_t q[4];
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const float u = l == 0.0f ? 0.0f : __uint_as_float(o[i + 2 * e]) * inv_l;
+                        const float v = l == 0.0f ? 0.0f : __uint_as_float(o[i + 2 * e + 1]) * inv_l;
+                        if (a.query_bf16) {
+                            const __nv_bfloat162 b = __floats2bfloat162_rn(u, v);
+                            q[e] = *reinterpret_cast<const uint32_t*>(&b);
+                        } else {
+                            q[e] = pack_half2(u, v);
+                        }
+                    }
+                    if (row < a.rows && k + i < a.head_dim)
+                        *reinterpret_cast<uint4*>(out + k + i) = make_uint4(q[0], q[1], q[2], q[3]);
+                }
+            }
+            if (row < a.rows && half == 0) {
+                const float lse2 = l == 0.0f ? -INFINITY : ref + log2f(l);
+                if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
+                if (w.lse2 != nullptr) w.lse2[head * a.rows + row] = lse2;
+            }
         }
         tc_fence_before();
     }
@@ -684,15 +872,91 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, f
     }
 }
 
+constexpr int kMergeRows = 64;
+
+// Joins the parts of the items that more than one CTA of k_kv_prompt worked on: a block for each boundary between two
+// stretches and 64 of an item's 256 rows, 16 lanes for a row at a time. The item's first boundary does the work.
+template <int EP>
+__global__ void __launch_bounds__(256) k_kv_prompt_merge(KvAttnArgs a, PromptParts w, int row_tiles) {
+    const PromptList list = *w.list;
+    if (list.each * (blockIdx.x + 1) >= list.total) return;
+    const PromptItem pos(w, row_tiles, w.starts[blockIdx.x + 1]);
+    // an item that begins here, or before the stretch that ends here, is not this block's
+    if (pos.tile == 0 || pos.tile > list.each) return;
+    const int c0 = blockIdx.x, parts = 2 + (pos.tiles - pos.tile - 1) / static_cast<int>(list.each);
+    const int lane = threadIdx.x & 15;
+    constexpr int kVec = EP / 64;  // float4 of the row a lane has
+    const size_t head = static_cast<size_t>(pos.n) * a.kv_heads + pos.h;
+    for (int i = threadIdx.x >> 4; i < kMergeRows; i += 16) {
+        const int r = blockIdx.y * kMergeRows + i, row = pos.rt * kItemRows + r;
+        if (row >= a.rows) return;
+        // part k is in slot 2 (c0 + k) but for the first, which goes on behind its stretch: 2 c0 + 1
+        const float2* const stats = w.stats + static_cast<size_t>(c0) * 2 * kItemRows + r;
+        const float4* const out = reinterpret_cast<const float4*>(w.out + (static_cast<size_t>(c0) * 2 * kItemRows + r) * EP) + lane;
+        float m = -INFINITY;
+        for (int k = 0; k < parts; ++k) m = fmaxf(m, stats[(k == 0 ? 1 : 2 * k) * kItemRows].x);
+        float l = 0.0f;
+        float4 acc[kVec];
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int k = 0; k < parts; ++k) {
+            const int64_t at = static_cast<int64_t>(k == 0 ? 1 : 2 * k) * kItemRows;
+            const float2 st = stats[at];
+            const float f = st.x == m ? 1.0f : ex2(st.x - m);
+            l += st.y * f;
+#pragma unroll
+            for (int v = 0; v < kVec; ++v) {
+                const float4 o = out[at * (EP / 4) + v * 16];
+                acc[v].x = fmaf(o.x, f, acc[v].x);
+                acc[v].y = fmaf(o.y, f, acc[v].y);
+                acc[v].z = fmaf(o.z, f, acc[v].z);
+                acc[v].w = fmaf(o.w, f, acc[v].w);
+            }
+        }
+        const float g = l == 0.0f ? 0.0f : 1.0f / l;
+        const int t = row / a.group, jj = row - t * a.group;
+        const size_t orow = (head * a.group + jj) * a.tokens + t;
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+            const int e = (v * 16 + lane) * 4;
+            if (e >= a.head_dim) continue;
+            uint2 u;
+            if (a.query_bf16) {
+                const __nv_bfloat162 lo = __floats2bfloat162_rn(acc[v].x * g, acc[v].y * g);
+                const __nv_bfloat162 hi = __floats2bfloat162_rn(acc[v].z * g, acc[v].w * g);
+                u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            } else {
+                u = make_uint2(pack_half2(acc[v].x * g, acc[v].y * g), pack_half2(acc[v].z * g, acc[v].w * g));
+            }
+            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) = u;
+        }
+        if (lane == 0) {
+            const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
+            if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
+            if (w.lse2 != nullptr) w.lse2[head * a.rows + row] = lse2;
+        }
+    }
+}
+
 template <bool E4M3, int EP>
-int launch(const KvAttnArgs& a, float* lse2, cudaStream_t stream) {
+int launch(const KvAttnArgs& a, const KvPromptPlan& p, char* ws, float* lse2, cudaStream_t stream) {
     using S = PromptShape<EP>;
     cudaError_t e = cudaFuncSetAttribute(k_kv_prompt<E4M3, EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
     if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
-    const int row_tiles = (a.rows + 2 * kRowTile - 1) / (2 * kRowTile);
-    const int64_t ctas = static_cast<int64_t>(row_tiles) * a.batch * a.kv_heads;
-    if (ctas > INT32_MAX) return set_error(DT_ERR_INVALID, "dt_kv_attention: too many blocks");
-    k_kv_prompt<E4M3, EP><<<static_cast<unsigned>(ctas), kPromptThreads, S::kSmem, stream>>>(a, lse2, row_tiles);
+    const int row_tiles = (a.rows + kItemRows - 1) / kItemRows;
+    int64_t* const prefix = reinterpret_cast<int64_t*>(ws + p.prefix);
+    PromptList* const list = reinterpret_cast<PromptList*>(ws + p.list);
+    PromptStart* const starts = reinterpret_cast<PromptStart*>(ws + p.starts);
+    const PromptParts w{reinterpret_cast<float*>(ws + p.out), reinterpret_cast<float2*>(ws + p.stats), list, starts, prefix,
+                        lse2};
+    k_kv_prompt_plan<<<1, 1024, 0, stream>>>(a, list, starts, prefix,
+                                             prefix + static_cast<int64_t>(a.batch) * (row_tiles + 1), row_tiles, p.ctas);
+    int st = check_launch("dt_kv_attention");
+    if (st != DT_OK) return st;
+    k_kv_prompt<E4M3, EP><<<p.ctas, kPromptThreads, S::kSmem, stream>>>(a, w, row_tiles);
+    st = check_launch("dt_kv_attention");
+    if (st != DT_OK || p.ctas < 2) return st;
+    k_kv_prompt_merge<EP><<<dim3(p.ctas - 1, kItemRows / kMergeRows), 256, 0, stream>>>(a, w, row_tiles);
     return check_launch("dt_kv_attention");
 }
 
@@ -700,10 +964,26 @@ int launch(const KvAttnArgs& a, float* lse2, cudaStream_t stream) {
 
 namespace dtb {
 
-int kv_prompt_attention(const KvAttnArgs& a, int code, float* lse2, cudaStream_t stream) {
+KvPromptPlan kv_prompt_plan(int64_t batch, int64_t rows, int64_t head_dim, int sms) {
+    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    const size_t ep = head_dim <= 64 ? 64 : 128, row_tiles = (rows + kItemRows - 1) / kItemRows;
+    KvPromptPlan p{};
+    p.ctas = sms;
+    p.out = 0;
+    p.stats = up(static_cast<size_t>(sms) * 2 * kItemRows * ep * 4);
+    p.list = p.stats + up(static_cast<size_t>(sms) * 2 * kItemRows * 8);
+    p.starts = p.list + up(sizeof(PromptList));
+    p.prefix = p.starts + up(static_cast<size_t>(sms) * sizeof(PromptStart));
+    p.bytes = p.prefix + up((static_cast<size_t>(batch) * (row_tiles + 1) + batch + 1) * 8);
+    return p;
+}
+
+int kv_prompt_attention(const KvAttnArgs& a, int code, const KvPromptPlan& p, void* workspace, float* lse2,
+                        cudaStream_t stream) {
+    char* const ws = static_cast<char*>(workspace);
     if (a.head_dim <= 64)
-        return code == DT_KV_E4M3 ? launch<true, 64>(a, lse2, stream) : launch<false, 64>(a, lse2, stream);
-    return code == DT_KV_E4M3 ? launch<true, 128>(a, lse2, stream) : launch<false, 128>(a, lse2, stream);
+        return code == DT_KV_E4M3 ? launch<true, 64>(a, p, ws, lse2, stream) : launch<false, 64>(a, p, ws, lse2, stream);
+    return code == DT_KV_E4M3 ? launch<true, 128>(a, p, ws, lse2, stream) : launch<false, 128>(a, p, ws, lse2, stream);
 }
 
 }  // namespace dtb
