@@ -1108,7 +1108,9 @@ struct AttnPlan {
     bool many_rows;
     KvPromptPlan prompt;  // of many rows
     int grid;             // of few
-    size_t out, stats, lse2, scores, bytes;  // offsets and the total
+    KvColumnPlan columns;  // weights of many rows, on tensor cores
+    bool column_tiles;
+    size_t out, stats, lse2, scores, bytes;  // offsets and the total (scores: or the columns' workspace)
 };
 
 int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool weights, AttnPlan* p) {
@@ -1131,8 +1133,13 @@ int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool we
     }
     p->scores = p->lse2 + (weights ? up(static_cast<size_t>(c->batch) * c->kv_heads * p->rows * 4) : 0);
     p->bytes = p->scores;
-    if (weights && stores_scores(c, p->rows))
+    if (weights && stores_scores(c, p->rows)) {
         p->bytes += static_cast<size_t>(c->batch) * c->kv_heads * 16 * c->capacity * 4;
+    } else if (weights && c->head_dim <= 128) {
+        p->column_tiles = true;
+        p->columns = kv_column_plan(c->batch, c->kv_heads, p->rows, c->head_dim, c->capacity, sms);
+        p->bytes += p->columns.bytes;
+    }
     return DT_OK;
 }
 
@@ -1163,6 +1170,9 @@ int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, v
         const unsigned y = static_cast<unsigned>(std::min<int64_t>(heads, 32768));
         const dim3 g(static_cast<unsigned>((a.capacity + 1023) / 1024), y, static_cast<unsigned>((heads + y - 1) / y));
         k_kv_weights<<<g, 256, 0, stream>>>(a, w);
+    } else if (p.column_tiles) {
+        return kv_column_sums(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.columns, static_cast<char*>(workspace) + p.scores, w.lse2,
+                              stream);
     } else {
         const int key_tiles = static_cast<int>((a.capacity + kTile - 1) / kTile);
         st = grid_of(heads * key_tiles, "dt_kv_attention", &grid);
@@ -1331,7 +1341,7 @@ int dt_kv_attention(const dt_kv_cache* cache, const void* query, int64_t query_h
     w.out = reinterpret_cast<float*>(ws + p.out);
     w.stats = reinterpret_cast<float2*>(ws + p.stats);
     w.lse2 = weights != nullptr ? reinterpret_cast<float*>(ws + p.lse2) : nullptr;
-    w.scores = p.bytes > p.scores ? reinterpret_cast<float*>(ws + p.scores) : nullptr;
+    w.scores = p.bytes > p.scores && !p.column_tiles ? reinterpret_cast<float*>(ws + p.scores) : nullptr;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return with_head_dim(cache->head_dim, [&](auto ep) {
         constexpr int EP = decltype(ep)::value;

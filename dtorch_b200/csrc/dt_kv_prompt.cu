@@ -397,8 +397,25 @@ __device__ __forceinline__ int64_t quotient(int64_t x, int64_t y) {
     return x / y;
 }
 
-// Lays out the list, in one block. prefix[n][rt]: tiles of a head's items before item rt of sequence n, and of all of
-// them at prefix[n][row_tiles]; base[n]: tiles of the sequences before n.
+// Row tiles (of 128) that see a token of key tile `kt` of a sequence: all from the first of them on, as rows are in the
+// order of the tokens. At least one where the tile holds tokens, so that weights nobody gives are written as 0.
+__device__ __forceinline__ int key_tile_first_row(const KvAttnArgs& a, int kt, int len, int cnt) {
+    if (!a.causal) return 0;
+    // query i sees token t where t <= len - cnt + i
+    const int64_t i = max(kt * kTokTile - (len - cnt), 0);
+    const int64_t row_tiles = (a.rows + kRowTile - 1) / kRowTile;
+    return static_cast<int>(min(i * a.group / kRowTile, row_tiles - 1));
+}
+
+__device__ __forceinline__ int key_tile_rows(const KvAttnArgs& a, int kt, int len, int cnt) {
+    if (kt * kTokTile >= len) return 0;
+    return (a.rows + kRowTile - 1) / kRowTile - key_tile_first_row(a, kt, len, cnt);
+}
+
+// Lays out a list, in one block: of (sequence, head, 256 rows) items and their key tiles, or (COLUMNS) of (sequence,
+// head, 128 keys) items and their row tiles. prefix[n][i]: tiles of a head's items before item i of sequence n, and of
+// all of them at prefix[n][items]; base[n]: tiles of the sequences before n.
+template <bool COLUMNS>
 __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptList* list, PromptStart* starts,
                                                          int64_t* prefix, int64_t* base, int row_tiles, int ctas) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -408,7 +425,7 @@ __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptLis
         int64_t done = 0;
         for (int r0 = 0; r0 < row_tiles; r0 += 32) {
             const int rt = r0 + lane;
-            const int64_t mine = rt < row_tiles ? item_tiles(a, rt, len, cnt) : 0;
+            const int64_t mine = rt >= row_tiles ? 0 : COLUMNS ? key_tile_rows(a, rt, len, cnt) : item_tiles(a, rt, len, cnt);
             int64_t incl = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -487,14 +504,17 @@ struct PromptItem {
         const int64_t* const p = w.prefix + static_cast<int64_t>(n) * (row_tiles + 1) + rt;
         tiles = static_cast<int>(p[1] - p[0]);
     }
-    // The next item, whole.
+    // The next item that has tiles, whole; there is one. Empty items stand only behind a head's others (keys behind a
+    // sequence's length), and are passed over at once.
     __device__ __forceinline__ void next(const PromptParts& w, int row_tiles, int kv_heads) {
         tile = 0;
-        if (++rt == row_tiles) {
+        const int64_t* const p = w.prefix + static_cast<int64_t>(n) * (row_tiles + 1);
+        if (++rt == row_tiles || p[rt] == p[row_tiles]) {
             rt = 0;
             if (++h == kv_heads) {
                 h = 0;
-                ++n;
+                do ++n;
+                while (w.prefix[static_cast<int64_t>(n) * (row_tiles + 1) + row_tiles] == 0);
             }
         }
         measure(w, row_tiles);
@@ -949,7 +969,7 @@ int launch(const KvAttnArgs& a, const KvPromptPlan& p, char* ws, float* lse2, cu
     PromptStart* const starts = reinterpret_cast<PromptStart*>(ws + p.starts);
     const PromptParts w{reinterpret_cast<float*>(ws + p.out), reinterpret_cast<float2*>(ws + p.stats), list, starts, prefix,
                         lse2};
-    k_kv_prompt_plan<<<1, 1024, 0, stream>>>(a, list, starts, prefix,
+    k_kv_prompt_plan<false><<<1, 1024, 0, stream>>>(a, list, starts, prefix,
                                              prefix + static_cast<int64_t>(a.batch) * (row_tiles + 1), row_tiles, p.ctas);
     int st = check_launch("dt_kv_attention");
     if (st != DT_OK) return st;
@@ -957,6 +977,334 @@ int launch(const KvAttnArgs& a, const KvPromptPlan& p, char* ws, float* lse2, cu
     st = check_launch("dt_kv_attention");
     if (st != DT_OK || p.ctas < 2) return st;
     k_kv_prompt_merge<EP><<<dim3(p.ctas - 1, kItemRows / kMergeRows), 256, 0, stream>>>(a, w, row_tiles);
+    return check_launch("dt_kv_attention");
+}
+
+// ---------------------------------------------------------------------------------------------------------------
+// Weights of each token, summed over many query rows
+// ---------------------------------------------------------------------------------------------------------------
+// S^T = K Q^T, 128 keys against tiles of 128 query rows: a thread owns a key and adds up 2^(score - log2 sum of the row)
+// over the rows, so there are no atomics and the order of the sum is fixed. An item is (sequence, head, 128 keys); the
+// row tiles of all items stand in one list, as above, and items that are split leave 128 sums a part.
+// Warps 0-3 and 4-7 take turns at the row tiles; they also turn an item's keys into the operand. Warp 8 issues the
+// products into four buffers of 128 TMEM columns, warp 9 copies row blocks (k_kv_row_blocks, laid out as operands) with
+// one bulk copy each. Bound by the exponentials: 1024 cycles a tile against 512 of the tensor core.
+template <int EP>
+struct ColumnShape {
+    static constexpr int kOperand = 128 * EP * 2;
+    // what a row tile needs: the operand, then (factor, log2 sum) and the limit of each row
+    static constexpr int kBlock = kOperand + 128 * 8 + 128 * 4;
+    static constexpr int kStages = 3;
+    static constexpr int kBlockRoom = (kBlock + 1023) / 1024 * 1024;
+    static constexpr int kKeys = 0;
+    static constexpr int kBlocks = kOperand;
+    static constexpr int kBars = kBlocks + kStages * kBlockRoom;
+    static constexpr int kSums = kBars + 256;
+    static constexpr int kSmem = kSums + 128 * 4;
+};
+constexpr int kColumnThreads = 320;
+enum ColumnBar { kBFull = 0, kBEmpty = 3, kTFull = 6, kTEmpty = 10, kKReady = 14, kColumnBars = 15 };
+
+// The query rows of 128-row tiles as operand blocks in the workspace, with each row's score factor, log2 sum (+infinity
+// for rows that give no weight: 2^-infinity is 0) and limit.
+template <bool E4M3, int EP>
+__global__ void __launch_bounds__(128) k_kv_row_blocks(KvAttnArgs a, const float* __restrict__ lse2, uint8_t* blocks) {
+    const int tiles = (a.rows + kRowTile - 1) / kRowTile;
+    const size_t head = blockIdx.x / tiles;
+    const int n = static_cast<int>(head / a.kv_heads), h = static_cast<int>(head % a.kv_heads);
+    const int r = threadIdx.x, row = static_cast<int>(blockIdx.x % tiles) * kRowTile + r;
+    uint8_t* const out = blocks + static_cast<size_t>(blockIdx.x) * ColumnShape<EP>::kBlock;
+    const int len = kv_length(a.lengths, n, a.capacity), cnt = kv_count(a.counts, n, a.tokens);
+    const int lim = kv_limit(a, row, len, cnt);
+    const uint16_t* p = nullptr;
+    if (lim > 0) {
+        const int t = row / a.group, jj = row - t * a.group;
+        p = static_cast<const uint16_t*>(a.query) + n * a.q_stride_n + static_cast<int64_t>(h * a.group + jj) * a.q_stride_h +
+            t * a.q_stride_t;
+    }
+    uint32_t x[EP / 2];
+    float amax = 0.0f;
+#pragma unroll
+    for (int c = 0; c < EP / 8; ++c) {
+        const bool live = p != nullptr && c * 8 < a.head_dim;
+        if (live && a.q_vec) {
+            const uint4 u = *reinterpret_cast<const uint4*>(p + c * 8);
+            x[c * 4] = u.x, x[c * 4 + 1] = u.y, x[c * 4 + 2] = u.z, x[c * 4 + 3] = u.w;
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                x[c * 4 + j] = live ? p[c * 8 + 2 * j] | (static_cast<uint32_t>(p[c * 8 + 2 * j + 1]) << 16) : 0u;
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack16(x[c * 4 + j], a.query_bf16);
+            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+        }
+    }
+    float mul, inv;
+    row_power(amax, mul, inv);
+#pragma unroll
+    for (int c = 0; c < EP / 8; ++c) {
+        uint32_t q[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float2 f = unpack16(x[c * 4 + j], a.query_bf16);
+            q[j] = pack_half2(f.x * mul, f.y * mul);
+        }
+        *reinterpret_cast<uint4*>(out + operand_offset(r, c)) = make_uint4(q[0], q[1], q[2], q[3]);
+    }
+    const float l = lim > 0 ? lse2[head * a.rows + row] : INFINITY;
+    reinterpret_cast<float2*>(out + ColumnShape<EP>::kOperand)[r] =
+        make_float2(inv * a.scale_log2 * code_unit<E4M3>(), l == -INFINITY ? INFINITY : l);
+    reinterpret_cast<int*>(out + ColumnShape<EP>::kOperand + 128 * 8)[r] = lim;
+}
+
+struct ColumnParts {
+    PromptParts list;      // out: [slot][128] sums
+    const uint8_t* blocks;
+};
+
+template <bool E4M3, int EP>
+__global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, ColumnParts w, int key_tiles) {
+    using S = ColumnShape<EP>;
+    extern __shared__ __align__(1024) uint8_t smem[];
+    const uint32_t base = smem_addr(smem);
+    const uint32_t bars = base + S::kBars;
+    volatile uint32_t* const tmem_slot = reinterpret_cast<volatile uint32_t*>(smem + S::kBars + kColumnBars * 8);
+    volatile uint32_t* const dead = tmem_slot + 1;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+    const PromptList list = *w.list.list;
+    const int64_t x_begin = list.each * blockIdx.x;
+    if (x_begin >= list.total) return;
+    const int count = static_cast<int>(min(list.each, list.total - x_begin));
+    const PromptStart start = w.list.starts[blockIdx.x];
+    const int row_tiles = (a.rows + kRowTile - 1) / kRowTile;
+
+    if (tid == 0) {
+        for (int i = 0; i < S::kStages; ++i) {
+            mbar_init(bars + (kBFull + i) * 8, 1);
+            mbar_init(bars + (kBEmpty + i) * 8, 1 + 4);
+        }
+        for (int i = 0; i < 4; ++i) {
+            mbar_init(bars + (kTFull + i) * 8, 1);
+            mbar_init(bars + (kTEmpty + i) * 8, 4);
+        }
+        mbar_init(bars + kKReady * 8, 8);
+        *dead = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if (warp == 8) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(
+                         smem_addr(const_cast<uint32_t*>(tmem_slot)))
+                     : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, *tmem_slot, 0);
+
+    // Every role walks the same items; c counts the row tiles of this CTA.
+    PromptItem pos(w.list, key_tiles, start);
+    uint32_t c = 0;
+    if (warp == 9) {
+        // ---- row blocks ----
+        for (int left = count;;) {
+            const int steps = min(pos.tiles - pos.tile, left);
+            const int first = row_tiles - pos.tiles + pos.tile;
+            const size_t head = static_cast<size_t>(pos.n) * a.kv_heads + pos.h;
+            const uint8_t* src = w.blocks + (head * row_tiles + first) * S::kBlock;
+            for (int j = 0; j < steps; ++j, ++c, src += S::kBlock) {
+                const uint32_t st = c % S::kStages, full = bars + (kBFull + st) * 8;
+                mbar_wait(bars + (kBEmpty + st) * 8, (c / S::kStages & 1) ^ 1, dead);
+                __syncwarp();
+                if (elect_one()) {
+                    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "n"(S::kBlock) : "memory");
+                    asm volatile(
+                        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(
+                            base + S::kBlocks + st * S::kBlockRoom),
+                        "l"(src), "n"(S::kBlock), "r"(full)
+                        : "memory");
+                }
+                __syncwarp();
+            }
+            left -= steps;
+            if (left == 0) break;
+            pos.next(w.list, key_tiles, a.kv_heads);
+        }
+    } else if (warp == 8) {
+        // ---- products ----
+        const uint64_t k_desc = operand_desc(base + S::kKeys, 16, 1024);
+        constexpr uint32_t kInstr = instr_desc(kRowTile, false);
+        for (int left = count, item = 0;; ++item) {
+            const int steps = min(pos.tiles - pos.tile, left);
+            mbar_wait(bars + kKReady * 8, item & 1, dead);
+            for (int j = 0; j < steps; ++j, ++c) {
+                const uint32_t st = c % S::kStages, b = c & 3;
+                mbar_wait(bars + (kBFull + st) * 8, c / S::kStages & 1, dead);
+                mbar_wait(bars + (kTEmpty + b) * 8, (c >> 2 & 1) ^ 1, dead);
+                __syncwarp();
+                tc_fence_after();
+                const uint64_t q_desc = operand_desc(base + S::kBlocks + st * S::kBlockRoom, 16, 1024);
+                if (elect_one()) {
+#pragma unroll
+                    for (int k = 0; k < EP / 16; ++k) {
+                        const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                        mma_ss(tmem + b * 128, k_desc + off, q_desc + off, kInstr, k > 0);
+                    }
+                    tc_commit(bars + (kTFull + b) * 8);
+                    tc_commit(bars + (kBEmpty + st) * 8);
+                }
+                __syncwarp();
+            }
+            left -= steps;
+            if (left == 0) break;
+            pos.next(w.list, key_tiles, a.kv_heads);
+        }
+    } else {
+        // ---- sums ----
+        const int turn = warp >> 2;
+        const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
+        float* const sums = reinterpret_cast<float*>(smem + S::kSums);
+        for (int left = count;;) {
+            const int steps = min(pos.tiles - pos.tile, left);
+            const size_t head = static_cast<size_t>(pos.n) * a.kv_heads + pos.h;
+            const int len = kv_length(a.lengths, pos.n, a.capacity), tok = pos.rt * kTokTile;
+            const int key = tok + (tid & 127);
+            // the keys: a thread takes 16 codes at a time
+            for (int v = tid; v < 128 * (EP / 16); v += 256) {
+                const int r = v / (EP / 16), e = v % (EP / 16);
+                uint4 q = make_uint4(0, 0, 0, 0);
+                if (tok + r < len && e * 16 < a.head_dim)
+                    q = __ldg(reinterpret_cast<const uint4*>(a.key + (head * a.capacity + tok + r) * a.head_dim + e * 16));
+                uint4 lo, hi;
+                codes_to_half<E4M3, 0>(q.x, lo.x, lo.y);
+                codes_to_half<E4M3, 0>(q.y, lo.z, lo.w);
+                codes_to_half<E4M3, 0>(q.z, hi.x, hi.y);
+                codes_to_half<E4M3, 0>(q.w, hi.z, hi.w);
+                *reinterpret_cast<uint4*>(smem + S::kKeys + operand_offset(r, 2 * e)) = lo;
+                *reinterpret_cast<uint4*>(smem + S::kKeys + operand_offset(r, 2 * e + 1)) = hi;
+            }
+            async_proxy_fence();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(bars + kKReady * 8);
+            // one scale for the 32 keys of a warp
+            const int span = tok + (warp & 3) * 32;
+            const float ks = span < len ? a.key_scale[head * a.nblocks + (span >> a.block_shift)] : 0.0f;
+            const Pair ks2 = pair_of(ks, ks);
+            Pair sum[2] = {0, 0};
+            for (int j = 0; j < steps; ++j, ++c) {
+                if ((c & 1) != static_cast<uint32_t>(turn)) continue;
+                const uint32_t st = c % S::kStages, b = c & 3;
+                mbar_wait(bars + (kTFull + b) * 8, c >> 2 & 1, dead);
+                mbar_wait(bars + (kBFull + st) * 8, c / S::kStages & 1, dead);  // the block's numbers, for this thread too
+                __syncwarp();
+                tc_fence_after();
+                const uint8_t* const block = smem + S::kBlocks + st * S::kBlockRoom;
+                const float4* const rows = reinterpret_cast<const float4*>(block + S::kOperand);
+                const int2* const limits = reinterpret_cast<const int2*>(block + S::kOperand + 128 * 8);
+                // rows that see less than all of these keys: the first of the tile, where there are any
+                const bool ragged = reinterpret_cast<const int*>(limits)[0] < tok + kTokTile ||
+                                    reinterpret_cast<const int*>(limits)[127] < tok + kTokTile;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    uint32_t s[32];
+                    tmem_load32(tmem + b * 128 + k * 32 + lanes, s);
+                    tmem_wait_load32(s);
+#pragma unroll
+                    for (int i = 0; i < 32; i += 2) {
+                        const float4 f = rows[(k * 32 + i) / 2];  // factor and log2 sum of two rows
+                        const Pair x = fma2(pair_of(__uint_as_float(s[i]), __uint_as_float(s[i + 1])),
+                                            mul2(pair_of(f.x, f.z), ks2), pair_of(-f.y, -f.w));
+                        float u, v;
+                        unpair(x, u, v);
+                        u = ex2(u);
+                        v = ex2(v);
+                        if (ragged) {
+                            const int2 lim = limits[(k * 32 + i) / 2];
+                            if (key >= lim.x) u = 0.0f;
+                            if (key >= lim.y) v = 0.0f;
+                        }
+                        sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair_of(u, v));
+                    }
+                }
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(bars + (kTEmpty + b) * 8);
+                    mbar_arrive(bars + (kBEmpty + st) * 8);
+                }
+            }
+            float u, v;
+            unpair(add2(sum[0], sum[1]), u, v);
+            u += v;
+            // both groups' tiles are done, and with them every product of these keys
+            if (turn == 1) sums[tid & 127] = u;
+            asm volatile("bar.sync 1, 256;" ::: "memory");
+            if (turn == 0) {
+                u += sums[tid];
+                if (*dead) u = __int_as_float(0x7fc00000);
+                if (steps < pos.tiles) {
+                    const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (pos.tile > 0 ? 0 : 1);
+                    w.list.out[slot * 128 + tid] = u;
+                } else if (key < len) {
+                    float* const o = a.weights + head * a.capacity + key;
+                    *o = a.accumulate ? *o + u : u;
+                }
+            }
+            asm volatile("bar.sync 1, 256;" ::: "memory");  // the sums have been read
+            left -= steps;
+            if (left == 0) break;
+            pos.next(w.list, key_tiles, a.kv_heads);
+        }
+        tc_fence_before();
+    }
+    __syncthreads();
+    if (warp == 8) {
+        tc_fence_after();
+        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+    }
+}
+
+// Adds up the parts of the key tiles that more than one CTA of k_kv_columns worked on.
+__global__ void __launch_bounds__(128) k_kv_columns_merge(KvAttnArgs a, PromptParts w, int key_tiles) {
+    const PromptList list = *w.list;
+    if (list.each * (blockIdx.x + 1) >= list.total) return;
+    const PromptItem pos(w, key_tiles, w.starts[blockIdx.x + 1]);
+    if (pos.tile == 0 || pos.tile > list.each) return;
+    const int c0 = blockIdx.x, parts = 2 + (pos.tiles - pos.tile - 1) / static_cast<int>(list.each);
+    const int key = pos.rt * kTokTile + threadIdx.x;
+    if (key >= kv_length(a.lengths, pos.n, a.capacity)) return;
+    float u = 0.0f;
+    for (int k = 0; k < parts; ++k) u += w.out[(static_cast<size_t>(c0) * 2 + (k == 0 ? 1 : 2 * k)) * 128 + threadIdx.x];
+    float* const o = a.weights + (static_cast<size_t>(pos.n) * a.kv_heads + pos.h) * a.capacity + key;
+    *o = a.accumulate ? *o + u : u;
+}
+
+template <bool E4M3, int EP>
+int launch_columns(const KvAttnArgs& a, const KvColumnPlan& p, char* ws, const float* lse2, cudaStream_t stream) {
+    using S = ColumnShape<EP>;
+    cudaError_t e = cudaFuncSetAttribute(k_kv_columns<E4M3, EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
+    const int key_tiles = static_cast<int>((a.capacity + kTokTile - 1) / kTokTile);
+    const int64_t blocks = static_cast<int64_t>(a.batch) * a.kv_heads * ((a.rows + kRowTile - 1) / kRowTile);
+    if (blocks > INT32_MAX) return set_error(DT_ERR_INVALID, "dt_kv_attention: too many blocks");
+    int64_t* const prefix = reinterpret_cast<int64_t*>(ws + p.prefix);
+    PromptList* const list = reinterpret_cast<PromptList*>(ws + p.list);
+    PromptStart* const starts = reinterpret_cast<PromptStart*>(ws + p.starts);
+    uint8_t* const rows = reinterpret_cast<uint8_t*>(ws + p.blocks);
+    const ColumnParts w{PromptParts{reinterpret_cast<float*>(ws + p.sums), nullptr, list, starts, prefix, nullptr}, rows};
+    k_kv_row_blocks<E4M3, EP><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(a, lse2, rows);
+    int st = check_launch("dt_kv_attention");
+    if (st != DT_OK) return st;
+    k_kv_prompt_plan<true><<<1, 1024, 0, stream>>>(a, list, starts, prefix,
+                                                   prefix + static_cast<int64_t>(a.batch) * (key_tiles + 1), key_tiles, p.ctas);
+    st = check_launch("dt_kv_attention");
+    if (st != DT_OK) return st;
+    k_kv_columns<E4M3, EP><<<p.ctas, kColumnThreads, S::kSmem, stream>>>(a, w, key_tiles);
+    st = check_launch("dt_kv_attention");
+    if (st != DT_OK || p.ctas < 2) return st;
+    k_kv_columns_merge<<<p.ctas - 1, 128, 0, stream>>>(a, w.list, key_tiles);
     return check_launch("dt_kv_attention");
 }
 
@@ -984,6 +1332,31 @@ int kv_prompt_attention(const KvAttnArgs& a, int code, const KvPromptPlan& p, vo
     if (a.head_dim <= 64)
         return code == DT_KV_E4M3 ? launch<true, 64>(a, p, ws, lse2, stream) : launch<false, 64>(a, p, ws, lse2, stream);
     return code == DT_KV_E4M3 ? launch<true, 128>(a, p, ws, lse2, stream) : launch<false, 128>(a, p, ws, lse2, stream);
+}
+
+KvColumnPlan kv_column_plan(int64_t batch, int64_t kv_heads, int64_t rows, int64_t head_dim, int64_t capacity, int sms) {
+    const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+    const size_t block = head_dim <= 64 ? ColumnShape<64>::kBlock : ColumnShape<128>::kBlock;
+    const size_t row_tiles = (rows + kRowTile - 1) / kRowTile, key_tiles = (capacity + kTokTile - 1) / kTokTile;
+    KvColumnPlan p{};
+    p.ctas = sms;
+    p.blocks = 0;
+    p.sums = up(static_cast<size_t>(batch) * kv_heads * row_tiles * block);
+    p.list = p.sums + up(static_cast<size_t>(sms) * 2 * 128 * 4);
+    p.starts = p.list + up(sizeof(PromptList));
+    p.prefix = p.starts + up(static_cast<size_t>(sms) * sizeof(PromptStart));
+    p.bytes = p.prefix + up((static_cast<size_t>(batch) * (key_tiles + 1) + batch + 1) * 8);
+    return p;
+}
+
+int kv_column_sums(const KvAttnArgs& a, int code, const KvColumnPlan& p, void* workspace, const float* lse2,
+                   cudaStream_t stream) {
+    char* const ws = static_cast<char*>(workspace);
+    if (a.head_dim <= 64)
+        return code == DT_KV_E4M3 ? launch_columns<true, 64>(a, p, ws, lse2, stream)
+                                  : launch_columns<false, 64>(a, p, ws, lse2, stream);
+    return code == DT_KV_E4M3 ? launch_columns<true, 128>(a, p, ws, lse2, stream)
+                              : launch_columns<false, 128>(a, p, ws, lse2, stream);
 }
 
 }  // namespace dtb
