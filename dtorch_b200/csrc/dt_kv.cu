@@ -317,27 +317,9 @@ __device__ __forceinline__ void load_query(const KvAttnArgs& a, int n, int h, in
     for (int half = 0; half < 2; ++half) {
         const uint16_t* p = query_row(a, n, h, row0 + (lane >> 2) + half * 8);
         uint32_t x[EP / 8];
-        float amax = 0.0f;
 #pragma unroll
-        for (int kc = 0; kc < EP / 64; ++kc) {
-            const int e = kc * 64 + c * 16;
-            const bool live = p != nullptr && e < a.head_dim;
-            if (live && a.q_vec) {
-                const uint4 u = *reinterpret_cast<const uint4*>(p + e);
-                const uint4 w = *reinterpret_cast<const uint4*>(p + e + 8);
-                x[kc * 8 + 0] = u.x, x[kc * 8 + 1] = u.y, x[kc * 8 + 2] = u.z, x[kc * 8 + 3] = u.w;
-                x[kc * 8 + 4] = w.x, x[kc * 8 + 5] = w.y, x[kc * 8 + 6] = w.z, x[kc * 8 + 7] = w.w;
-            } else {
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-                    x[kc * 8 + j] = live ? p[e + 2 * j] | (static_cast<uint32_t>(p[e + 2 * j + 1]) << 16) : 0u;
-            }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float2 f = unpack16(x[kc * 8 + j], a.query_bf16);
-                amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-            }
-        }
+        for (int kc = 0; kc < EP / 64; ++kc) load_row<2>(a, p, kc * 64 + c * 16, x + kc * 8);
+        float amax = row_max<EP / 8>(a, x);
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
         amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
         float mul;

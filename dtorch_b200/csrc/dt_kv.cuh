@@ -125,4 +125,37 @@ __device__ __forceinline__ void row_power(float amax, float& mul, float& inv) {
     inv = __uint_as_float(static_cast<uint32_t>(127 - 13 + ex) << 23);
 }
 
+// 8 N elements of a query row from element `e` on, as words of two; zeros where there is no row and behind head_dim. All
+// loads are issued before any is used.
+template <int N>
+__device__ __forceinline__ void load_row(const KvAttnArgs& a, const uint16_t* p, int e, uint32_t* x) {
+#pragma unroll
+    for (int j = 0; j < 4 * N; ++j) x[j] = 0;
+    if (p == nullptr) return;
+    if (a.q_vec) {
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+            if (e + c * 8 < a.head_dim) {
+                const uint4 u = __ldg(reinterpret_cast<const uint4*>(p + e + c * 8));
+                x[c * 4] = u.x, x[c * 4 + 1] = u.y, x[c * 4 + 2] = u.z, x[c * 4 + 3] = u.w;
+            }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4 * N; ++j)
+            if (e + 2 * j < a.head_dim) x[j] = p[e + 2 * j] | (static_cast<uint32_t>(p[e + 2 * j + 1]) << 16);
+    }
+}
+
+// Largest |element| of words of two.
+template <int N>
+__device__ __forceinline__ float row_max(const KvAttnArgs& a, const uint32_t* x) {
+    float m = 0.0f;
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        const float2 f = unpack16(x[j], a.query_bf16);
+        m = fmaxf(m, fmaxf(fabsf(f.x), fabsf(f.y)));
+    }
+    return m;
+}
+
 }  // namespace dtb

@@ -201,25 +201,8 @@ template <int EP>
 __device__ __forceinline__ float stage_query(const KvAttnArgs& a, const uint16_t* p, uint8_t* smem, int r, int half,
                                              volatile uint16_t* mine, volatile uint16_t* other, int id, float sign) {
     uint32_t x[EP / 4];
-    float amax = 0.0f;
-#pragma unroll
-    for (int c = 0; c < EP / 16; ++c) {
-        const int e = half * (EP / 2) + c * 8;
-        const bool live = p != nullptr && e < a.head_dim;
-        if (live && a.q_vec) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p + e);
-            x[c * 4] = u.x, x[c * 4 + 1] = u.y, x[c * 4 + 2] = u.z, x[c * 4 + 3] = u.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                x[c * 4 + j] = live ? p[e + 2 * j] | (static_cast<uint32_t>(p[e + 2 * j + 1]) << 16) : 0u;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack16(x[c * 4 + j], a.query_bf16);
-            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-    }
+    load_row<EP / 16>(a, p, half * (EP / 2), x);
+    const float amax = row_max<EP / 4>(a, x);
     *mine = round_up16(amax);
     pair_sync(id);
     float mul, inv;
@@ -371,7 +354,8 @@ __device__ __forceinline__ void weigh(const uint32_t* s, float f, float vf, floa
 }
 
 constexpr int kItemRows = 2 * kRowTile;
-constexpr int kLeastTiles = 2;  // a stretch is not shorter: each part costs its queries' staging and a join
+constexpr int kItemCost = 2;    // tiles that an item costs besides its own: its queries' staging, its outputs
+constexpr int kLeastTiles = 2;  // a stretch is not shorter: each part costs that too, and a join
 
 // Tiles of 128 tokens that the rows of item `rt` of a sequence see; at least one, so that rows that see nothing are
 // written too. Rows are in the order of the tokens: the last live one sees the most.
@@ -381,13 +365,15 @@ __device__ __forceinline__ int item_tiles(const KvAttnArgs& a, int rt, int len, 
     return max(1, (most + kTokTile - 1) / kTokTile);
 }
 
-// Where a CTA's stretch of the list begins: an item, and a tile of it.
+// Where a CTA's stretch of the list begins: an item and a tile of it, and what is left of the item's own cost before it.
+// An item stands in the list as kItemCost and then its tiles; a boundary inside its cost leaves all tiles to what comes
+// behind.
 struct PromptStart {
-    int n, h, rt, tile;
+    int n, h, rt, tile, lead;
 };
 
 struct PromptList {
-    int64_t total;  // tiles
+    int64_t total;  // cost of all items
     int64_t each;   // of every stretch but the last
 };
 
@@ -413,8 +399,8 @@ __device__ __forceinline__ int key_tile_rows(const KvAttnArgs& a, int kt, int le
 }
 
 // Lays out a list, in one block: of (sequence, head, 256 rows) items and their key tiles, or (COLUMNS) of (sequence,
-// head, 128 keys) items and their row tiles. prefix[n][i]: tiles of a head's items before item i of sequence n, and of
-// all of them at prefix[n][items]; base[n]: tiles of the sequences before n.
+// head, 128 keys) items and their row tiles. prefix[n][i]: cost of a head's items before item i of sequence n, and of
+// all of them at prefix[n][items]; base[n]: that of the sequences before n.
 template <bool COLUMNS>
 __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptList* list, PromptStart* starts,
                                                          int64_t* prefix, int64_t* base, int row_tiles, int ctas) {
@@ -425,7 +411,8 @@ __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptLis
         int64_t done = 0;
         for (int r0 = 0; r0 < row_tiles; r0 += 32) {
             const int rt = r0 + lane;
-            const int64_t mine = rt >= row_tiles ? 0 : COLUMNS ? key_tile_rows(a, rt, len, cnt) : item_tiles(a, rt, len, cnt);
+            const int tiles = rt >= row_tiles ? 0 : COLUMNS ? key_tile_rows(a, rt, len, cnt) : item_tiles(a, rt, len, cnt);
+            const int64_t mine = tiles > 0 ? tiles + kItemCost : 0;
             int64_t incl = mine;
 #pragma unroll
             for (int d = 1; d < 32; d <<= 1) {
@@ -478,13 +465,15 @@ __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptLis
         s.h = static_cast<int>(quotient(x, p[row_tiles]));
         x -= s.h * p[row_tiles];
         s.rt = find(p, row_tiles, x);
-        s.tile = static_cast<int>(x - p[s.rt]);
+        const int at = static_cast<int>(x - p[s.rt]);
+        s.tile = max(at - kItemCost, 0);
+        s.lead = max(kItemCost - at, 0);
         starts[b] = s;
     }
 }
 
 struct PromptParts {
-    float* out;             // [slot][256][EP], unnormalised
+    float* out;             // [slot][EP / 4][256][4], unnormalised: neighbouring rows side by side
     float2* stats;          // [slot][256]: reference (log2), sum
     const PromptList* list;
     const PromptStart* starts;
@@ -502,7 +491,7 @@ struct PromptItem {
     }
     __device__ __forceinline__ void measure(const PromptParts& w, int row_tiles) {
         const int64_t* const p = w.prefix + static_cast<int64_t>(n) * (row_tiles + 1) + rt;
-        tiles = static_cast<int>(p[1] - p[0]);
+        tiles = static_cast<int>(p[1] - p[0]) - kItemCost;
     }
     // The next item that has tiles, whole; there is one. Empty items stand only behind a head's others (keys behind a
     // sequence's length), and are passed over at once.
@@ -535,8 +524,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
     const PromptList list = *w.list;
     const int64_t x_begin = list.each * blockIdx.x;
     if (x_begin >= list.total) return;
-    const int count = static_cast<int>(min(list.each, list.total - x_begin));  // tiles of this CTA
     const PromptStart start = w.starts[blockIdx.x];
+    const int count = static_cast<int>(min(list.each, list.total - x_begin)) - start.lead;  // cost, from the first tile on
+    if (count <= 0) return;
 
     if (tid == 0) {
         for (int i = 0; i < 2; ++i) {
@@ -625,8 +615,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                     c_group1 += groups - 1;
                 }
                 ++items;
-                left -= steps;
-                if (left == 0) break;
+                left -= steps + kItemCost;
+                if (left <= 0) break;
                 pos.next(w, row_tiles, a.kv_heads);
             }
         }
@@ -673,8 +663,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 fetch_codes<EP>(smem_addr(vcodes), vbase, next, len, a.head_dim, t);
             }
             asm volatile("cp.async.wait_group 0;" ::: "memory");
-            left -= steps;
-            if (left == 0) break;
+            left -= steps + kItemCost;
+            if (left <= 0) break;
             pos.next(w, row_tiles, a.kv_heads);
         }
     } else {
@@ -811,7 +801,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 live -= kTokTile;
             }
             c += item_steps;
-            left -= item_steps;
+            left -= item_steps + kItemCost;
             ++items;
             if (steps == 0) {  // no rows here: keep pace with the other row tile, whose warps report their queries too
                 mbar_wait(bars + kQReady * 8, (items - 1) & 1, dead);
@@ -833,7 +823,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 // an item that other CTAs work on too: one that began before this stretch, or goes on behind it
                 const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (pos.tile > 0 ? 0 : 1);
                 const size_t at = slot * kItemRows + g * kRowTile + r;
-                float4* const out = reinterpret_cast<float4*>(w.out + at * EP + half * (EP / 2));
+                float4* const out = reinterpret_cast<float4*>(w.out) + slot * (EP / 4) * kItemRows +
+                                    half * (EP / 8) * kItemRows + g * kRowTile + r;
 #pragma unroll 1
                 for (int k = 0; k < EP / 2; k += 32) {
                     uint32_t o[32];
@@ -841,21 +832,18 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                     tmem_wait_load32(o);
 #pragma unroll
                     for (int i = 0; i < 32; i += 4)
-                        out[(k + i) / 4] = make_float4(__uint_as_float(o[i]) * v_up, __uint_as_float(o[i + 1]) * v_up,
-                                                       __uint_as_float(o[i + 2]) * v_up, __uint_as_float(o[i + 3]) * v_up);
+                        out[(k + i) / 4 * kItemRows] =
+                            make_float4(__uint_as_float(o[i]) * v_up, __uint_as_float(o[i + 1]) * v_up,
+                                        __uint_as_float(o[i + 2]) * v_up, __uint_as_float(o[i + 3]) * v_up);
                 }
                 if (half == 0) w.stats[at] = make_float2(ref, l);
                 continue;
             }
             const float inv_l = v_up / l;
-            int at_end = row;
-            asm volatile("" : "+r"(at_end));  // worked out again: not held through the loop
-            const int t = at_end / a.group, jj = at_end - t * a.group;
-            const size_t orow = (head * a.group + jj) * a.tokens + t;
-            uint16_t* const out = static_cast<uint16_t*>(a.out) + orow * a.head_dim;
+            // the rows go through the memory of their queries, which are done with, so that stores are of whole rows
+            uint8_t* const rows = smem + S::kQuery + g * S::kOperand;
 #pragma unroll 1
             for (int k0 = 0; k0 < EP / 2; k0 += 32) {
-                const int k = half * (EP / 2) + k0;  // element of the row
                 uint32_t o[32];
                 tmem_load32(o_col + k0, o);
                 tmem_wait_load32(o);
@@ -873,10 +861,30 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                             q[e] = pack_half2(u, v);
                         }
                     }
-                    if (row < a.rows && k + i < a.head_dim)
-                        *reinterpret_cast<uint4*>(out + k + i) = make_uint4(q[0], q[1], q[2], q[3]);
+                    *reinterpret_cast<uint4*>(rows + operand_offset(r, (half * (EP / 2) + k0 + i) / 8)) =
+                        make_uint4(q[0], q[1], q[2], q[3]);
                 }
             }
+            pair_sync(pair);
+            // this pair's 32 rows: its two warps take 16 each, a row of EP / 8 lanes at a time
+            {
+                const int first = (warp & 3) * 32 + half * 16;
+#pragma unroll 1
+                for (int i = lane; i < 16 * (EP / 8); i += 32) {
+                    const int rr = first + i / (EP / 8), c8 = i % (EP / 8);
+                    const int orow_in = pos.rt * kItemRows + g * kRowTile + rr;
+                    if (orow_in >= a.rows || c8 * 8 >= a.head_dim) continue;
+                    const int t = orow_in / a.group, jj = orow_in - t * a.group;
+                    const size_t at = ((head * a.group + jj) * a.tokens + t) * a.head_dim + c8 * 8;
+                    *reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + at) =
+                        *reinterpret_cast<const uint4*>(rows + operand_offset(rr, c8));
+                }
+            }
+            pair_sync(pair);  // the next queries take the place of these rows
+            int at_end = row;
+            asm volatile("" : "+r"(at_end));  // worked out again: not held through the loop
+            const int t = at_end / a.group, jj = at_end - t * a.group;
+            const size_t orow = (head * a.group + jj) * a.tokens + t;
             if (row < a.rows && half == 0) {
                 const float lse2 = l == 0.0f ? -INFINITY : ref + log2f(l);
                 if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
@@ -895,7 +903,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
 constexpr int kMergeRows = 64;
 
 // Joins the parts of the items that more than one CTA of k_kv_prompt worked on: a block for each boundary between two
-// stretches and 64 of an item's 256 rows, 16 lanes for a row at a time. The item's first boundary does the work.
+// stretches and 64 of an item's 256 rows, four threads a row. The item's first boundary does the work.
 template <int EP>
 __global__ void __launch_bounds__(256) k_kv_prompt_merge(KvAttnArgs a, PromptParts w, int row_tiles) {
     const PromptList list = *w.list;
@@ -904,57 +912,55 @@ __global__ void __launch_bounds__(256) k_kv_prompt_merge(KvAttnArgs a, PromptPar
     // an item that begins here, or before the stretch that ends here, is not this block's
     if (pos.tile == 0 || pos.tile > list.each) return;
     const int c0 = blockIdx.x, parts = 2 + (pos.tiles - pos.tile - 1) / static_cast<int>(list.each);
-    const int lane = threadIdx.x & 15;
-    constexpr int kVec = EP / 64;  // float4 of the row a lane has
+    constexpr int kVec = EP / 16;  // float4 of the row a thread has
+    const int quarter = threadIdx.x >> 6, r = blockIdx.y * kMergeRows + (threadIdx.x & 63), row = pos.rt * kItemRows + r;
+    if (row >= a.rows) return;
     const size_t head = static_cast<size_t>(pos.n) * a.kv_heads + pos.h;
-    for (int i = threadIdx.x >> 4; i < kMergeRows; i += 16) {
-        const int r = blockIdx.y * kMergeRows + i, row = pos.rt * kItemRows + r;
-        if (row >= a.rows) return;
-        // part k is in slot 2 (c0 + k) but for the first, which goes on behind its stretch: 2 c0 + 1
-        const float2* const stats = w.stats + static_cast<size_t>(c0) * 2 * kItemRows + r;
-        const float4* const out = reinterpret_cast<const float4*>(w.out + (static_cast<size_t>(c0) * 2 * kItemRows + r) * EP) + lane;
-        float m = -INFINITY;
-        for (int k = 0; k < parts; ++k) m = fmaxf(m, stats[(k == 0 ? 1 : 2 * k) * kItemRows].x);
-        float l = 0.0f;
-        float4 acc[kVec];
+    // part k is in slot 2 (c0 + k) but for the first, which goes on behind its stretch: 2 c0 + 1
+    const float2* const stats = w.stats + static_cast<size_t>(c0) * 2 * kItemRows + r;
+    const float4* const out = reinterpret_cast<const float4*>(w.out) +
+                              (static_cast<size_t>(c0) * 2 * (EP / 4) + quarter * kVec) * kItemRows + r;
+    float m = -INFINITY;
+    for (int k = 0; k < parts; ++k) m = fmaxf(m, stats[(k == 0 ? 1 : 2 * k) * kItemRows].x);
+    float l = 0.0f;
+    float4 acc[kVec];
 #pragma unroll
-        for (int v = 0; v < kVec; ++v) acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int k = 0; k < parts; ++k) {
-            const int64_t at = static_cast<int64_t>(k == 0 ? 1 : 2 * k) * kItemRows;
-            const float2 st = stats[at];
-            const float f = st.x == m ? 1.0f : ex2(st.x - m);
-            l += st.y * f;
-#pragma unroll
-            for (int v = 0; v < kVec; ++v) {
-                const float4 o = out[at * (EP / 4) + v * 16];
-                acc[v].x = fmaf(o.x, f, acc[v].x);
-                acc[v].y = fmaf(o.y, f, acc[v].y);
-                acc[v].z = fmaf(o.z, f, acc[v].z);
-                acc[v].w = fmaf(o.w, f, acc[v].w);
-            }
-        }
-        const float g = l == 0.0f ? 0.0f : 1.0f / l;
-        const int t = row / a.group, jj = row - t * a.group;
-        const size_t orow = (head * a.group + jj) * a.tokens + t;
+    for (int v = 0; v < kVec; ++v) acc[v] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (int k = 0; k < parts; ++k) {
+        const int64_t slot = k == 0 ? 1 : 2 * k;
+        const float2 st = stats[slot * kItemRows];
+        const float f = st.x == m ? 1.0f : ex2(st.x - m);
+        l += st.y * f;
 #pragma unroll
         for (int v = 0; v < kVec; ++v) {
-            const int e = (v * 16 + lane) * 4;
-            if (e >= a.head_dim) continue;
-            uint2 u;
-            if (a.query_bf16) {
-                const __nv_bfloat162 lo = __floats2bfloat162_rn(acc[v].x * g, acc[v].y * g);
-                const __nv_bfloat162 hi = __floats2bfloat162_rn(acc[v].z * g, acc[v].w * g);
-                u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-            } else {
-                u = make_uint2(pack_half2(acc[v].x * g, acc[v].y * g), pack_half2(acc[v].z * g, acc[v].w * g));
-            }
-            *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) = u;
+            const float4 o = out[(slot * (EP / 4) + v) * kItemRows];
+            acc[v].x = fmaf(o.x, f, acc[v].x);
+            acc[v].y = fmaf(o.y, f, acc[v].y);
+            acc[v].z = fmaf(o.z, f, acc[v].z);
+            acc[v].w = fmaf(o.w, f, acc[v].w);
         }
-        if (lane == 0) {
-            const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
-            if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
-            if (w.lse2 != nullptr) w.lse2[head * a.rows + row] = lse2;
+    }
+    const float g = l == 0.0f ? 0.0f : 1.0f / l;
+    const int t = row / a.group, jj = row - t * a.group;
+    const size_t orow = (head * a.group + jj) * a.tokens + t;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+        const int e = (quarter * kVec + v) * 4;
+        if (e >= a.head_dim) continue;
+        uint2 u;
+        if (a.query_bf16) {
+            const __nv_bfloat162 lo = __floats2bfloat162_rn(acc[v].x * g, acc[v].y * g);
+            const __nv_bfloat162 hi = __floats2bfloat162_rn(acc[v].z * g, acc[v].w * g);
+            u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+        } else {
+            u = make_uint2(pack_half2(acc[v].x * g, acc[v].y * g), pack_half2(acc[v].z * g, acc[v].w * g));
         }
+        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) = u;
+    }
+    if (quarter == 0) {
+        const float lse2 = l == 0.0f ? -INFINITY : m + log2f(l);
+        if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
+        if (w.lse2 != nullptr) w.lse2[head * a.rows + row] = lse2;
     }
 }
 
@@ -1023,24 +1029,8 @@ __global__ void __launch_bounds__(128) k_kv_row_blocks(KvAttnArgs a, const float
             t * a.q_stride_t;
     }
     uint32_t x[EP / 2];
-    float amax = 0.0f;
-#pragma unroll
-    for (int c = 0; c < EP / 8; ++c) {
-        const bool live = p != nullptr && c * 8 < a.head_dim;
-        if (live && a.q_vec) {
-            const uint4 u = *reinterpret_cast<const uint4*>(p + c * 8);
-            x[c * 4] = u.x, x[c * 4 + 1] = u.y, x[c * 4 + 2] = u.z, x[c * 4 + 3] = u.w;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                x[c * 4 + j] = live ? p[c * 8 + 2 * j] | (static_cast<uint32_t>(p[c * 8 + 2 * j + 1]) << 16) : 0u;
-        }
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 f = unpack16(x[c * 4 + j], a.query_bf16);
-            amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
-        }
-    }
+    load_row<EP / 8>(a, p, 0, x);
+    const float amax = row_max<EP / 2>(a, x);
     float mul, inv;
     row_power(amax, mul, inv);
 #pragma unroll
@@ -1076,8 +1066,9 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
     const PromptList list = *w.list.list;
     const int64_t x_begin = list.each * blockIdx.x;
     if (x_begin >= list.total) return;
-    const int count = static_cast<int>(min(list.each, list.total - x_begin));
     const PromptStart start = w.list.starts[blockIdx.x];
+    const int count = static_cast<int>(min(list.each, list.total - x_begin)) - start.lead;
+    if (count <= 0) return;
     const int row_tiles = (a.rows + kRowTile - 1) / kRowTile;
 
     if (tid == 0) {
@@ -1128,8 +1119,8 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
                 }
                 __syncwarp();
             }
-            left -= steps;
-            if (left == 0) break;
+            left -= steps + kItemCost;
+            if (left <= 0) break;
             pos.next(w.list, key_tiles, a.kv_heads);
         }
     } else if (warp == 8) {
@@ -1157,8 +1148,8 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
                 }
                 __syncwarp();
             }
-            left -= steps;
-            if (left == 0) break;
+            left -= steps + kItemCost;
+            if (left <= 0) break;
             pos.next(w.list, key_tiles, a.kv_heads);
         }
     } else {
@@ -1253,8 +1244,8 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
                 }
             }
             asm volatile("bar.sync 1, 256;" ::: "memory");  // the sums have been read
-            left -= steps;
-            if (left == 0) break;
+            left -= steps + kItemCost;
+            if (left <= 0) break;
             pos.next(w.list, key_tiles, a.kv_heads);
         }
         tc_fence_before();
