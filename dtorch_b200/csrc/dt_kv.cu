@@ -54,10 +54,10 @@ __device__ __forceinline__ void decode4(uint32_t w, float* v) {
     codes_to_half<E4M3, 0>(w, lo, hi);
     const float2 a = __half22float2(*reinterpret_cast<__half2*>(&lo));
     const float2 b = __half22float2(*reinterpret_cast<__half2*>(&hi));
-    v[0] = a.x * code_unit<E4M3>();
-    v[1] = a.y * code_unit<E4M3>();
-    v[2] = b.x * code_unit<E4M3>();
-    v[3] = b.y * code_unit<E4M3>();
+    v[0] = a.x;
+    v[1] = a.y;
+    v[2] = b.x;
+    v[3] = b.y;
 }
 
 struct KvAppendArgs {
@@ -236,38 +236,43 @@ __global__ void __launch_bounds__(256) k_kv_read(KvReadArgs a) {
 // ---------------------------------------------------------------------------------------------------------------
 // Attention of few query rows (single tokens, drafts)
 // ---------------------------------------------------------------------------------------------------------------
-// 16 query rows of a key head against tiles of 128 tokens. The tiles of all (sequence, head, row tile) items stand in
-// one list, and every CTA takes an equal stretch of it, whatever the lengths: a stretch may end one item and begin the
+// 8 or 16 query rows of a key head against tiles of 128 tokens. The tiles of all (sequence, head, row tile) items stand
+// in one list, and every CTA takes an equal stretch of it, whatever the lengths: a stretch may end one item and begin the
 // next. An item inside one stretch is finished there; the others leave (running maximum, sum, unnormalised output) in
 // the workspace, and k_kv_merge joins them in the order of the list.
 //
 // Within a CTA each of the four warps streams its own 32 tokens of every tile through shared memory with cp.async and
 // keeps its own softmax state: no barrier inside the loop; the four states are joined once per item.
-// Scores and outputs use mma.m16n8k16 with fp16 operands: this path is bound by reading the cache, and 16 rows would
-// leave 7/8 of a tcgen05 tile empty. Which elements share a k16 step is free as long as queries and keys agree, so a
-// lane takes 16 consecutive bytes of a key row, enough for four steps.
+// Scores and outputs use mma.m16n8k16 with fp16 operands: this path is bound by reading the cache, and up to 16 rows would
+// leave most of a tcgen05 tile empty. Keys and values are the 16-row operand and the query rows the 8 columns (S^T = K Q^T,
+// O^T = V^T P^T), so that 8 rows, the common group of heads, fill the instruction. Which elements share a k16 step is free
+// as long as queries and keys agree, so a lane takes 16 consecutive bytes of a key row, enough for four steps.
 constexpr int kTile = 128;
 constexpr int kWarpTokens = 32;
 constexpr int kAttnThreads = 128;
 constexpr float kShift = 10.0f;  // weights are kept as 2^(x - max + 10): fp16 then reaches down to 2^-34 of the largest
 
 struct KvPartials {
-    float* out;     // [slot][16][EP]
-    float2* stats;  // [slot][16]: maximum (log2), sum
-    float* scores;  // [item][16][capacity] log2 scores, or null
+    float* out;     // [slot][row tile's rows][EP]
+    float2* stats;  // [slot][row tile's rows]: maximum (log2), sum
+    float* scores;  // [batch * kv_heads][row tile's rows][capacity] log2 scores, or null
     float* lse2;    // [batch * kv_heads][rows]: log2 of the sum of 2^score
 };
 
-template <int EP>
+// NT: column tiles of 8 query rows.
+template <int EP, int NT>
 struct AttnShape {
+    static constexpr int kRows = 8 * NT;
     static constexpr int kChunks = EP / 16;
-    static constexpr int kStages = EP == 64 ? 4 : 3;
-    static constexpr int kSliceBytes = kWarpTokens * EP;      // keys, or values, of one warp's tokens
+    static constexpr int kStages = EP == 64 ? 3 : 2;
+    static constexpr int kCtas = EP == 64 ? 4 : EP == 128 ? 3 : 1;  // on an SM
+    static constexpr int kSliceBytes = kWarpTokens * EP;            // keys, or values, of one warp's tokens
     static constexpr int kStageBytes = 2 * kSliceBytes;
     static constexpr int kWarpBytes = kStages * kStageBytes;
-    static constexpr int kScaleBytes = 4 * kStages * 2 * 4;   // after the four warps' stages
-    static constexpr int kSmem = 4 * kWarpBytes + kScaleBytes + 4 * 16 * 8 + 64;
-    static_assert(kWarpBytes >= 16 * EP * 4, "the outputs of an item's join reuse a warp's stages");
+    static constexpr int kScaleBytes = 4 * kStages * 2 * 4;         // after the four warps' stages
+    static constexpr int kSmem = 4 * kWarpBytes + kScaleBytes + 4 * kRows * 8 + 64;
+    static constexpr int kJoin = EP + 8;  // floats between rows in the join: no two rows of a store meet in a bank
+    static_assert(kWarpBytes >= kRows * kJoin * 4, "the outputs of an item's join reuse a warp's stages");
 };
 
 // Byte offset of 16-byte chunk `c` of row `r`: chunks are permuted within 128 bytes so that neither the key reads (two
@@ -308,31 +313,45 @@ __device__ __forceinline__ const uint16_t* query_row(const KvAttnArgs& a, int n,
            static_cast<int64_t>(h * a.group + j) * a.q_stride_h + t * a.q_stride_t;
 }
 
-// The A fragments of 16 query rows as fp16, and each lane's two row factors (inverse of the rows' powers of two).
-// Registers [kc * 16 + s * 4 + i]: 64-wide span kc, step s, fragment register i.
+// The B fragments of 8 query rows as fp16: registers [kc * 8 + step * 2 + i], 64-wide span kc, fragment register i. The
+// lane's row is row0 + lane / 4; the inverse of the row's power of two goes to inv[0], inv[1] for the rows 2 c and 2 c + 1
+// (c = lane % 4), the columns that the lane has of an accumulator.
 template <int EP>
 __device__ __forceinline__ void load_query(const KvAttnArgs& a, int n, int h, int row0, uint32_t* q, float* inv) {
     const int lane = threadIdx.x & 31, c = lane & 3;
+    const uint16_t* p = query_row(a, n, h, row0 + (lane >> 2));
+    uint32_t x[EP / 8];
 #pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        const uint16_t* p = query_row(a, n, h, row0 + (lane >> 2) + half * 8);
-        uint32_t x[EP / 8];
+    for (int kc = 0; kc < EP / 64; ++kc) load_row<2>(a, p, kc * 64 + c * 16, x + kc * 8);
+    float amax = row_max<EP / 8>(a, x);
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+    float mul, mine;
+    row_power(amax, mul, mine);
 #pragma unroll
-        for (int kc = 0; kc < EP / 64; ++kc) load_row<2>(a, p, kc * 64 + c * 16, x + kc * 8);
-        float amax = row_max<EP / 8>(a, x);
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-        amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-        float mul;
-        row_power(amax, mul, inv[half]);
-#pragma unroll
-        for (int kc = 0; kc < EP / 64; ++kc)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float2 f = unpack16(x[kc * 8 + j], a.query_bf16);
-                // words 2s and 2s + 1 of the lane's 16 elements are step s's k columns (2c, 2c+1) and (2c+8, 2c+9)
-                q[kc * 16 + (j >> 1) * 4 + (j & 1) * 2 + half] = pack_half2(f.x * mul, f.y * mul);
-            }
+    for (int j = 0; j < EP / 8; ++j) {
+        // words 2 s and 2 s + 1 of the lane's 16 elements are step s's k rows (2c, 2c + 1) and (2c + 8, 2c + 9)
+        const float2 f = unpack16(x[j], a.query_bf16);
+        q[j] = pack_half2(f.x * mul, f.y * mul);
     }
+    inv[0] = __shfl_sync(0xffffffffu, mine, c * 8);
+    inv[1] = __shfl_sync(0xffffffffu, mine, c * 8 + 4);
+}
+
+// The 8 x 8 matrix of 16-bit elements that the warp's words hold, transposed.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+    uint32_t d;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(x));
+    return d;
+}
+
+// Four fp32 of an output row in the query's type.
+__device__ __forceinline__ uint2 pack_out(float4 v, float g, bool bf16) {
+    if (bf16) {
+        const __nv_bfloat162 lo = __floats2bfloat162_rn(v.x * g, v.y * g), hi = __floats2bfloat162_rn(v.z * g, v.w * g);
+        return make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+    }
+    return make_uint2(pack_half2(v.x * g, v.y * g), pack_half2(v.z * g, v.w * g));
 }
 
 // Tiles of a sequence of `len` tokens: at least one, so that an empty sequence's outputs are written too.
@@ -372,14 +391,16 @@ __device__ __forceinline__ TilePos find_tile(const KvAttnArgs& a, int per_seq, i
     return TilePos{a.batch, 0, 0, base};
 }
 
-template <bool E4M3, int EP>
-__global__ void __launch_bounds__(kAttnThreads, EP == 256 ? 1 : EP == 128 ? 2 : 3) k_kv_attend(KvAttnArgs a, KvPartials w, int row_tiles) {
-    using S = AttnShape<EP>;
+template <bool E4M3, int EP, int NT>
+__global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_attend(KvAttnArgs a, KvPartials w, int row_tiles) {
+    using S = AttnShape<EP, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
+    // what follows may be launched already: it waits for this grid's end before it reads
+    asm volatile("griddepcontrol.launch_dependents;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c4 = lane & 3, r4 = lane >> 2;
     uint8_t* const stages = smem + warp * S::kWarpBytes;
     float* const scales = reinterpret_cast<float*>(smem + 4 * S::kWarpBytes) + warp * S::kStages * 2;
-    float2* const joined = reinterpret_cast<float2*>(smem + 4 * S::kWarpBytes + S::kScaleBytes);  // [warp][16]
+    float2* const joined = reinterpret_cast<float2*>(smem + 4 * S::kWarpBytes + S::kScaleBytes);  // [warp][row]
     const uint32_t stages_s = static_cast<uint32_t>(__cvta_generic_to_shared(stages));
     const uint32_t scales_s = static_cast<uint32_t>(__cvta_generic_to_shared(scales));
     const int per_seq = a.kv_heads * row_tiles;
@@ -403,17 +424,17 @@ __global__ void __launch_bounds__(kAttnThreads, EP == 256 ? 1 : EP == 128 ? 2 : 
         const uint8_t* const vbase = a.value + head * a.capacity * a.head_dim;
         const float* const ks = a.key_scale + head * a.nblocks;
         const float* const vs = a.value_scale + head * a.nblocks;
-        const int row_lo = rt * 16 + r4, row_hi = row_lo + 8;
-        const int lim_lo = kv_limit(a, row_lo, len, cnt), lim_hi = kv_limit(a, row_hi, len, cnt);
         float* const scores = w.scores == nullptr ? nullptr
-                                                  : w.scores + (head * row_tiles + rt) * 16 * static_cast<size_t>(a.capacity);
+                                                  : w.scores + head * S::kRows * static_cast<size_t>(a.capacity);
 
-        auto fetch = [&](int it) {
+        const auto fetch = [&](int it) {
             const int st = it % S::kStages;
             const int tok = (t0 + it) * kTile + warp * kWarpTokens;
             if (it < nt && tok < len) {
                 const uint32_t ks_s = stages_s + st * S::kStageBytes, vs_s = ks_s + S::kSliceBytes;
                 const size_t off = static_cast<size_t>(tok) * a.head_dim;
+                // rows a lane copies are 32 / kChunks apart, columns the same: one address and one swizzle a lane where
+                // that is the swizzle's period
 #pragma unroll
                 for (int j = 0; j < S::kChunks; ++j) {
                     const int idx = j * 32 + lane, r = idx / S::kChunks, c = idx % S::kChunks;
@@ -430,20 +451,28 @@ __global__ void __launch_bounds__(kAttnThreads, EP == 256 ? 1 : EP == 128 ? 2 : 
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
 
-        float o[EP / 16][2][4];
-#pragma unroll
-        for (int i = 0; i < EP / 16; ++i)
-#pragma unroll
-            for (int j = 0; j < 8; ++j) o[i][j >> 2][j & 3] = 0.0f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
-
 #pragma unroll
         for (int it = 0; it < S::kStages - 1; ++it) fetch(it);
-        uint32_t q[EP / 4];
-        float f[2];
-        load_query<EP>(a, n, h, rt * 16, q, f);
-        f[0] *= a.scale_log2 * code_unit<E4M3>();
-        f[1] *= a.scale_log2 * code_unit<E4M3>();
+        uint32_t q[NT][EP / 8];
+        float f[NT][2];
+        int lim[NT][2], least = INT_MAX;
+        float o[EP / 16][NT][4], m[NT][2], l[NT][2];
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            load_query<EP>(a, n, h, rt * S::kRows + j * 8, q[j], f[j]);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                f[j][i] *= a.scale_log2;
+                lim[j][i] = kv_limit(a, rt * S::kRows + j * 8 + c4 * 2 + i, len, cnt);
+                least = min(least, lim[j][i]);
+                m[j][i] = -INFINITY;
+                l[j][i] = 0.0f;
+            }
+#pragma unroll
+            for (int e = 0; e < EP / 16; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[e][j][i] = 0.0f;
+        }
 
         for (int it = 0; it < nt; ++it) {
             asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 2) : "memory");
@@ -453,81 +482,95 @@ __global__ void __launch_bounds__(kAttnThreads, EP == 256 ? 1 : EP == 128 ? 2 : 
             if (tok >= len) continue;
             const int st = it % S::kStages;
             const uint8_t* const kst = stages + st * S::kStageBytes;
-            const float kscale = scales[st * 2], vscale = scales[st * 2 + 1] * code_unit<E4M3>();
+            const float kscale = scales[st * 2], vscale = scales[st * 2 + 1];
 
-            float s[4][4];
+            // scores: accumulator t of 16 tokens has tokens r4 (registers 0, 1) and r4 + 8 (2, 3), rows 2 c4 and 2 c4 + 1
+            float s[2][NT][4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                s[j][0] = s[j][1] = s[j][2] = s[j][3] = 0.0f;
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int j = 0; j < NT; ++j) s[t][j][0] = s[t][j][1] = s[t][j][2] = s[t][j][3] = 0.0f;
 #pragma unroll
                 for (int kc = 0; kc < EP / 64; ++kc) {
-                    const uint4 k4 = *reinterpret_cast<const uint4*>(kst + swizzled<EP>(j * 8 + r4, kc * 4 + c4));
-                    const uint32_t kw[4] = {k4.x, k4.y, k4.z, k4.w};
+                    const uint4 lo = *reinterpret_cast<const uint4*>(kst + swizzled<EP>(t * 16 + r4, kc * 4 + c4));
+                    const uint4 hi = *reinterpret_cast<const uint4*>(kst + swizzled<EP>(t * 16 + r4 + 8, kc * 4 + c4));
+                    const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                     for (int step = 0; step < 4; ++step) {
-                        uint32_t b0, b1;
-                        codes_to_half<E4M3, 0>(kw[step], b0, b1);
-                        const uint32_t* qa = q + kc * 16 + step * 4;
-                        mma16816(s[j], qa[0], qa[1], qa[2], qa[3], b0, b1);
+                        uint32_t a0, a1, a2, a3;
+                        codes_to_half<E4M3, 0>(wl[step], a0, a2);
+                        codes_to_half<E4M3, 0>(wh[step], a1, a3);
+#pragma unroll
+                        for (int j = 0; j < NT; ++j)
+                            mma16816(s[t][j], a0, a1, a2, a3, q[j][kc * 8 + step * 2], q[j][kc * 8 + step * 2 + 1]);
                     }
                 }
             }
-            const float g[2] = {f[0] * kscale, f[1] * kscale};
-            float top[2] = {-INFINITY, -INFINITY};
-            const bool ragged = tok + kWarpTokens > min(lim_lo, lim_hi);
+            const bool ragged = __any_sync(0xffffffffu, tok + kWarpTokens > least);
+            bool grown = false;
+            float alpha[NT][2], base[NT][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int j = 0; j < NT; ++j)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = s[j][i] * g[i >> 1];
-                    if (ragged && tok + j * 8 + c4 * 2 + (i & 1) >= (i < 2 ? lim_lo : lim_hi)) v = -INFINITY;
-                    s[j][i] = v;
-                    top[i >> 1] = fmaxf(top[i >> 1], v);
+                for (int i = 0; i < 2; ++i) {
+                    const float g = f[j][i] * kscale;
+                    float top = -INFINITY;
+#pragma unroll
+                    for (int t = 0; t < 2; ++t)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            float v = s[t][j][k * 2 + i] * g;
+                            if (ragged && tok + t * 16 + k * 8 + r4 >= lim[j][i]) v = -INFINITY;
+                            s[t][j][k * 2 + i] = v;
+                            top = fmaxf(top, v);
+                        }
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
+                    const float now = fmaxf(m[j][i], top);
+                    alpha[j][i] = now == m[j][i] ? 1.0f : ex2(m[j][i] - now);
+                    grown |= now != m[j][i];
+                    m[j][i] = now;
+                    base[j][i] = now == -INFINITY ? 0.0f : now - kShift;  // a row that saw nothing: 2^-inf = 0
                 }
             if (scores != nullptr) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const size_t t = tok + j * 8 + c4 * 2;  // the capacity is a multiple of 32: the pair is inside
-                    *reinterpret_cast<float2*>(scores + r4 * static_cast<size_t>(a.capacity) + t) =
-                        make_float2(s[j][0], s[j][1]);
-                    *reinterpret_cast<float2*>(scores + (r4 + 8) * static_cast<size_t>(a.capacity) + t) =
-                        make_float2(s[j][2], s[j][3]);
-                }
-            }
-            float base[2];
-            bool grown = false;
-            float alpha[2];
+                for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-                top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-                const float now = fmaxf(m[i], top[i]);
-                alpha[i] = now == m[i] ? 1.0f : ex2(m[i] - now);
-                grown |= now != m[i];
-                m[i] = now;
-                base[i] = now == -INFINITY ? 0.0f : now - kShift;  // a row that saw nothing: 2^-inf = 0
+                    for (int i = 0; i < 2; ++i) {
+                        const int row = j * 8 + c4 * 2 + i;
+                        if (row >= a.rows) continue;
+                        float* const sc = scores + row * static_cast<size_t>(a.capacity) + tok + r4;
+#pragma unroll
+                        for (int t = 0; t < 2; ++t)
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) sc[t * 16 + k * 8] = s[t][j][k * 2 + i];
+                    }
             }
             if (__any_sync(0xffffffffu, grown)) {
-                l[0] *= alpha[0];
-                l[1] *= alpha[1];
 #pragma unroll
-                for (int i = 0; i < EP / 16; ++i)
+                for (int j = 0; j < NT; ++j) {
+                    l[j][0] *= alpha[j][0];
+                    l[j][1] *= alpha[j][1];
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) o[i][j >> 2][j & 3] *= alpha[(j & 3) >> 1];
-            }
-            uint32_t p[4][2];
+                    for (int e = 0; e < EP / 16; ++e)
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    s[j][i] = ex2(s[j][i] - base[i >> 1]);
-                    l[i >> 1] += s[j][i];
+                        for (int i = 0; i < 4; ++i) o[e][j][i] *= alpha[j][i & 1];
                 }
-                // fp16 weights: 11 significant bits, half a bf16 output's rounding at most
-                p[j][0] = pack_half2(s[j][0], s[j][1]);
-                p[j][1] = pack_half2(s[j][2], s[j][3]);
             }
-            // values: 8 x 8 pairs of bytes transposed on the way in; even and odd elements become two column tiles
+            // weights: fp16 (11 significant bits, half a bf16 output's rounding at most), as the B operand of 16 tokens
+            uint32_t p[2][NT][2];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const float u = ex2(s[t][j][k * 2] - base[j][0]), v = ex2(s[t][j][k * 2 + 1] - base[j][1]);
+                        l[j][0] += u;
+                        l[j][1] += v;
+                        p[t][j][k] = transpose8(pack_half2(u, v));
+                    }
+            // values: 8 x 8 pairs of bytes transposed on the way in; even elements are rows 0-7 of the operand, odd 8-15
             const uint32_t vst = stages_s + st * S::kStageBytes + S::kSliceBytes;
 #pragma unroll
             for (int e = 0; e < EP / 16; ++e) {
@@ -535,84 +578,72 @@ __global__ void __launch_bounds__(kAttnThreads, EP == 256 ? 1 : EP == 128 ? 2 : 
                 asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                              : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3])
                              : "r"(vst + swizzled<EP>(lane, e)));
-                float even[4] = {0.0f, 0.0f, 0.0f, 0.0f}, odd[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                float acc[NT][4];
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    uint32_t e0, o0, e1, o1;
-                    codes_to_half<E4M3, 1>(v[2 * j], e0, o0);
-                    codes_to_half<E4M3, 1>(v[2 * j + 1], e1, o1);
-                    mma16816(even, p[2 * j][0], p[2 * j][1], p[2 * j + 1][0], p[2 * j + 1][1], e0, e1);
-                    mma16816(odd, p[2 * j][0], p[2 * j][1], p[2 * j + 1][0], p[2 * j + 1][1], o0, o1);
+                for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t) {
+                    uint32_t a0, a1, a2, a3;
+                    codes_to_half<E4M3, 1>(v[2 * t], a0, a1);
+                    codes_to_half<E4M3, 1>(v[2 * t + 1], a2, a3);
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) mma16816(acc[j], a0, a1, a2, a3, p[t][j][0], p[t][j][1]);
                 }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    o[e][0][i] = fmaf(vscale, even[i], o[e][0][i]);
-                    o[e][1][i] = fmaf(vscale, odd[i], o[e][1][i]);
-                }
+                for (int j = 0; j < NT; ++j)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) o[e][j][i] = fmaf(vscale, acc[j][i], o[e][j][i]);
             }
         }
 
-        // join the four warps' states; the stages are free once every warp's copies have landed
+        // join the four warps' states; a warp's stages are free once its copies have landed
         asm volatile("cp.async.wait_group 0;" ::: "memory");
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 1);
-            l[i] += __shfl_xor_sync(0xffffffffu, l[i], 2);
-            if (c4 == 0) joined[warp * 16 + r4 + i * 8] = make_float2(m[i], l[i]);
-        }
-        float* const mine = reinterpret_cast<float*>(stages);
         __syncwarp();
+        float* const mine = reinterpret_cast<float*>(stages);
 #pragma unroll
-        for (int e = 0; e < EP / 16; ++e)
+        for (int j = 0; j < NT; ++j)
 #pragma unroll
-            for (int i = 0; i < 2; ++i)
-                *reinterpret_cast<float4*>(mine + (r4 + i * 8) * EP + e * 16 + c4 * 4) =
-                    make_float4(o[e][0][i * 2], o[e][1][i * 2], o[e][0][i * 2 + 1], o[e][1][i * 2 + 1]);
+            for (int i = 0; i < 2; ++i) {
+                const int r = j * 8 + c4 * 2 + i;
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) l[j][i] += __shfl_xor_sync(0xffffffffu, l[j][i], d);
+                if (r4 == 0) joined[warp * S::kRows + r] = make_float2(m[j][i], l[j][i]);
+#pragma unroll
+                for (int e = 0; e < EP / 16; ++e)
+                    *reinterpret_cast<float2*>(mine + r * S::kJoin + e * 16 + r4 * 2) = make_float2(o[e][j][i], o[e][j][i + 2]);
+            }
         __syncthreads();
         const bool whole = nt == tiles;
         // a CTA has at most two open ends: an item that began before its stretch, and one that goes on behind it
         const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (t0 > 0 ? 0 : 1);
-        for (int idx = threadIdx.x; idx < 16 * (EP / 4); idx += kAttnThreads) {
-            const int r = idx / (EP / 4), e = (idx % (EP / 4)) * 4;
-            float2 ml[4];
+        for (int idx = threadIdx.x; idx < S::kRows * (EP / 4); idx += kAttnThreads) {
+            const int r = idx / (EP / 4), e = (idx % (EP / 4)) * 4, row = rt * S::kRows + r;
+            if (row >= a.rows) continue;
             float mm = -INFINITY, ll = 0.0f;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                ml[k] = joined[k * 16 + r];
-                mm = fmaxf(mm, ml[k].x);
-            }
+            for (int k = 0; k < 4; ++k) mm = fmaxf(mm, joined[k * S::kRows + r].x);
             float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
-                const float g = ml[k].x == mm ? 1.0f : ex2(ml[k].x - mm);
-                ll += ml[k].y * g;
-                const float4 v = *reinterpret_cast<const float4*>(smem + k * S::kWarpBytes + (r * EP + e) * 4);
+                const float2 ml = joined[k * S::kRows + r];
+                const float g = ml.x == mm ? 1.0f : ex2(ml.x - mm);
+                ll += ml.y * g;
+                const float4 v = *reinterpret_cast<const float4*>(smem + k * S::kWarpBytes + (r * S::kJoin + e) * 4);
                 acc.x = fmaf(v.x, g, acc.x);
                 acc.y = fmaf(v.y, g, acc.y);
                 acc.z = fmaf(v.z, g, acc.z);
                 acc.w = fmaf(v.w, g, acc.w);
             }
             if (!whole) {
-                reinterpret_cast<float4*>(w.out)[(slot * 16 + r) * (EP / 4) + e / 4] = acc;
-                if (e == 0) w.stats[slot * 16 + r] = make_float2(mm, ll);
+                reinterpret_cast<float4*>(w.out)[(slot * S::kRows + r) * (EP / 4) + e / 4] = acc;
+                if (e == 0) w.stats[slot * S::kRows + r] = make_float2(mm, ll);
                 continue;
             }
-            const int row = rt * 16 + r;
-            if (row >= a.rows) continue;
-            const float g = ll == 0.0f ? 0.0f : 1.0f / ll;
             const int t = row / a.group, j = row - t * a.group;
-            const size_t orow = (static_cast<size_t>(n) * a.kv_heads * a.group + h * a.group + j) * a.tokens + t;
-            if (e < a.head_dim) {
-                uint2 u;
-                if (a.query_bf16) {
-                    const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * g, acc.y * g);
-                    const __nv_bfloat162 hi = __floats2bfloat162_rn(acc.z * g, acc.w * g);
-                    u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
-                } else {
-                    u = make_uint2(pack_half2(acc.x * g, acc.y * g), pack_half2(acc.z * g, acc.w * g));
-                }
-                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) = u;
-            }
+            const size_t orow = (head * a.group + j) * a.tokens + t;
+            if (e < a.head_dim)
+                *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) =
+                    pack_out(acc, ll == 0.0f ? 0.0f : 1.0f / ll, a.query_bf16);
             if (e == 0) {
                 const float lse2 = ll == 0.0f ? -INFINITY : mm + log2f(ll) - kShift;
                 if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
@@ -626,72 +657,80 @@ __global__ void __launch_bounds__(kAttnThreads, EP == 256 ? 1 : EP == 128 ? 2 : 
 }
 
 // Joins the parts of the items that more than one CTA of k_kv_attend (of `grid` CTAs) worked on: one (item, row) per
-// CTA, a thread per four output elements.
+// warp, four CTAs' parts at a time.
 template <int EP>
-__global__ void __launch_bounds__(EP / 4 < 32 ? 32 : EP / 4) k_kv_merge(KvAttnArgs a, KvPartials w, int row_tiles, int grid) {
-    const int per_seq = a.kv_heads * row_tiles;
-    const int64_t item = blockIdx.x / 16;
-    const int r = blockIdx.x % 16;
+__global__ void __launch_bounds__(128) k_kv_merge(KvAttnArgs a, KvPartials w, int row_tiles, int tile_rows, int grid) {
+    asm volatile("griddepcontrol.launch_dependents;");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int lane = threadIdx.x & 31, per_seq = a.kv_heads * row_tiles;
+    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+    const int64_t item = unit / tile_rows;
+    const int r = static_cast<int>(unit % tile_rows);
     const int n = static_cast<int>(item / per_seq), in_seq = static_cast<int>(item % per_seq);
-    const int h = in_seq / row_tiles, row = (in_seq % row_tiles) * 16 + r;
-    if (row >= a.rows) return;
+    const int h = in_seq / row_tiles, row = (in_seq % row_tiles) * tile_rows + r;
+    if (n >= a.batch || row >= a.rows) return;
     // list position of the item's first tile
     int64_t total = 0, first = 0;
-    {
-        const int lane = threadIdx.x & 31;
-        for (int n0 = 0; n0 < a.batch; n0 += 32) {
-            const int k = n0 + lane;
-            int64_t t = k < a.batch ? static_cast<int64_t>(tiles_of(kv_length(a.lengths, k, a.capacity))) * per_seq : 0;
-            int64_t before = k < n ? t : 0;
+    for (int n0 = 0; n0 < a.batch; n0 += 32) {
+        const int k = n0 + lane;
+        int64_t t = k < a.batch ? static_cast<int64_t>(tiles_of(kv_length(a.lengths, k, a.capacity))) * per_seq : 0;
+        int64_t before = k < n ? t : 0;
 #pragma unroll
-            for (int d = 16; d > 0; d >>= 1) {
-                t += __shfl_xor_sync(0xffffffffu, t, d);
-                before += __shfl_xor_sync(0xffffffffu, before, d);
-            }
-            total += t;
-            first += before;
+        for (int d = 16; d > 0; d >>= 1) {
+            t += __shfl_xor_sync(0xffffffffu, t, d);
+            before += __shfl_xor_sync(0xffffffffu, before, d);
         }
+        total += t;
+        first += before;
     }
     const int tiles = tiles_of(kv_length(a.lengths, n, a.capacity));
     first += static_cast<int64_t>(in_seq) * tiles;
     const int64_t each = (total + grid - 1) / grid;
-    const int c0 = static_cast<int>(first / each), c1 = static_cast<int>((first + tiles - 1) / each);
-    if (c0 == c1) return;
-    const int e = threadIdx.x * 4;
+    const int c0 = static_cast<int>(first / each), parts = static_cast<int>((first + tiles - 1) / each) - c0 + 1;
+    if (parts == 1) return;
+    // part k is in slot 2 (c0 + k) but for the first, which goes on behind its stretch: 2 c0 + 1
+    const float2* const stats = w.stats + static_cast<size_t>(c0) * 2 * tile_rows + r;
+    const float* const out = w.out + (static_cast<size_t>(c0) * 2 * tile_rows + r) * EP;
     float mm = -INFINITY;
-    for (int c = c0; c <= c1; ++c) mm = fmaxf(mm, w.stats[(static_cast<size_t>(c) * 2 + (c == c0 ? 1 : 0)) * 16 + r].x);
+    for (int k = lane; k < parts; k += 32) mm = fmaxf(mm, stats[static_cast<size_t>(k == 0 ? 1 : 2 * k) * tile_rows].x);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) mm = fmaxf(mm, __shfl_xor_sync(0xffffffffu, mm, d));
     float ll = 0.0f;
-    float4 acc = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll 4
-    for (int c = c0; c <= c1; ++c) {
-        const size_t slot = (static_cast<size_t>(c) * 2 + (c == c0 ? 1 : 0)) * 16 + r;
-        const float2 ml = w.stats[slot];
+    constexpr int kVec = EP / 64;  // float2 of the row a lane has
+    float2 acc[kVec];
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) acc[v] = make_float2(0.0f, 0.0f);
+#pragma unroll 8
+    for (int k = 0; k < parts; ++k) {
+        const size_t at = static_cast<size_t>(k == 0 ? 1 : 2 * k) * tile_rows;
+        const float2 ml = stats[at];
         const float g = ml.x == mm ? 1.0f : ex2(ml.x - mm);
         ll += ml.y * g;
-        if (e < EP) {
-            const float4 v = reinterpret_cast<const float4*>(w.out)[slot * (EP / 4) + threadIdx.x];
-            acc.x = fmaf(v.x, g, acc.x);
-            acc.y = fmaf(v.y, g, acc.y);
-            acc.z = fmaf(v.z, g, acc.z);
-            acc.w = fmaf(v.w, g, acc.w);
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+            const float2 u = reinterpret_cast<const float2*>(out + at * EP)[v * 32 + lane];
+            acc[v].x = fmaf(u.x, g, acc[v].x);
+            acc[v].y = fmaf(u.y, g, acc[v].y);
         }
     }
     const float g = ll == 0.0f ? 0.0f : 1.0f / ll;
     const int t = row / a.group, j = row - t * a.group;
     const size_t head = static_cast<size_t>(n) * a.kv_heads + h;
     const size_t orow = (head * a.group + j) * a.tokens + t;
-    if (e < a.head_dim) {
-        uint2 u;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) {
+        const int e = (v * 32 + lane) * 2;
+        if (e >= a.head_dim) continue;
+        uint32_t u;
         if (a.query_bf16) {
-            const __nv_bfloat162 lo = __floats2bfloat162_rn(acc.x * g, acc.y * g);
-            const __nv_bfloat162 hi = __floats2bfloat162_rn(acc.z * g, acc.w * g);
-            u = make_uint2(*reinterpret_cast<const uint32_t*>(&lo), *reinterpret_cast<const uint32_t*>(&hi));
+            const __nv_bfloat162 b = __floats2bfloat162_rn(acc[v].x * g, acc[v].y * g);
+            u = *reinterpret_cast<const uint32_t*>(&b);
         } else {
-            u = make_uint2(pack_half2(acc.x * g, acc.y * g), pack_half2(acc.z * g, acc.w * g));
+            u = pack_half2(acc[v].x * g, acc[v].y * g);
         }
-        *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) = u;
+        *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + orow * a.head_dim + e) = u;
     }
-    if (e == 0) {
+    if (lane == 0) {
         const float lse2 = ll == 0.0f ? -INFINITY : mm + log2f(ll) - kShift;
         if (a.lse != nullptr) a.lse[orow] = lse2 * kLn2;
         if (w.lse2 != nullptr) w.lse2[head * a.rows + row] = lse2;
@@ -704,15 +743,17 @@ __device__ __forceinline__ float weight_of(float score, float lse2) {
 }
 
 // Weights from the stored scores: a thread sums four tokens' columns over the (at most 16) rows of a head.
-__global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w) {
+__global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w, int tile_rows) {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const size_t head = blockIdx.y + static_cast<size_t>(gridDim.y) * blockIdx.z;
     const int n = static_cast<int>(head / a.kv_heads);
     if (n >= a.batch) return;
     const int len = kv_length(a.lengths, n, a.capacity);
     const int64_t t = (static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x) * 4;
     if (t >= len) return;
-    const float* sc = w.scores + head * 16 * static_cast<size_t>(a.capacity) + t;
+    const float* sc = w.scores + head * tile_rows * static_cast<size_t>(a.capacity) + t;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 4
     for (int r = 0; r < a.rows; ++r) {
         const float lse2 = w.lse2[head * a.rows + r];
         const float4 x = *reinterpret_cast<const float4*>(sc + r * static_cast<size_t>(a.capacity));
@@ -727,12 +768,11 @@ __global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w) 
         if (t + i < len) o[i] = a.accumulate ? o[i] + v[i] : v[i];
 }
 
-// Weights of many query rows: the scores are computed again, 128 tokens of a head a CTA, 32 a warp, with the keys in
-// registers and the rows streamed past them 16 at a time; every token's sum stays in one lane's registers until the
-// end, so there are no atomics and the order of the sum is fixed.
+// Weights of heads larger than the tensor-core kernels take: the scores are computed again, 128 tokens of a head a CTA,
+// 32 a warp, with the keys in registers and the rows streamed past them 8 at a time; every token's sum stays in one
+// lane's registers until the end, so there are no atomics and the order of the sum is fixed.
 template <bool E4M3, int EP>
-__global__ void __launch_bounds__(kAttnThreads) k_kv_column_sums(KvAttnArgs a, const float* __restrict__ lse2s, int row_tiles,
-                                                                 int key_tiles) {
+__global__ void __launch_bounds__(kAttnThreads) k_kv_column_sums(KvAttnArgs a, const float* __restrict__ lse2s, int key_tiles) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c4 = lane & 3, r4 = lane >> 2;
     const size_t head = blockIdx.x / key_tiles;
     const int n = static_cast<int>(head / a.kv_heads), h = static_cast<int>(head % a.kv_heads);
@@ -740,68 +780,66 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv_column_sums(KvAttnArgs a, c
     const int tok = static_cast<int>(blockIdx.x % key_tiles) * kTile + warp * kWarpTokens;
     if (tok >= len) return;
     const uint8_t* const kbase = a.key + (head * a.capacity + tok) * a.head_dim;
-    const float kscale = a.key_scale[head * a.nblocks + (tok >> a.block_shift)] * code_unit<E4M3>();
-    float sum[4][2];
+    const float kscale = a.key_scale[head * a.nblocks + (tok >> a.block_shift)];
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // tokens r4 + 8 k
+    uint4 keys[4][EP / 64];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) sum[j][0] = sum[j][1] = 0.0f;
-    uint4 k4[4][EP / 64];
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
         for (int kc = 0; kc < EP / 64; ++kc) {
-            const int r = j * 8 + r4, e = (kc * 4 + c4) * 16;
-            k4[j][kc] = tok + r < len && e < a.head_dim
-                            ? *reinterpret_cast<const uint4*>(kbase + static_cast<size_t>(r) * a.head_dim + e)
-                            : make_uint4(0, 0, 0, 0);
+            const int r = k * 8 + r4, e = (kc * 4 + c4) * 16;
+            keys[k][kc] = tok + r < len && e < a.head_dim
+                              ? *reinterpret_cast<const uint4*>(kbase + static_cast<size_t>(r) * a.head_dim + e)
+                              : make_uint4(0, 0, 0, 0);
         }
+    const int row_tiles = (a.rows + 7) / 8;
     for (int rt = 0; rt < row_tiles; ++rt) {
         // the last row of a tile sees the most
-        const int last = min(rt * 16 + 15, a.rows - 1);
-        if (a.causal && kv_limit(a, min(last, cnt * a.group - 1), len, cnt) <= tok) continue;
-        uint32_t q[EP / 4];
-        float f[2];
-        load_query<EP>(a, n, h, rt * 16, q, f);
-        const int row[2] = {rt * 16 + r4, rt * 16 + r4 + 8};
+        const int last = min(rt * 8 + 7, min(a.rows, cnt * a.group) - 1);
+        if (last < rt * 8 || kv_limit(a, last, len, cnt) <= tok) continue;
+        uint32_t q[EP / 8];
+        float f[2], lse2[2];
         int lim[2];
-        float lse2[2];
+        load_query<EP>(a, n, h, rt * 8, q, f);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
+            const int row = rt * 8 + c4 * 2 + i;
             f[i] = f[i] * a.scale_log2 * kscale;
-            lim[i] = kv_limit(a, row[i], len, cnt);
-            lse2[i] = row[i] < a.rows ? lse2s[head * a.rows + row[i]] : 0.0f;
+            lim[i] = kv_limit(a, row, len, cnt);
+            lse2[i] = row < a.rows ? lse2s[head * a.rows + row] : 0.0f;
         }
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
+        for (int t = 0; t < 2; ++t) {
             float s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
             for (int kc = 0; kc < EP / 64; ++kc) {
-                const uint32_t kw[4] = {k4[j][kc].x, k4[j][kc].y, k4[j][kc].z, k4[j][kc].w};
+                const uint4 lo = keys[2 * t][kc], hi = keys[2 * t + 1][kc];
+                const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
                 for (int step = 0; step < 4; ++step) {
-                    uint32_t b0, b1;
-                    codes_to_half<E4M3, 0>(kw[step], b0, b1);
-                    const uint32_t* qa = q + kc * 16 + step * 4;
-                    mma16816(s, qa[0], qa[1], qa[2], qa[3], b0, b1);
+                    uint32_t a0, a1, a2, a3;
+                    codes_to_half<E4M3, 0>(wl[step], a0, a2);
+                    codes_to_half<E4M3, 0>(wh[step], a1, a3);
+                    mma16816(s, a0, a1, a2, a3, q[kc * 8 + step * 2], q[kc * 8 + step * 2 + 1]);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (tok + j * 8 + c4 * 2 + (i & 1) < lim[i >> 1])
-                    sum[j][i & 1] += ex2(s[i] * f[i >> 1] - lse2[i >> 1]);
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (tok + t * 16 + k * 8 + r4 < lim[i]) sum[t * 2 + k] += ex2(s[k * 2 + i] * f[i] - lse2[i]);
         }
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-#pragma unroll
-            for (int d = 4; d < 32; d <<= 1) sum[j][i] += __shfl_xor_sync(0xffffffffu, sum[j][i], d);
-            const int t = tok + j * 8 + c4 * 2 + i;
-            if (r4 == 0 && t < len) {
-                float* o = a.weights + head * a.capacity + t;
-                *o = a.accumulate ? *o + sum[j][i] : sum[j][i];
-            }
+    for (int k = 0; k < 4; ++k) {
+        sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
+        sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
+        const int t = tok + k * 8 + r4;
+        if (c4 == 0 && t < len) {
+            float* o = a.weights + head * a.capacity + t;
+            *o = a.accumulate ? *o + sum[k] : sum[k];
         }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -1075,11 +1113,13 @@ int with_head_dim(int64_t head_dim, F f) {
 }
 
 int64_t padded_head(int64_t e) { return e <= 64 ? 64 : e <= 128 ? 128 : 256; }
-int attn_ctas_per_sm(int64_t e) { return e <= 64 ? 3 : e <= 128 ? 2 : 1; }
+
+// Query rows in a row tile of k_kv_attend.
+int64_t tile_rows(int64_t rows) { return rows <= 8 ? 8 : 16; }
 
 // Stored scores against computing them again, where few rows ask for weights: see k_kv_weights.
 bool stores_scores(const dt_kv_cache* c, int64_t rows) {
-    return rows <= 16 && c->batch * c->kv_heads * 16 * c->capacity * 4 <= (int64_t{1} << 30);
+    return rows <= 16 && c->batch * c->kv_heads * tile_rows(rows) * c->capacity * 4 <= (int64_t{1} << 30);
 }
 
 // Many rows of a head take the tensor-core kernel.
@@ -1101,22 +1141,23 @@ int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool we
     if (st != DT_OK) return st;
     const int64_t ep = padded_head(c->head_dim);
     p->rows = query_heads / c->kv_heads * tokens;
-    p->row_tiles = (p->rows + 15) / 16;
+    p->row_tiles = (p->rows + tile_rows(p->rows) - 1) / tile_rows(p->rows);
     p->many_rows = many_rows(c, p->rows);
-    p->grid = sms * attn_ctas_per_sm(c->head_dim);
+    p->grid = sms * (ep == 64 ? AttnShape<64, 1>::kCtas : ep == 128 ? AttnShape<128, 1>::kCtas : AttnShape<256, 1>::kCtas);
     const auto up = [](size_t v) { return (v + 255) / 256 * 256; };
     p->out = 0;
     if (p->many_rows) {
         p->prompt = kv_prompt_plan(c->batch, p->rows, c->head_dim, sms);
         p->lse2 = p->prompt.bytes;
     } else {
-        p->stats = up(static_cast<size_t>(p->grid) * 2 * 16 * ep * 4);
-        p->lse2 = p->stats + up(static_cast<size_t>(p->grid) * 2 * 16 * 8);
+        const size_t parts = static_cast<size_t>(p->grid) * 2 * tile_rows(p->rows);
+        p->stats = up(parts * ep * 4);
+        p->lse2 = p->stats + up(parts * 8);
     }
     p->scores = p->lse2 + (weights ? up(static_cast<size_t>(c->batch) * c->kv_heads * p->rows * 4) : 0);
     p->bytes = p->scores;
     if (weights && stores_scores(c, p->rows)) {
-        p->bytes += static_cast<size_t>(c->batch) * c->kv_heads * 16 * c->capacity * 4;
+        p->bytes += static_cast<size_t>(c->batch) * c->kv_heads * tile_rows(p->rows) * c->capacity * 4;
     } else if (weights && c->head_dim <= 128) {
         p->column_tiles = true;
         p->columns = kv_column_plan(c->batch, c->kv_heads, p->rows, c->head_dim, c->capacity, sms);
@@ -1125,42 +1166,62 @@ int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool we
     return DT_OK;
 }
 
+// Launch behind a kernel that lets its successor start early (griddepcontrol in both).
+template <typename... P, typename... A>
+int launch_next(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t stream, A... args) {
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.stream = stream;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
+    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
+    return check_launch("dt_kv_attention");
+}
+
+template <bool E4M3, int EP, int NT>
+int launch_few_rows(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, cudaStream_t stream) {
+    using S = AttnShape<EP, NT>;
+    // per device and cheap: the limit belongs to the kernel in the current context
+    const auto kernel = k_kv_attend<E4M3, EP, NT>;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
+    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
+    const int row_tiles = static_cast<int>(p.row_tiles);
+    unsigned grid = 0;
+    int st = grid_of((static_cast<int64_t>(a.batch) * a.kv_heads * row_tiles * S::kRows + 3) / 4, "dt_kv_attention", &grid);
+    if (st != DT_OK) return st;
+    kernel<<<p.grid, kAttnThreads, S::kSmem, stream>>>(a, w, row_tiles);
+    st = check_launch("dt_kv_attention");
+    if (st != DT_OK) return st;
+    return launch_next(k_kv_merge<EP>, dim3(grid), 128, stream, a, w, row_tiles, S::kRows, p.grid);
+}
+
 template <bool E4M3, int EP>
 int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, void* workspace, bool weights,
                   cudaStream_t stream) {
-    using S = AttnShape<EP>;
-    // per device and cheap: the limit belongs to the kernel in the current context
-    cudaError_t e = cudaFuncSetAttribute(k_kv_attend<E4M3, EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
-    const int row_tiles = static_cast<int>(p.row_tiles);
     int st = DT_OK;
-    unsigned grid = 0;
-    if (p.many_rows) {
-        st = kv_prompt_attention(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.prompt, workspace, w.lse2, stream);
-    } else {
-        k_kv_attend<E4M3, EP><<<p.grid, kAttnThreads, S::kSmem, stream>>>(a, w, row_tiles);
-        st = check_launch("dt_kv_attention");
-        if (st != DT_OK) return st;
-        st = grid_of(static_cast<int64_t>(a.batch) * a.kv_heads * row_tiles * 16, "dt_kv_attention", &grid);
-        if (st != DT_OK) return st;
-        k_kv_merge<EP><<<grid, std::max(32, EP / 4), 0, stream>>>(a, w, row_tiles, p.grid);
-        st = check_launch("dt_kv_attention");
-    }
+    if (p.many_rows) st = kv_prompt_attention(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.prompt, workspace, w.lse2, stream);
+    else if (tile_rows(p.rows) == 8) st = launch_few_rows<E4M3, EP, 1>(a, w, p, stream);
+    else st = launch_few_rows<E4M3, EP, 2>(a, w, p, stream);
     if (st != DT_OK || !weights) return st;
     const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
     if (w.scores != nullptr) {
         const unsigned y = static_cast<unsigned>(std::min<int64_t>(heads, 32768));
         const dim3 g(static_cast<unsigned>((a.capacity + 1023) / 1024), y, static_cast<unsigned>((heads + y - 1) / y));
-        k_kv_weights<<<g, 256, 0, stream>>>(a, w);
-    } else if (p.column_tiles) {
+        return launch_next(k_kv_weights, g, 256, stream, a, w, static_cast<int>(tile_rows(p.rows)));
+    }
+    if (p.column_tiles)
         return kv_column_sums(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.columns, static_cast<char*>(workspace) + p.scores, w.lse2,
                               stream);
-    } else {
-        const int key_tiles = static_cast<int>((a.capacity + kTile - 1) / kTile);
-        st = grid_of(heads * key_tiles, "dt_kv_attention", &grid);
-        if (st != DT_OK) return st;
-        k_kv_column_sums<E4M3, EP><<<grid, kAttnThreads, 0, stream>>>(a, w.lse2, row_tiles, key_tiles);
-    }
+    const int key_tiles = static_cast<int>((a.capacity + kTile - 1) / kTile);
+    unsigned grid = 0;
+    st = grid_of(heads * key_tiles, "dt_kv_attention", &grid);
+    if (st != DT_OK) return st;
+    k_kv_column_sums<E4M3, 256><<<grid, kAttnThreads, 0, stream>>>(a, w.lse2, key_tiles);
     return check_launch("dt_kv_attention");
 }
 

@@ -72,29 +72,22 @@ __device__ __forceinline__ uint32_t hsub2(uint32_t a, uint32_t b) {
 }
 
 // Four codes of a word to two fp16 pairs; every code is exact in fp16. SPLIT 0: pairs (0,1) and (2,3); SPLIT 1: pairs
-// (0,2) and (1,3), the byte transposition that rows read through ldmatrix.trans need, at no further cost.
-// int8: 1024 + (code + 128) is the fp16 whose low byte is code + 128; subtracting 1152 leaves the code.
-// e4m3: exponent and mantissa land in fp16's fields when shifted by one, which gives code / 256 (fp16's bias is 15,
-// e4m3's 7; subnormals included); the factor 256 is left to the scale (code_unit). 0x7f (NaN) never occurs below a
-// sequence's length: the writers saturate and mark NaN in the scale.
+// (0,2) and (1,3), the byte transposition that rows read through ldmatrix.trans need.
+// int8: 1024 + (code + 128) is the fp16 whose low byte is code + 128; subtracting 1152 leaves the code; the transposition
+// costs nothing. e4m3: the conversion instruction, which runs at the rate of a byte permutation (2 cycles a warp, measured).
 template <bool E4M3, int SPLIT>
 __device__ __forceinline__ void codes_to_half(uint32_t w, uint32_t& lo, uint32_t& hi) {
     if constexpr (E4M3) {
-        const uint32_t a = prmt(w, 0u, SPLIT ? 0x2404 : 0x1404);  // bytes to the high halves of the fp16 pair
-        const uint32_t b = prmt(w, 0u, SPLIT ? 0x3414 : 0x3424);
-        lo = (a & 0x80008000u) | ((a >> 1) & 0x3f803f80u);
-        hi = (b & 0x80008000u) | ((b >> 1) & 0x3f803f80u);
+        if (SPLIT) w = prmt(w, 0u, 0x3120);
+        asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+            : "=r"(lo), "=r"(hi)
+            : "r"(w));
     } else {
         const uint32_t u = w ^ 0x80808080u;
         lo = hsub2(prmt(u, 0x64646464u, SPLIT ? 0x4240 : 0x4140), 0x64806480u);
         hi = hsub2(prmt(u, 0x64646464u, SPLIT ? 0x4341 : 0x4342), 0x64806480u);
     }
-}
-
-// What the fp16 values of codes_to_half are short of.
-template <bool E4M3>
-__device__ __forceinline__ constexpr float code_unit() {
-    return E4M3 ? 256.0f : 1.0f;
 }
 
 __device__ __forceinline__ float ex2(float x) {

@@ -697,7 +697,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 // in the places of odd tiles: the first tile's are written before the other thread has read these
                 const float inv = stage_query<EP>(a, qp, smem + S::kQuery + g * S::kOperand, r, half, tops + 2 + half,
                                                   tops + 2 + (half ^ 1), pair, a.scale_log2 < 0.0f ? -1.0f : 1.0f);
-                factor = inv * fabsf(a.scale_log2) * code_unit<E4M3>();
+                factor = inv * fabsf(a.scale_log2);
                 tc_fence_before();  // the reads of O of the item before
                 async_proxy_fence();
                 __syncwarp();
@@ -818,7 +818,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
             l += sums[half ^ 1];
             pair_sync(pair);  // and both have read the sums, whose places take the next queries' tops
             if (*dead) l = __int_as_float(0x7fc00000);
-            const float v_up = code_unit<E4M3>() / v_down;  // powers of two
+            const float v_up = 1.0f / v_down;  // powers of two
             if (item_steps < pos.tiles) {
                 // an item that other CTAs work on too: one that began before this stretch, or goes on behind it
                 const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (pos.tile > 0 ? 0 : 1);
@@ -1045,7 +1045,7 @@ __global__ void __launch_bounds__(128) k_kv_row_blocks(KvAttnArgs a, const float
     }
     const float l = lim > 0 ? lse2[head * a.rows + row] : INFINITY;
     reinterpret_cast<float2*>(out + ColumnShape<EP>::kOperand)[r] =
-        make_float2(inv * a.scale_log2 * code_unit<E4M3>(), l == -INFINITY ? INFINITY : l);
+        make_float2(inv * a.scale_log2, l == -INFINITY ? INFINITY : l);
     reinterpret_cast<int*>(out + ColumnShape<EP>::kOperand + 128 * 8)[r] = lim;
 }
 
