@@ -6,6 +6,8 @@
 #include <cstdint>
 #include <string>
 
+#include <cooperative_groups.h>
+
 #include "dt_internal.h"
 #include "dt_kv.cuh"
 #include "dt_kv_prompt.h"
@@ -27,25 +29,38 @@ __device__ __forceinline__ float scale_of(float amax) {
     return __uint_as_float((__float_as_uint(s) + 0xffffu) & 0xffff0000u);
 }
 
-// Codes of four values. The scale has 8 significant bits and the values at most 15: an exact quotient that is not
-// half way between two codes is at least 2^-17 of it away from there, further than fp32's division is off.
+// Codes of four values x / s, to nearest, ties to even, of the exact quotient. The scale has 8 significant bits and the
+// values at most 15, so an exact quotient that is not half way between two codes is well away from there, and a product
+// with the rounded reciprocal r (off by 2^-24 of itself, so by less than 2^-17) only has to be put back on the half way
+// points that it stands for, which costs a third of a division:
+//   int8: a quotient in [2^j, 2^(j+1)) that is no half way point is 2^(j-15) away from one, 2^-16 at least. Adding and
+//   taking off 128 rounds to multiples of 2^-16; half way points are such multiples.
+//   e4m3: half way points have 5 significant bits and others differ by 2^-13 of themselves; rounding to 18 bits restores them.
+// Scales below 2^-100, whose reciprocals may not be normal, take the division.
 template <bool E4M3>
-__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float s) {
+__device__ __forceinline__ uint32_t encode4(const float* x, float s, float r) {
     if (!(s > 0.0f)) return 0;  // 0: the block is all zero; NaN: the block is marked
-    a /= s;
-    b /= s;
-    c /= s;
-    d /= s;
+    const bool divide = s < 0x1p-100f;
+    float y[4];
     if constexpr (E4M3) {
-        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
-        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            y[i] = divide ? x[i] / s : __uint_as_float((__float_as_uint(x[i] * r) + 0x20u) & ~0x3fu);
+        const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
         return lo | (hi << 16);
     } else {
-        const uint32_t lo = (__float2int_rn(a) & 0xff) | ((__float2int_rn(b) & 0xff) << 8);
-        const uint32_t hi = (__float2int_rn(c) & 0xff) | ((__float2int_rn(d) & 0xff) << 8);
-        return lo | (hi << 16);
+        uint32_t q[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            y[i] = divide ? x[i] / s : copysignf(fmaf(fabsf(x[i]), r, 128.0f) - 128.0f, x[i]);
+            q[i] = __float_as_uint(y[i] + 12582912.0f);  // 1.5 * 2^23: the integer, ties to even, in the low byte
+        }
+        return prmt(prmt(q[0], q[1], 0x0040), prmt(q[2], q[3], 0x0040), 0x5410);
     }
 }
+
+__device__ __forceinline__ float reciprocal(float s) { return s >= 0x1p-100f ? 1.0f / s : 0.0f; }
 
 // The four codes of a word as fp32 (without the scale).
 template <bool E4M3>
@@ -77,12 +92,12 @@ constexpr int kAppendThreads = 256;
 
 // One block of the cache (`block` tokens of a head, keys or values) per CTA: largest |x| of the new tokens, the
 // block's scale, their codes; where the scale grows, the earlier tokens' codes again. The new tokens stay in registers
-// between the two passes (VPT vectors of 16 elements a thread), so every element is read once. The largest |x| is
+// between the two passes (VPT vectors of 8 elements a thread), so every element is read once. The largest |x| is
 // taken on the bit patterns: it also finds infinities and NaN, which a floating maximum would drop.
 template <bool E4M3, int VPT>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(KvAppendArgs a) {
     const int tid = threadIdx.x;
-    int64_t b = blockIdx.x;
+    unsigned b = blockIdx.x;
     const int i = static_cast<int>(b % a.spans);
     b /= a.spans;
     const int kv = static_cast<int>(b & 1);
@@ -98,34 +113,35 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(KvAppendArgs a) {
     if (begin >= end) return;
     const int held = static_cast<int>(begin - slot);
     const int fresh = static_cast<int>(end - begin);
-    const int cpr = a.head_dim >> 4;  // vectors of 16 elements in a row
+    const int cpr = a.head_dim >> 3;  // vectors of 8 elements in a row
     const size_t head = static_cast<size_t>(n) * a.heads + h;
     uint8_t* dst = a.codes[kv] + (head * a.capacity + slot) * a.head_dim;
     float* scale = a.scales[kv] + head * (a.capacity >> a.block_shift) + (slot >> a.block_shift);
-    const uint16_t* src = a.src[kv] + n * a.stride[kv][0] + h * a.stride[kv][1];
+    const uint16_t* src = a.src[kv] + n * a.stride[kv][0] + h * a.stride[kv][1] + (begin - len) * a.stride[kv][2];
 
-    uint32_t x[VPT][8];
+    uint32_t x[VPT][4];
     uint32_t most = 0;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
         const int idx = v * kAppendThreads + tid;
+        x[v][0] = x[v][1] = x[v][2] = x[v][3] = 0;
         if (idx < fresh * cpr) {
             const int t = idx / cpr;
-            const uint16_t* p = src + (begin - len + t) * a.stride[kv][2] + (idx - t * cpr) * 16;
+            const uint16_t* p = src + t * a.stride[kv][2] + (idx - t * cpr) * 8;
             if (a.vec[kv]) {
-                const uint4 lo = *reinterpret_cast<const uint4*>(p);
-                const uint4 hi = *reinterpret_cast<const uint4*>(p + 8);
-                x[v][0] = lo.x, x[v][1] = lo.y, x[v][2] = lo.z, x[v][3] = lo.w;
-                x[v][4] = hi.x, x[v][5] = hi.y, x[v][6] = hi.z, x[v][7] = hi.w;
+                const uint4 u = __ldcs(reinterpret_cast<const uint4*>(p));
+                x[v][0] = u.x, x[v][1] = u.y, x[v][2] = u.z, x[v][3] = u.w;
             } else {
 #pragma unroll
-                for (int j = 0; j < 8; ++j) x[v][j] = p[2 * j] | (static_cast<uint32_t>(p[2 * j + 1]) << 16);
+                for (int j = 0; j < 4; ++j) x[v][j] = p[2 * j] | (static_cast<uint32_t>(p[2 * j + 1]) << 16);
             }
-#pragma unroll
-            for (int j = 0; j < 8; ++j) most = __vmaxu2(most, x[v][j] & 0x7fff7fffu);
         }
     }
     const float old = held > 0 ? *scale : 0.0f;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) most = __vmaxu2(most, x[v][j] & 0x7fff7fffu);
     most = max(most & 0xffffu, most >> 16);
     __shared__ uint32_t part[kAppendThreads / 32];
     most = __reduce_max_sync(0xffffffffu, most);
@@ -141,33 +157,33 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_append(KvAppendArgs a) {
         if (now > s) s = now;  // an old NaN stays
     }
     if (tid == 0) *scale = s;
+    const float r = reciprocal(s);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
         const int idx = v * kAppendThreads + tid;
         if (idx < fresh * cpr) {
-            uint32_t q[4];
+            uint32_t q[2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < 2; ++j) {
                 const float2 lo = unpack16(x[v][2 * j], a.bf16);
                 const float2 hi = unpack16(x[v][2 * j + 1], a.bf16);
-                q[j] = encode4<E4M3>(lo.x, lo.y, hi.x, hi.y, s);
+                const float f[4] = {lo.x, lo.y, hi.x, hi.y};
+                q[j] = encode4<E4M3>(f, s, r);
             }
-            *reinterpret_cast<uint4*>(dst + static_cast<size_t>(held) * a.head_dim + static_cast<size_t>(idx) * 16) =
-                make_uint4(q[0], q[1], q[2], q[3]);
+            *reinterpret_cast<uint2*>(dst + static_cast<size_t>(held) * a.head_dim + static_cast<size_t>(idx) * 8) =
+                make_uint2(q[0], q[1]);
         }
     }
     if (held > 0 && s > old) {
         for (int idx = tid; idx < held * cpr; idx += kAppendThreads) {
-            uint4* p = reinterpret_cast<uint4*>(dst) + idx;
-            const uint4 w = *p;
-            uint32_t q[4] = {w.x, w.y, w.z, w.w};
+            uint2* p = reinterpret_cast<uint2*>(dst) + idx;
+            const uint2 w = *p;
+            float f[8];
+            decode4<E4M3>(w.x, f);
+            decode4<E4M3>(w.y, f + 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float f[4];
-                decode4<E4M3>(q[j], f);
-                q[j] = encode4<E4M3>(f[0] * old, f[1] * old, f[2] * old, f[3] * old, s);
-            }
-            *p = make_uint4(q[0], q[1], q[2], q[3]);
+            for (int j = 0; j < 8; ++j) f[j] *= old;
+            *p = make_uint2(encode4<E4M3>(f, s, r), encode4<E4M3>(f + 4, s, r));
         }
     }
 }
@@ -178,57 +194,68 @@ struct KvReadArgs {
     void* out[2];
     const int32_t* lengths;
     const int32_t* first;
-    int64_t first_all, count, capacity, vectors;  // vectors of 16 elements in one output
+    int64_t first_all, count, capacity, all_heads;
     int heads, head_dim, block_shift;
     int dtype;
 };
 
-// A vector of 16 elements a thread: 16 bytes of codes in, 32 or 64 bytes out.
+// Vectors of 8 elements: 8 bytes of codes in, 16 or 32 bytes out. A thread keeps its column and takes every 256 /
+// (vectors in a row)-th token of a head, kReadRows of them at a time.
+constexpr int kReadRows = 4;
+
 template <bool E4M3>
 __global__ void __launch_bounds__(256) k_kv_read(KvReadArgs a) {
-    const int cpr = a.head_dim >> 4;
     const int kv = blockIdx.y;
     if (a.out[kv] == nullptr) return;
-    for (int64_t v = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; v < a.vectors;
-         v += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        int64_t r = v / cpr;
-        const int c = static_cast<int>(v - r * cpr);
-        const int64_t head = r / a.count;
-        const int64_t i = r - head * a.count;
+    const int cpr = a.head_dim >> 3, step = 256 / cpr;
+    const int r = threadIdx.x / cpr, c = threadIdx.x - r * cpr;
+    if (r >= step) return;
+    const int64_t i0 = static_cast<int64_t>(blockIdx.x) * step * kReadRows + r;
+    for (int64_t head = blockIdx.z; head < a.all_heads; head += gridDim.z) {
         const int n = static_cast<int>(head / a.heads);
-        const int64_t t = (a.first != nullptr ? a.first[n] : a.first_all) + i;
-        float f[16];
-        if (t >= 0 && t < kv_length(a.lengths, n, a.capacity)) {
-            const float s = a.scales[kv][head * (a.capacity >> a.block_shift) + (t >> a.block_shift)];
-            const uint4 w = reinterpret_cast<const uint4*>(a.codes[kv] + (head * a.capacity + t) * a.head_dim)[c];
-            decode4<E4M3>(w.x, f);
-            decode4<E4M3>(w.y, f + 4);
-            decode4<E4M3>(w.z, f + 8);
-            decode4<E4M3>(w.w, f + 12);
+        const int len = kv_length(a.lengths, n, a.capacity);
+        const int64_t first = a.first != nullptr ? a.first[n] : a.first_all;
+        const uint8_t* const codes = a.codes[kv] + head * a.capacity * a.head_dim + c * 8;
+        const float* const scales = a.scales[kv] + head * (a.capacity >> a.block_shift);
+        uint2 w[kReadRows];
+        float s[kReadRows];
 #pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] *= s;
-        } else {
-#pragma unroll
-            for (int j = 0; j < 16; ++j) f[j] = 0.0f;
-        }
-        if (a.dtype == DT_FLOAT32) {
-            float4* o = reinterpret_cast<float4*>(a.out[kv]) + v * 4;
-#pragma unroll
-            for (int j = 0; j < 4; ++j) o[j] = make_float4(f[4 * j], f[4 * j + 1], f[4 * j + 2], f[4 * j + 3]);
-        } else {
-            uint32_t q[8];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                if (a.dtype == DT_BFLOAT16) {
-                    const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
-                    q[j] = *reinterpret_cast<const uint32_t*>(&p);
-                } else {
-                    q[j] = pack_half2(f[2 * j], f[2 * j + 1]);
-                }
+        for (int u = 0; u < kReadRows; ++u) {
+            const int64_t i = i0 + u * step, t = first + i;
+            w[u] = make_uint2(0, 0);
+            s[u] = 0.0f;
+            if (i < a.count && t >= 0 && t < len) {
+                w[u] = __ldg(reinterpret_cast<const uint2*>(codes + t * a.head_dim));
+                s[u] = __ldg(scales + (t >> a.block_shift));
             }
-            uint4* o = reinterpret_cast<uint4*>(a.out[kv]) + v * 2;
-            o[0] = make_uint4(q[0], q[1], q[2], q[3]);
-            o[1] = make_uint4(q[4], q[5], q[6], q[7]);
+        }
+#pragma unroll
+        for (int u = 0; u < kReadRows; ++u) {
+            const int64_t i = i0 + u * step;
+            if (i >= a.count) break;
+            float f[8];
+            decode4<E4M3>(w[u].x, f);
+            decode4<E4M3>(w[u].y, f + 4);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) f[j] *= s[u];
+            const int64_t at = (head * a.count + i) * cpr + c;
+            if (a.dtype == DT_FLOAT32) {
+                float4* o = reinterpret_cast<float4*>(a.out[kv]) + at * 2;
+                o[0] = make_float4(f[0], f[1], f[2], f[3]);
+                o[1] = make_float4(f[4], f[5], f[6], f[7]);
+            } else {
+                uint32_t q[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    if (a.dtype == DT_BFLOAT16) {
+                        const __nv_bfloat162 p = __floats2bfloat162_rn(f[2 * j], f[2 * j + 1]);
+                        q[j] = *reinterpret_cast<const uint32_t*>(&p);
+                    } else {
+                        q[j] = pack_half2(f[2 * j], f[2 * j + 1]);
+                    }
+                }
+                reinterpret_cast<uint4*>(a.out[kv])[at] = make_uint4(q[0], q[1], q[2], q[3]);
+            }
         }
     }
 }
@@ -657,15 +684,16 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
 }
 
 // Joins the parts of the items that more than one CTA of k_kv_attend (of `grid` CTAs) worked on: one (item, row) per
-// warp, four CTAs' parts at a time.
+// CTA, whose warps take every fourth part; their sums are joined in a fixed order.
 template <int EP>
 __global__ void __launch_bounds__(128) k_kv_merge(KvAttnArgs a, KvPartials w, int row_tiles, int tile_rows, int grid) {
     asm volatile("griddepcontrol.launch_dependents;");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int lane = threadIdx.x & 31, per_seq = a.kv_heads * row_tiles;
-    const int64_t unit = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
-    const int64_t item = unit / tile_rows;
-    const int r = static_cast<int>(unit % tile_rows);
+    __shared__ float parts_sum[4];
+    __shared__ float parts_out[4][EP];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_seq = a.kv_heads * row_tiles;
+    const unsigned item = blockIdx.x / tile_rows;
+    const int r = static_cast<int>(blockIdx.x % tile_rows);
     const int n = static_cast<int>(item / per_seq), in_seq = static_cast<int>(item % per_seq);
     const int h = in_seq / row_tiles, row = (in_seq % row_tiles) * tile_rows + r;
     if (n >= a.batch || row >= a.rows) return;
@@ -701,7 +729,7 @@ __global__ void __launch_bounds__(128) k_kv_merge(KvAttnArgs a, KvPartials w, in
 #pragma unroll
     for (int v = 0; v < kVec; ++v) acc[v] = make_float2(0.0f, 0.0f);
 #pragma unroll 8
-    for (int k = 0; k < parts; ++k) {
+    for (int k = warp; k < parts; k += 4) {
         const size_t at = static_cast<size_t>(k == 0 ? 1 : 2 * k) * tile_rows;
         const float2 ml = stats[at];
         const float g = ml.x == mm ? 1.0f : ex2(ml.x - mm);
@@ -711,6 +739,21 @@ __global__ void __launch_bounds__(128) k_kv_merge(KvAttnArgs a, KvPartials w, in
             const float2 u = reinterpret_cast<const float2*>(out + at * EP)[v * 32 + lane];
             acc[v].x = fmaf(u.x, g, acc[v].x);
             acc[v].y = fmaf(u.y, g, acc[v].y);
+        }
+    }
+    if (lane == 0) parts_sum[warp] = ll;
+#pragma unroll
+    for (int v = 0; v < kVec; ++v) reinterpret_cast<float2*>(parts_out[warp])[v * 32 + lane] = acc[v];
+    __syncthreads();
+    if (warp != 0) return;
+#pragma unroll
+    for (int k = 1; k < 4; ++k) {
+        ll += parts_sum[k];
+#pragma unroll
+        for (int v = 0; v < kVec; ++v) {
+            const float2 u = reinterpret_cast<const float2*>(parts_out[k])[v * 32 + lane];
+            acc[v].x += u.x;
+            acc[v].y += u.y;
         }
     }
     const float g = ll == 0.0f ? 0.0f : 1.0f / ll;
@@ -890,16 +933,32 @@ __device__ __forceinline__ int block_scan(int v, int* warp_sums, int* all) {
     return incl - v + __shfl_sync(0xffffffffu, winc - wsum, warp);
 }
 
+// Four keys from position i on; positions from `end` on do not count.
+__device__ __forceinline__ void four_keys(const float* w, int i, int end, bool vec, uint32_t* key) {
+    if (vec && i + 4 <= end) {
+        const float4 v = __ldg(reinterpret_cast<const float4*>(w + i));
+        key[0] = order_key(v.x), key[1] = order_key(v.y), key[2] = order_key(v.z), key[3] = order_key(v.w);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) key[k] = i + k < end ? order_key(w[i + k]) : 0u;
+    }
+}
+
 // Positions that stay, ascending: a radix selection of the threshold weight among the tokens before the recent ones
 // (digits of 11, 11 and 10 bits, a histogram in shared memory each), then one pass that writes the positions in
-// order, of those equal to the threshold the first ones. One head per CTA.
-__global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a) {
-    __shared__ int hist[2048];
+// order, of those equal to the threshold the first ones. A head per cluster, whose CTAs have a part of the tokens each
+// and read each other's histograms and counts: a head of 131072 tokens took one CTA 238 us.
+__global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a, bool vec) {
+    namespace cg = cooperative_groups;
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
+    __shared__ int hist[2][2048];
     __shared__ int warp_sums[32];
+    __shared__ int counts[2];  // of this CTA's tokens: above the threshold, and equal to it
     __shared__ uint32_t sh_digit;
     __shared__ int sh_above;
     const int tid = threadIdx.x;
-    const size_t head = blockIdx.x;
+    const size_t head = blockIdx.x / ctas;
     const int n = static_cast<int>(head / a.heads);
     const int len = kv_length(a.lengths, n, a.src_cap);
     const int count = min(len, a.budget);
@@ -908,41 +967,59 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a) {
     int need = count - late;      // places for them
     const float* const w = a.weights + head * a.src_cap;
     int32_t* const kept = a.kept + head * a.budget;
-    if (head % a.heads == 0 && tid == 0) a.dst_lengths[n] = count;
-    for (int i = count + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
+    const int all_threads = ctas * kSelectThreads, me = rank * kSelectThreads + tid;
+    if (head % a.heads == 0 && me == 0) a.dst_lengths[n] = count;
+    for (int i = count + me; i < a.budget; i += all_threads) kept[i] = -1;
     if (need == old) {
-        for (int i = tid; i < count; i += kSelectThreads) kept[i] = i;
+        for (int i = me; i < count; i += all_threads) kept[i] = i;
         return;
     }
-    for (int i = tid; i < late; i += kSelectThreads) kept[need + i] = old + i;
+    for (int i = me; i < late; i += all_threads) kept[need + i] = old + i;
     if (need == 0) return;
 
-    const int places = need;
+    const int part = ((old + ctas - 1) / ctas + 3) & ~3;
+    const int begin = min(rank * part, old), end = min(begin + part, old);
     uint32_t prefix = 0, mask = 0;
     const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
+    for (int i = tid; i < 2048; i += kSelectThreads) hist[0][i] = 0;
+    if (tid < 2) counts[tid] = 0;
+    __syncthreads();
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = shifts[pass], size = 1 << bits[pass];
-        for (int i = tid; i < 2048; i += kSelectThreads) hist[i] = 0;
-        __syncthreads();
-        for (int i = tid; i < (old + 31) / 32 * 32; i += kSelectThreads) {
-            const uint32_t key = i < old ? order_key(w[i]) : 0u;
-            const bool in = i < old && (key & mask) == prefix;
-            const uint32_t digit = (key >> shift) & (size - 1);
-            const uint32_t live = __ballot_sync(0xffffffffu, in);
-            if (live == 0) continue;
-            const int leader = __ffs(live) - 1;
-            const uint32_t lead_digit = __shfl_sync(0xffffffffu, digit, leader);  // every lane takes part
-            // a warp whose keys agree (ties, such as tokens never attended to) adds once
-            if (__all_sync(0xffffffffu, !in || digit == lead_digit)) {
-                if ((tid & 31) == leader) atomicAdd(&hist[digit], __popc(live));
-            } else if (in) {
-                atomicAdd(&hist[digit], 1);
-            }
+        int* const mine = hist[pass & 1];
+        for (int i0 = begin; i0 < end; i0 += 4 * 4 * kSelectThreads) {
+            uint32_t key[4][4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) four_keys(w, i0 + (u * kSelectThreads + tid) * 4, end, vec, key[u]);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const bool in = i0 + (u * kSelectThreads + tid) * 4 + k < end && (key[u][k] & mask) == prefix;
+                    const uint32_t digit = (key[u][k] >> shift) & (size - 1);
+                    const uint32_t live = __ballot_sync(0xffffffffu, in);
+                    if (live == 0) continue;
+                    const int leader = __ffs(live) - 1;
+                    const uint32_t lead_digit = __shfl_sync(0xffffffffu, digit, leader);  // every lane takes part
+                    // a warp whose keys agree (ties, such as tokens never attended to) adds once
+                    if (__all_sync(0xffffffffu, !in || digit == lead_digit)) {
+                        if ((tid & 31) == leader) atomicAdd(&mine[digit], __popc(live));
+                    } else if (in) {
+                        atomicAdd(&mine[digit], 1);
+                    }
+                }
         }
-        __syncthreads();
+        cluster.sync();
+        // the other histogram was last read before this barrier
+        for (int i = tid; i < 2048; i += kSelectThreads) hist[(pass + 1) & 1][i] = 0;
         // the digit at which the count from above reaches the places that are left; two bins a thread, from the top
         const int b0 = size - 1 - 2 * tid, b1 = b0 - 1;
-        const int h0 = b0 >= 0 ? hist[b0] : 0, h1 = b1 >= 0 ? hist[b1] : 0;
+        int h0 = 0, h1 = 0;
+        for (int c = 0; c < ctas; ++c) {
+            const int* const theirs = cluster.map_shared_rank(mine, c);
+            h0 += b0 >= 0 ? theirs[b0] : 0;
+            h1 += b1 >= 0 ? theirs[b1] : 0;
+        }
         int all;
         const int above = block_scan(h0 + h1, warp_sums, &all);
         if (above < need && above + h0 >= need) {
@@ -958,27 +1035,66 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a) {
         need -= sh_above;
         __syncthreads();
     }
-    // all above the threshold `prefix`, and the first `need` equal to it
-    int done = 0, ties = 0;
-    for (int i0 = 0; i0 < old && done < places; i0 += kSelectThreads) {
-        const int i = i0 + tid;
-        const uint32_t key = i < old ? order_key(w[i]) : 0u;
-        const bool more = i < old && key > prefix, tie = i < old && key == prefix;
-        int all;
-        const int before = block_scan((more ? 1 : 0) | (tie ? 0x10000 : 0), warp_sums, &all);
-        const int tie_at = ties + (before >> 16);
-        if (more || (tie && tie_at < need)) kept[done + (before & 0xffff) + min(tie_at, need) - min(ties, need)] = i;
-        const int now = ties + (all >> 16);
-        done += (all & 0xffff) + min(now, need) - min(ties, need);
-        ties = now;
+    // all above the threshold `prefix`, and the first `need` equal to it: what the parts before this one have of each
+    {
+        int more = 0, ties = 0;
+        for (int i0 = begin; i0 < end; i0 += 4 * kSelectThreads) {
+            uint32_t key[4];
+            const int i = i0 + tid * 4;
+            four_keys(w, i, end, vec, key);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                more += i + k < end && key[k] > prefix;
+                ties += i + k < end && key[k] == prefix;
+            }
+        }
+        more = __reduce_add_sync(0xffffffffu, more);
+        ties = __reduce_add_sync(0xffffffffu, ties);
+        if ((tid & 31) == 0) {
+            atomicAdd(&counts[0], more);
+            atomicAdd(&counts[1], ties);
+        }
     }
+    cluster.sync();
+    int more = 0, ties = 0;
+    for (int c = 0; c < rank; ++c) {
+        const int* const theirs = cluster.map_shared_rank(counts, c);
+        more += theirs[0];
+        ties += theirs[1];
+    }
+    for (int i0 = begin; i0 < end; i0 += 4 * kSelectThreads) {
+        uint32_t key[4];
+        const int i = i0 + tid * 4;
+        four_keys(w, i, end, vec, key);
+        int here = 0;  // above the threshold in the low half, equal in the high half: 4096 at most each
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (i + k < end) here += (key[k] > prefix ? 1 : 0) + (key[k] == prefix ? 0x10000 : 0);
+        int all;
+        const int before = block_scan(here, warp_sums, &all);
+        int m = more + (before & 0xffff), t = ties + (before >> 16);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            if (i + k >= end || key[k] < prefix) continue;
+            if (key[k] > prefix) {
+                kept[m + min(t, need)] = i + k;
+                ++m;
+            } else {
+                if (t < need) kept[m + t] = i + k;
+                ++t;
+            }
+        }
+        more += all & 0xffff;
+        ties += all >> 16;
+    }
+    cluster.sync();  // this CTA's counts may be read until here
 }
 
 // One block of dst (keys or values) per CTA: the kept tokens' values, their largest, the new scale, the codes.
 template <bool E4M3, int VPT>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_gather(KvEvictArgs a) {
     const int tid = threadIdx.x;
-    int64_t b = blockIdx.x;
+    unsigned b = blockIdx.x;
     const int i = static_cast<int>(b % a.spans);
     b /= a.spans;
     const int kv = static_cast<int>(b & 1);
@@ -994,53 +1110,59 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_gather(KvEvictArgs a) {
             tid < live ? a.weights[head * a.src_cap + kept[tid]] : 0.0f;
     }
     if (live <= 0) return;
-    const int cpr = a.head_dim >> 4;
+    const int cpr = a.head_dim >> 3;
     const uint8_t* const src = a.src[kv] + head * a.src_cap * a.head_dim;
     const float* const src_scale = a.src_scale[kv] + head * (a.src_cap >> a.block_shift);
-    uint4 x[VPT];
+    __shared__ int from[128];
+    __shared__ float from_scale[128];
+    if (tid < live) {
+        const int t = kept[tid];
+        from[tid] = t;
+        from_scale[tid] = src_scale[t >> a.block_shift];
+    }
+    __syncthreads();
+    uint2 x[VPT];
     float sc[VPT];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v) {
+        const int idx = v * kAppendThreads + tid, t = idx / cpr;
+        x[v] = make_uint2(0, 0);
+        sc[v] = 0.0f;
+        if (t < live) {
+            sc[v] = from_scale[t];
+            x[v] = __ldg(reinterpret_cast<const uint2*>(src + static_cast<size_t>(from[t]) * a.head_dim) + (idx - t * cpr));
+        }
+    }
     uint32_t most = 0;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-        const int idx = v * kAppendThreads + tid;
-        x[v] = make_uint4(0, 0, 0, 0);
-        sc[v] = 0.0f;
-        if (idx < live * cpr) {
-            const int t = idx / cpr;
-            const int from = kept[t];
-            x[v] = reinterpret_cast<const uint4*>(src + static_cast<size_t>(from) * a.head_dim)[idx - t * cpr];
-            sc[v] = src_scale[from >> a.block_shift];
-            const uint32_t q[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
+        float f[8], m = 0.0f;
+        decode4<E4M3>(x[v].x, f);
+        decode4<E4M3>(x[v].y, f + 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float f[4];
-                decode4<E4M3>(q[j], f);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) most = max(most, __float_as_uint(f[k] * sc[v]) & 0x7fffffffu);
-            }
-        }
+        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
+        most = max(most, __float_as_uint(m * sc[v]));  // not negative; a NaN scale gives the largest pattern
     }
     __shared__ uint32_t part[kAppendThreads / 32];
-    most = __reduce_max_sync(0xffffffffu, most);
+    most = __reduce_max_sync(0xffffffffu, most & 0x7fffffffu);
     if ((tid & 31) == 0) part[tid >> 5] = most;
     __syncthreads();
 #pragma unroll
     for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, part[w]);
     const float s = most >= 0x7f800000u ? kNan : scale_of<E4M3>(__uint_as_float(most));
     if (tid == 0) a.dst_scale[kv][head * (a.dst_cap >> a.block_shift) + i] = s;
-    uint4* const dst = reinterpret_cast<uint4*>(a.dst[kv] + (head * a.dst_cap + slot) * a.head_dim);
+    const float r = reciprocal(s);
+    uint2* const dst = reinterpret_cast<uint2*>(a.dst[kv] + (head * a.dst_cap + slot) * a.head_dim);
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
         const int idx = v * kAppendThreads + tid;
         if (idx < block * cpr) {
-            uint32_t q[4] = {x[v].x, x[v].y, x[v].z, x[v].w};
+            float f[8];
+            decode4<E4M3>(x[v].x, f);
+            decode4<E4M3>(x[v].y, f + 4);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                float f[4];
-                decode4<E4M3>(q[j], f);
-                q[j] = encode4<E4M3>(f[0] * sc[v], f[1] * sc[v], f[2] * sc[v], f[3] * sc[v], s);
-            }
-            dst[idx] = make_uint4(q[0], q[1], q[2], q[3]);
+            for (int k = 0; k < 8; ++k) f[k] *= sc[v];
+            dst[idx] = make_uint2(encode4<E4M3>(f, s, r), encode4<E4M3>(f + 4, s, r));
         }
     }
 }
@@ -1097,11 +1219,12 @@ int grid_of(int64_t ctas, const char* what, unsigned* grid) {
 // f(constant) for the number of vectors a thread of a block kernel holds.
 template <typename F>
 void with_vpt(int64_t block, int64_t head_dim, F f) {
-    const int64_t vectors = block * head_dim / 16;
+    const int64_t vectors = block * head_dim / 8;
     if (vectors <= kAppendThreads) f(std::integral_constant<int, 1>{});
     else if (vectors <= 2 * kAppendThreads) f(std::integral_constant<int, 2>{});
     else if (vectors <= 4 * kAppendThreads) f(std::integral_constant<int, 4>{});
-    else f(std::integral_constant<int, 8>{});
+    else if (vectors <= 8 * kAppendThreads) f(std::integral_constant<int, 8>{});
+    else f(std::integral_constant<int, 16>{});
 }
 
 // f(constant) for the padded head size of the attention kernels.
@@ -1192,7 +1315,7 @@ int launch_few_rows(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p,
     if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
     const int row_tiles = static_cast<int>(p.row_tiles);
     unsigned grid = 0;
-    int st = grid_of((static_cast<int64_t>(a.batch) * a.kv_heads * row_tiles * S::kRows + 3) / 4, "dt_kv_attention", &grid);
+    int st = grid_of(static_cast<int64_t>(a.batch) * a.kv_heads * row_tiles * S::kRows, "dt_kv_attention", &grid);
     if (st != DT_OK) return st;
     kernel<<<p.grid, kAttnThreads, S::kSmem, stream>>>(a, w, row_tiles);
     st = check_launch("dt_kv_attention");
@@ -1299,8 +1422,10 @@ int dt_kv_read(const dt_kv_cache* cache, const int32_t* lengths, const int32_t* 
     a.head_dim = static_cast<int>(cache->head_dim);
     a.block_shift = log2_of(cache->block);
     a.dtype = dtype;
-    a.vectors = cache->batch * cache->kv_heads * count * (cache->head_dim / 16);
-    const dim3 grid(static_cast<unsigned>(std::min<int64_t>((a.vectors + 255) / 256, 148 * 64)), 2);
+    a.all_heads = cache->batch * cache->kv_heads;
+    const int64_t rows = 256 / (cache->head_dim / 8) * kReadRows;
+    const dim3 grid(static_cast<unsigned>((count + rows - 1) / rows), 2,
+                    static_cast<unsigned>(std::min<int64_t>(a.all_heads, 65535)));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (cache->code == DT_KV_E4M3) k_kv_read<true><<<grid, 256, 0, s>>>(a);
     else k_kv_read<false><<<grid, 256, 0, s>>>(a);
@@ -1466,7 +1591,21 @@ int dt_kv_evict(const dt_kv_cache* src, const dt_kv_cache* dst, const int32_t* l
     unsigned grid = 0;
     st = grid_of(static_cast<int64_t>(heads) * 2 * a.spans, "dt_kv_evict", &grid);
     if (st != DT_OK) return st;
-    k_kv_select<<<static_cast<unsigned>(heads), kSelectThreads, 0, s>>>(a);
+    // CTAs for a head: one for each 16384 tokens that it can hold, 8 at most (16 keys a thread and pass)
+    unsigned ctas = 1;
+    while (ctas < 8 && src->capacity > static_cast<int64_t>(ctas) * 16384) ctas *= 2;
+    cudaLaunchAttribute attr{};
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = ctas;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>(heads) * ctas);
+    cfg.blockDim = dim3(kSelectThreads);
+    cfg.stream = s;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_kv_select, a, aligned16(weights));
+    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_evict: ") + cudaGetErrorString(e));
     st = check_launch("dt_kv_evict");
     if (st != DT_OK) return st;
     if (grid > 0) {
