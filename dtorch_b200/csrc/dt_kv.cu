@@ -38,26 +38,34 @@ __device__ __forceinline__ float scale_of(float amax) {
 //   e4m3: half way points have 5 significant bits and others differ by 2^-13 of themselves; rounding to 18 bits restores them.
 // Scales below 2^-100, whose reciprocals may not be normal, take the division.
 template <bool E4M3>
-__device__ __forceinline__ uint32_t encode4(const float* x, float s, float r) {
-    if (!(s > 0.0f)) return 0;  // 0: the block is all zero; NaN: the block is marked
-    const bool divide = s < 0x1p-100f;
-    float y[4];
+__device__ __forceinline__ uint32_t pack_codes(const float* y) {
     if constexpr (E4M3) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            y[i] = divide ? x[i] / s : __uint_as_float((__float_as_uint(x[i] * r) + 0x20u) & ~0x3fu);
         const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(y[0], y[1]), __NV_SATFINITE, __NV_E4M3);
         const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(y[2], y[3]), __NV_SATFINITE, __NV_E4M3);
         return lo | (hi << 16);
     } else {
-        uint32_t q[4];
+        uint32_t q[4];  // 1.5 * 2^23 more: the integer, ties to even, in the low byte
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            y[i] = divide ? x[i] / s : copysignf(fmaf(fabsf(x[i]), r, 128.0f) - 128.0f, x[i]);
-            q[i] = __float_as_uint(y[i] + 12582912.0f);  // 1.5 * 2^23: the integer, ties to even, in the low byte
-        }
+        for (int i = 0; i < 4; ++i) q[i] = __float_as_uint(y[i] + 12582912.0f);
         return prmt(prmt(q[0], q[1], 0x0040), prmt(q[2], q[3], 0x0040), 0x5410);
     }
+}
+
+template <bool E4M3>
+__device__ __noinline__ uint32_t encode4_divided(float a, float b, float c, float d, float s) {
+    const float y[4] = {a / s, b / s, c / s, d / s};
+    return pack_codes<E4M3>(y);
+}
+
+template <bool E4M3>
+__device__ __forceinline__ uint32_t encode4(const float* x, float s, float r) {
+    if (!(s >= 0x1p-100f)) return s > 0.0f ? encode4_divided<E4M3>(x[0], x[1], x[2], x[3], s) : 0;  // 0: all zero; NaN: marked
+    float y[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+        y[i] = E4M3 ? __uint_as_float((__float_as_uint(x[i] * r) + 0x20u) & ~0x3fu)
+                    : copysignf(fmaf(fabsf(x[i]), r, 128.0f) - 128.0f, x[i]);
+    return pack_codes<E4M3>(y);
 }
 
 __device__ __forceinline__ float reciprocal(float s) { return s >= 0x1p-100f ? 1.0f / s : 0.0f; }
@@ -957,6 +965,11 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a, boo
     __shared__ int counts[2];  // of this CTA's tokens: above the threshold, and equal to it
     __shared__ uint32_t sh_digit;
     __shared__ int sh_above;
+    // one CTA needs no barrier of the cluster
+    const auto cluster_sync = [&] {
+        if (ctas > 1) cluster.sync();
+        else __syncthreads();
+    };
     const int tid = threadIdx.x;
     const size_t head = blockIdx.x / ctas;
     const int n = static_cast<int>(head / a.heads);
@@ -992,7 +1005,8 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a, boo
 #pragma unroll
             for (int u = 0; u < 4; ++u) four_keys(w, i0 + (u * kSelectThreads + tid) * 4, end, vec, key[u]);
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
+            for (int u = 0; u < 4; ++u) {
+                if (i0 + u * 4 * kSelectThreads >= end) break;
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const bool in = i0 + (u * kSelectThreads + tid) * 4 + k < end && (key[u][k] & mask) == prefix;
@@ -1008,8 +1022,9 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a, boo
                         atomicAdd(&mine[digit], 1);
                     }
                 }
+            }
         }
-        cluster.sync();
+        cluster_sync();
         // the other histogram was last read before this barrier
         for (int i = tid; i < 2048; i += kSelectThreads) hist[(pass + 1) & 1][i] = 0;
         // the digit at which the count from above reaches the places that are left; two bins a thread, from the top
@@ -1055,7 +1070,7 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a, boo
             atomicAdd(&counts[1], ties);
         }
     }
-    cluster.sync();
+    cluster_sync();
     int more = 0, ties = 0;
     for (int c = 0; c < rank; ++c) {
         const int* const theirs = cluster.map_shared_rank(counts, c);
@@ -1087,82 +1102,90 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a, boo
         more += all & 0xffff;
         ties += all >> 16;
     }
-    cluster.sync();  // this CTA's counts may be read until here
+    cluster_sync();  // this CTA's counts may be read until here
 }
 
-// One block of dst (keys or values) per CTA: the kept tokens' values, their largest, the new scale, the codes.
-template <bool E4M3, int VPT>
+// One block of dst, keys and values, per CTA: the kept tokens' codes come to shared memory with cp.async, all of them in
+// flight together (what bounds this kernel is how many bytes an SM has under way: codes in registers, keys and values in
+// CTAs of their own took 64 us where this takes the time of the commit that brought it); then the largest value of each,
+// the new scale, the codes.
+template <bool E4M3>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_gather(KvEvictArgs a) {
+    extern __shared__ __align__(16) uint8_t codes[];  // keys, then values: block * head_dim each
     const int tid = threadIdx.x;
-    unsigned b = blockIdx.x;
-    const int i = static_cast<int>(b % a.spans);
-    b /= a.spans;
-    const int kv = static_cast<int>(b & 1);
-    const size_t head = static_cast<size_t>(b >> 1);
+    const int i = static_cast<int>(blockIdx.x % a.spans);
+    const size_t head = blockIdx.x / a.spans;
     const int n = static_cast<int>(head / a.heads);
     const int count = min(kv_length(a.lengths, n, a.src_cap), a.budget);
     const int block = 1 << a.block_shift;
     const int slot = i << a.block_shift;
     const int live = min(block, count - slot);
     const int32_t* const kept = a.kept + head * a.budget + slot;
-    if (kv == 0 && a.dst_weights != nullptr && tid < block) {
-        a.dst_weights[head * a.dst_cap + slot + tid] =
-            tid < live ? a.weights[head * a.src_cap + kept[tid]] : 0.0f;
-    }
-    if (live <= 0) return;
-    const int cpr = a.head_dim >> 3;
-    const uint8_t* const src = a.src[kv] + head * a.src_cap * a.head_dim;
-    const float* const src_scale = a.src_scale[kv] + head * (a.src_cap >> a.block_shift);
     __shared__ int from[128];
-    __shared__ float from_scale[128];
-    if (tid < live) {
-        const int t = kept[tid];
-        from[tid] = t;
-        from_scale[tid] = src_scale[t >> a.block_shift];
-    }
+    __shared__ float from_scale[2][128];
+    if (tid < live) from[tid] = kept[tid];
     __syncthreads();
-    uint2 x[VPT];
-    float sc[VPT];
+    if (a.dst_weights != nullptr && tid < block)
+        a.dst_weights[head * a.dst_cap + slot + tid] = tid < live ? a.weights[head * a.src_cap + from[tid]] : 0.0f;
+    if (live <= 0) return;
+    const int chunks = a.head_dim >> 4, vectors = a.head_dim >> 3, bytes = block * a.head_dim;
+    // idx / vectors for idx < 2^12, vectors <= 32: the rounded reciprocal is off by less than 2^-8 of a row
+    const uint32_t row_of = ((1u << 20) + vectors - 1) / vectors;
+    for (int idx = tid; idx < live * chunks; idx += kAppendThreads) {
+        const int t = idx / chunks, c = idx - t * chunks;
+        const size_t at = (head * a.src_cap + from[t]) * a.head_dim + c * 16;
+        const uint32_t to = static_cast<uint32_t>(__cvta_generic_to_shared(codes)) + idx * 16;
+        cp_async16(to, a.src[0] + at, true);
+        cp_async16(to + bytes, a.src[1] + at, true);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    if (tid < 2 * live) {
+        const int kv = tid & 1, t = tid >> 1;
+        from_scale[kv][t] = a.src_scale[kv][head * (a.src_cap >> a.block_shift) + (from[t] >> a.block_shift)];
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncthreads();
+    __shared__ uint32_t part[2][kAppendThreads / 32];
+#pragma unroll 1
+    for (int kv = 0; kv < 2; ++kv) {
+        const uint2* const src = reinterpret_cast<const uint2*>(codes + kv * bytes);
+        uint32_t most = 0;
+        for (int idx = tid; idx < live * vectors; idx += kAppendThreads) {
+            const uint2 x = src[idx];
+            float f[8], m = 0.0f;
+            decode4<E4M3>(x.x, f);
+            decode4<E4M3>(x.y, f + 4);
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-        const int idx = v * kAppendThreads + tid, t = idx / cpr;
-        x[v] = make_uint2(0, 0);
-        sc[v] = 0.0f;
-        if (t < live) {
-            sc[v] = from_scale[t];
-            x[v] = __ldg(reinterpret_cast<const uint2*>(src + static_cast<size_t>(from[t]) * a.head_dim) + (idx - t * cpr));
+            for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
+            most = max(most, __float_as_uint(m * from_scale[kv][idx * row_of >> 20]) & 0x7fffffffu);  // NaN: the largest pattern
         }
+        most = __reduce_max_sync(0xffffffffu, most);
+        if ((tid & 31) == 0) part[kv][tid >> 5] = most;
     }
-    uint32_t most = 0;
-#pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-        float f[8], m = 0.0f;
-        decode4<E4M3>(x[v].x, f);
-        decode4<E4M3>(x[v].y, f + 4);
-#pragma unroll
-        for (int k = 0; k < 8; ++k) m = fmaxf(m, fabsf(f[k]));
-        most = max(most, __float_as_uint(m * sc[v]));  // not negative; a NaN scale gives the largest pattern
-    }
-    __shared__ uint32_t part[kAppendThreads / 32];
-    most = __reduce_max_sync(0xffffffffu, most & 0x7fffffffu);
-    if ((tid & 31) == 0) part[tid >> 5] = most;
     __syncthreads();
+#pragma unroll 1
+    for (int kv = 0; kv < 2; ++kv) {
+        uint32_t most = 0;
 #pragma unroll
-    for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, part[w]);
-    const float s = most >= 0x7f800000u ? kNan : scale_of<E4M3>(__uint_as_float(most));
-    if (tid == 0) a.dst_scale[kv][head * (a.dst_cap >> a.block_shift) + i] = s;
-    const float r = reciprocal(s);
-    uint2* const dst = reinterpret_cast<uint2*>(a.dst[kv] + (head * a.dst_cap + slot) * a.head_dim);
+        for (int w = 0; w < kAppendThreads / 32; ++w) most = max(most, part[kv][w]);
+        const float s = most >= 0x7f800000u ? kNan : scale_of<E4M3>(__uint_as_float(most));
+        if (tid == 0) a.dst_scale[kv][head * (a.dst_cap >> a.block_shift) + i] = s;
+        const float r = reciprocal(s);
+        const uint2* const src = reinterpret_cast<const uint2*>(codes + kv * bytes);
+        uint2* const dst = reinterpret_cast<uint2*>(a.dst[kv] + (head * a.dst_cap + slot) * a.head_dim);
+        for (int idx = tid; idx < block * vectors; idx += kAppendThreads) {
+            uint2 q = make_uint2(0, 0);
+            if (idx < live * vectors) {
+                const uint2 x = src[idx];
+                const float sc = from_scale[kv][idx * row_of >> 20];
+                float f[8];
+                decode4<E4M3>(x.x, f);
+                decode4<E4M3>(x.y, f + 4);
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) {
-        const int idx = v * kAppendThreads + tid;
-        if (idx < block * cpr) {
-            float f[8];
-            decode4<E4M3>(x[v].x, f);
-            decode4<E4M3>(x[v].y, f + 4);
-#pragma unroll
-            for (int k = 0; k < 8; ++k) f[k] *= sc[v];
-            dst[idx] = make_uint2(encode4<E4M3>(f, s, r), encode4<E4M3>(f + 4, s, r));
+                for (int k = 0; k < 8; ++k) f[k] *= sc;
+                q = make_uint2(encode4<E4M3>(f, s, r), encode4<E4M3>(f + 4, s, r));
+            }
+            dst[idx] = q;
         }
     }
 }
@@ -1589,7 +1612,7 @@ int dt_kv_evict(const dt_kv_cache* src, const dt_kv_cache* dst, const int32_t* l
     a.spans = static_cast<int>((budget + src->block - 1) / src->block);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     unsigned grid = 0;
-    st = grid_of(static_cast<int64_t>(heads) * 2 * a.spans, "dt_kv_evict", &grid);
+    st = grid_of(static_cast<int64_t>(heads) * a.spans, "dt_kv_evict", &grid);
     if (st != DT_OK) return st;
     // CTAs for a head: one for each 16384 tokens that it can hold, 8 at most (16 keys a thread and pass)
     unsigned ctas = 1;
@@ -1609,11 +1632,11 @@ int dt_kv_evict(const dt_kv_cache* src, const dt_kv_cache* dst, const int32_t* l
     st = check_launch("dt_kv_evict");
     if (st != DT_OK) return st;
     if (grid > 0) {
-        with_vpt(src->block, src->head_dim, [&](auto vpt) {
-            constexpr int V = decltype(vpt)::value;
-            if (src->code == DT_KV_E4M3) k_kv_gather<true, V><<<grid, kAppendThreads, 0, s>>>(a);
-            else k_kv_gather<false, V><<<grid, kAppendThreads, 0, s>>>(a);
-        });
+        const int smem = static_cast<int>(2 * src->block * src->head_dim);
+        const auto kernel = src->code == DT_KV_E4M3 ? k_kv_gather<true> : k_kv_gather<false>;
+        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+        if (err != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_evict: ") + cudaGetErrorString(err));
+        kernel<<<grid, kAppendThreads, smem, s>>>(a);
         st = check_launch("dt_kv_evict");
         if (st != DT_OK) return st;
     }

@@ -30,7 +30,7 @@ namespace {
 // A softmax row keeps a reference instead of its exact maximum: it moves (and O is scaled, in TMEM) only when the
 // maximum has grown by more than 2^3, so weights stay below 2^3 and the scaling is rare. Block scales: a key scale is
 // constant over 32 columns and goes into the row's factor; a value scale, relative to a power of two above all of the
-// sequence's, into the weight before it is rounded to fp16 (11 bits; 2^kPromptShift keeps values down to 2^-29 of the
+// sequence's, into the weight before it is rounded to fp16 (11 bits; 2^kPromptShift keeps values down to 2^-26 of the
 // largest normal).
 constexpr int kRowTile = 128;
 constexpr int kTokTile = 128;
