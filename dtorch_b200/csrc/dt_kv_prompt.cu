@@ -400,7 +400,8 @@ __device__ __forceinline__ int key_tile_rows(const KvAttnArgs& a, int kt, int le
 
 // Lays out a list, in one block: of (sequence, head, 256 rows) items and their key tiles, or (COLUMNS) of (sequence,
 // head, 128 keys) items and their row tiles. prefix[n][i]: cost of a head's items before item i of sequence n, and of
-// all of them at prefix[n][items]; base[n]: that of the sequences before n.
+// all of them at prefix[n][items]; base[n]: that of the sequences before n. Items behind a sequence's length have no
+// entries: the last entry before them, at the count of those within, is that of all.
 template <bool COLUMNS>
 __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptList* list, PromptStart* starts,
                                                          int64_t* prefix, int64_t* base, int row_tiles, int ctas) {
@@ -409,9 +410,10 @@ __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptLis
         const int len = kv_length(a.lengths, n, a.capacity), cnt = kv_count(a.counts, n, a.tokens);
         int64_t* const out = prefix + static_cast<int64_t>(n) * (row_tiles + 1);
         int64_t done = 0;
-        for (int r0 = 0; r0 < row_tiles; r0 += 32) {
+        const int used = COLUMNS ? min((len + kTokTile - 1) / kTokTile, row_tiles) : row_tiles;
+        for (int r0 = 0; r0 < used; r0 += 32) {
             const int rt = r0 + lane;
-            const int tiles = rt >= row_tiles ? 0 : COLUMNS ? key_tile_rows(a, rt, len, cnt) : item_tiles(a, rt, len, cnt);
+            const int tiles = rt >= used ? 0 : COLUMNS ? key_tile_rows(a, rt, len, cnt) : item_tiles(a, rt, len, cnt);
             const int64_t mine = tiles > 0 ? tiles + kItemCost : 0;
             int64_t incl = mine;
 #pragma unroll
@@ -419,10 +421,10 @@ __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptLis
                 const int64_t o = __shfl_up_sync(0xffffffffu, incl, d);
                 if (lane >= d) incl += o;
             }
-            if (rt < row_tiles) out[rt] = done + incl - mine;
+            if (rt < used) out[rt] = done + incl - mine;
             done += __shfl_sync(0xffffffffu, incl, 31);
         }
-        if (lane == 0) out[row_tiles] = done;
+        if (lane == 0) out[used] = out[row_tiles] = done;
     }
     __syncthreads();
     if (warp == 0) {
@@ -464,7 +466,8 @@ __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptLis
         const int64_t* const p = prefix + static_cast<int64_t>(s.n) * (row_tiles + 1);
         s.h = static_cast<int>(quotient(x, p[row_tiles]));
         x -= s.h * p[row_tiles];
-        s.rt = find(p, row_tiles, x);
+        const int len = kv_length(a.lengths, s.n, a.capacity);
+        s.rt = find(p, COLUMNS ? min((len + kTokTile - 1) / kTokTile, row_tiles) : row_tiles, x);
         const int at = static_cast<int>(x - p[s.rt]);
         s.tile = max(at - kItemCost, 0);
         s.lead = max(kItemCost - at, 0);

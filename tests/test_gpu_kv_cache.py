@@ -328,6 +328,38 @@ def test_attention_in_long_caches_and_ragged_batches():
             assert not w[i, :, l:].any()
 
 
+@pytest.mark.parametrize("n,h,g,t,lo,hi,cap,e", [
+    (40, 3, 4, 9, 1, 40, 64, 64),        # many items of one tile, rows in one of the two row tiles
+    (24, 4, 2, 100, 90, 700, 65536, 128),  # short sequences in a large cache, rows in both
+    (3, 1, 1, 129, 0, 1000, 1024, 96), (1, 2, 3, 400, 399, 399, 512, 128), (70, 1, 4, 33, 0, 3, 128, 32)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_many_items_for_a_cta(n, h, g, t, lo, hi, cap, e, causal):
+    # oracle on the GPU, in 64 bits
+    gen = torch.Generator().manual_seed(n + t)
+    lengths = [lo + (hi - lo) * (i * 7 % n) // max(n - 1, 1) for i in range(n)]
+    cache = dt.QuantizedKVCache(n, h, cap, e, dtype=E4M3, block=32)
+    k, v = (torch.randn((n, h, max(lengths), e), generator=gen).to(BF16).cuda() for _ in range(2))
+    dt.kv_cache_append(cache, k, v, ints([0] * n), counts=ints(lengths))
+    kk, vv = (x.double() for x in dt.kv_cache_read(cache, ints(lengths), count=max(lengths), dtype=torch.float32))
+    q = torch.randn((n, h * g, t, e), generator=gen).to(FP16).cuda()
+    w = torch.full((n, h, cap), 7.0, device="cuda")
+    out = dt.kv_cache_attention(q, cache, ints(lengths), is_causal=causal, weights=w, accumulate=False)
+    pos = torch.arange(max(lengths), device="cuda")
+    s = torch.einsum("nhgte,nhle->nhgtl", q.double().view(n, h, g, t, e), kk) / math.sqrt(e)
+    lim = ints(lengths)[:, None] - (t - 1 - torch.arange(t, device="cuda") if causal else 0 * torch.arange(t, device="cuda"))
+    s = s.masked_fill((pos >= lim[..., None])[:, None, None], -math.inf)
+    p = torch.softmax(s, -1).nan_to_num()
+    want = torch.einsum("nhgtl,nhle->nhgte", p, vv).reshape(out.shape)
+    mag = torch.einsum("nhgtl,nhle->nhgte", p, vv.abs()).reshape(out.shape)
+    size = torch.full(out.shape[:3], 25.0, device="cuda", dtype=torch.float64)  # scale * sum |q k| is 4 to 8, and spreads
+    assert ((out.double() - want).abs() <= ko.attention_bounds(want, mag, size, FP16)).all()
+    ew = p.sum(dim=(2, 3))
+    for i, l in enumerate(lengths):
+        off = (w[i, :, :l].double() - ew[i, :, :l]).abs() - (2.0 ** -18 + 2 * 25 * 2.0 ** -19) * ew[i, :, :l]
+        assert l == 0 or off.max() <= g * t * 2.0 ** -126
+        assert (w[i, :, l:] == 7.0).all()
+
+
 def test_offsets_beyond_32_bits():
     # two heads of 2^24 + 64 tokens of 128 elements: the second head's codes begin behind 2^31 bytes
     cap, e = (1 << 24) + 64, 128
