@@ -468,15 +468,29 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
             if (it < nt && tok < len) {
                 const uint32_t ks_s = stages_s + st * S::kStageBytes, vs_s = ks_s + S::kSliceBytes;
                 const size_t off = static_cast<size_t>(tok) * a.head_dim;
-                // rows a lane copies are 32 / kChunks apart, columns the same: one address and one swizzle a lane where
-                // that is the swizzle's period
+                if (a.head_dim == EP && tok + kWarpTokens <= len) {
+                    // a whole slice is one piece of memory; a lane's rows are 32 / kChunks apart, which changes known bits
+                    // of the permutation
+                    constexpr int kStep = 32 / S::kChunks;
+                    const int own = swizzled<EP>(lane / S::kChunks, lane % S::kChunks);
+                    const uint8_t* const kp = kbase + off + lane * 16;
+                    const uint8_t* const vp = vbase + off + lane * 16;
 #pragma unroll
-                for (int j = 0; j < S::kChunks; ++j) {
-                    const int idx = j * 32 + lane, r = idx / S::kChunks, c = idx % S::kChunks;
-                    const bool live = tok + r < len && c * 16 < a.head_dim;
-                    const size_t o = live ? off + static_cast<size_t>(r) * a.head_dim + c * 16 : off;
-                    cp_async16(ks_s + swizzled<EP>(r, c), kbase + o, live);
-                    cp_async16(vs_s + swizzled<EP>(r, c), vbase + o, live);
+                    for (int j = 0; j < S::kChunks; ++j) {
+                        const int flip = swizzled<EP>(j * kStep, 0) - j * kStep * EP;
+                        const uint32_t to = (own ^ flip) + j * kStep * EP;
+                        cp_async16(ks_s + to, kp + j * 512, true);
+                        cp_async16(vs_s + to, vp + j * 512, true);
+                    }
+                } else {
+#pragma unroll 1
+                    for (int j = 0; j < S::kChunks; ++j) {
+                        const int idx = j * 32 + lane, r = idx / S::kChunks, c = idx % S::kChunks;
+                        const bool live = tok + r < len && c * 16 < a.head_dim;
+                        const size_t o = live ? off + static_cast<size_t>(r) * a.head_dim + c * 16 : off;
+                        cp_async16(ks_s + swizzled<EP>(r, c), kbase + o, live);
+                        cp_async16(vs_s + swizzled<EP>(r, c), vbase + o, live);
+                    }
                 }
                 if (lane < 2) {
                     const int b = tok >> a.block_shift;
