@@ -106,6 +106,7 @@ constexpr int kAppendThreads = 256;
 // 101 MB in and out, 30 us, 3.4 TB/s; one token of 32 sequences 5 us.
 template <bool E4M3, int VPT>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_append(KvAppendArgs a) {
+    enter_kernel();
     const int tid = threadIdx.x;
     unsigned b = blockIdx.x;
     const int i = static_cast<int>(b % a.spans);
@@ -216,6 +217,7 @@ constexpr int kReadRows = 4;
 
 template <bool E4M3>
 __global__ void __launch_bounds__(256) k_kv_read(KvReadArgs a) {
+    enter_kernel();
     const int kv = blockIdx.y;
     if (a.out[kv] == nullptr) return;
     const int cpr = a.head_dim >> 3, step = 256 / cpr;
@@ -433,10 +435,9 @@ __device__ __forceinline__ TilePos find_tile(const KvAttnArgs& a, int per_seq, i
 
 template <bool E4M3, int EP, int NT>
 __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_attend(KvAttnArgs a, KvPartials w, int row_tiles) {
+    enter_kernel();
     using S = AttnShape<EP, NT>;
     extern __shared__ __align__(128) uint8_t smem[];
-    // what follows may be launched already: it waits for this grid's end before it reads
-    asm volatile("griddepcontrol.launch_dependents;");
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c4 = lane & 3, r4 = lane >> 2;
     uint8_t* const stages = smem + warp * S::kWarpBytes;
     float* const scales = reinterpret_cast<float*>(smem + 4 * S::kWarpBytes) + warp * S::kStages * 2;
@@ -715,8 +716,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
 // warp a row).
 template <int EP>
 __global__ void __launch_bounds__(128) k_kv_merge(KvAttnArgs a, KvPartials w, int row_tiles, int tile_rows, int grid) {
-    asm volatile("griddepcontrol.launch_dependents;");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    enter_kernel();
     __shared__ float parts_sum[4];
     __shared__ float parts_out[4][EP];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, per_seq = a.kv_heads * row_tiles;
@@ -816,7 +816,7 @@ __device__ __forceinline__ float weight_of(float score, float lse2) {
 // Weights from the stored scores: a thread sums four tokens' columns over the (at most 16) rows of a head. 8 rows of 8
 // heads and 131071 tokens (38 MB, most of it still in L2): 9 us.
 __global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w, int tile_rows) {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+    enter_kernel();
     const size_t head = blockIdx.y + static_cast<size_t>(gridDim.y) * blockIdx.z;
     const int n = static_cast<int>(head / a.kv_heads);
     if (n >= a.batch) return;
@@ -845,6 +845,7 @@ __global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w, 
 // lane's registers until the end, so there are no atomics and the order of the sum is fixed.
 template <bool E4M3, int EP>
 __global__ void __launch_bounds__(kAttnThreads) k_kv_column_sums(KvAttnArgs a, const float* __restrict__ lse2s, int key_tiles) {
+    enter_kernel();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, c4 = lane & 3, r4 = lane >> 2;
     const size_t head = blockIdx.x / key_tiles;
     const int n = static_cast<int>(head / a.kv_heads), h = static_cast<int>(head % a.kv_heads);
@@ -979,6 +980,7 @@ __device__ __forceinline__ void four_keys(const float* w, int i, int end, bool v
 // and read each other's histograms and counts. Bound by its four passes and their barriers: 8 heads of 131072 tokens 37 us
 // (238 with one CTA a head), 64 heads of up to 32768 27 us.
 __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a, bool vec) {
+    enter_kernel();
     namespace cg = cooperative_groups;
     const cg::cluster_group cluster = cg::this_cluster();
     const int ctas = static_cast<int>(cluster.num_blocks()), rank = static_cast<int>(cluster.block_rank());
@@ -1132,6 +1134,7 @@ __global__ void __launch_bounds__(kSelectThreads) k_kv_select(KvEvictArgs a, boo
 // twice and encoded once. 8 sequences cut to 4096 tokens of 8 heads (134 MB): 46 us, 2.9 TB/s; 63 with divisions.
 template <bool E4M3>
 __global__ void __launch_bounds__(kAppendThreads) k_kv_gather(KvEvictArgs a) {
+    enter_kernel();
     extern __shared__ __align__(16) uint8_t codes[];  // keys, then values: block * head_dim each
     const int tid = threadIdx.x;
     const int i = static_cast<int>(blockIdx.x % a.spans);
@@ -1213,6 +1216,7 @@ __global__ void __launch_bounds__(kAppendThreads) k_kv_gather(KvEvictArgs a) {
 
 // dst_weights behind the blocks that k_kv_gather writes.
 __global__ void __launch_bounds__(256) k_kv_zero_tail(float* w, int64_t heads, int64_t cap, int64_t from) {
+    enter_kernel();
     const int64_t tail = cap - from;
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x; i < heads * tail;
          i += static_cast<int64_t>(gridDim.x) * blockDim.x)
@@ -1333,38 +1337,17 @@ int attn_plan(const dt_kv_cache* c, int64_t query_heads, int64_t tokens, bool we
     return DT_OK;
 }
 
-// Launch behind a kernel that lets its successor start early (griddepcontrol in both).
-template <typename... P, typename... A>
-int launch_next(void (*kernel)(P...), dim3 grid, int threads, cudaStream_t stream, A... args) {
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr.val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.stream = stream;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, P(args)...);
-    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
-    return check_launch("dt_kv_attention");
-}
-
 template <bool E4M3, int EP, int NT>
 int launch_few_rows(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, cudaStream_t stream) {
     using S = AttnShape<EP, NT>;
-    // per device and cheap: the limit belongs to the kernel in the current context
-    const auto kernel = k_kv_attend<E4M3, EP, NT>;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
     const int row_tiles = static_cast<int>(p.row_tiles);
     unsigned grid = 0;
     int st = grid_of(static_cast<int64_t>(a.batch) * a.kv_heads * row_tiles * S::kRows, "dt_kv_attention", &grid);
     if (st != DT_OK) return st;
-    kernel<<<p.grid, kAttnThreads, S::kSmem, stream>>>(a, w, row_tiles);
-    st = check_launch("dt_kv_attention");
+    st = launch_kernel("dt_kv_attention", k_kv_attend<E4M3, EP, NT>, dim3(p.grid), kAttnThreads, S::kSmem, stream, 1, a, w,
+                       row_tiles);
     if (st != DT_OK) return st;
-    return launch_next(k_kv_merge<EP>, dim3(grid), 128, stream, a, w, row_tiles, S::kRows, p.grid);
+    return launch_kernel("dt_kv_attention", k_kv_merge<EP>, dim3(grid), 128, 0, stream, 1, a, w, row_tiles, S::kRows, p.grid);
 }
 
 template <bool E4M3, int EP>
@@ -1379,7 +1362,7 @@ int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, v
     if (w.scores != nullptr) {
         const unsigned y = static_cast<unsigned>(std::min<int64_t>(heads, 32768));
         const dim3 g(static_cast<unsigned>((a.capacity + 1023) / 1024), y, static_cast<unsigned>((heads + y - 1) / y));
-        return launch_next(k_kv_weights, g, 256, stream, a, w, static_cast<int>(tile_rows(p.rows)));
+        return launch_kernel("dt_kv_attention", k_kv_weights, g, 256, 0, stream, 1, a, w, static_cast<int>(tile_rows(p.rows)));
     }
     if (p.column_tiles)
         return kv_column_sums(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.columns, static_cast<char*>(workspace) + p.scores, w.lse2,
@@ -1388,8 +1371,8 @@ int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, v
     unsigned grid = 0;
     st = grid_of(heads * key_tiles, "dt_kv_attention", &grid);
     if (st != DT_OK) return st;
-    k_kv_column_sums<E4M3, 256><<<grid, kAttnThreads, 0, stream>>>(a, w.lse2, key_tiles);
-    return check_launch("dt_kv_attention");
+    return launch_kernel("dt_kv_attention", k_kv_column_sums<E4M3, 256>, dim3(grid), kAttnThreads, 0, stream, 1, a, w.lse2,
+                         key_tiles);
 }
 
 }  // namespace
@@ -1434,10 +1417,10 @@ int dt_kv_append(const dt_kv_cache* cache, const void* key, const void* value, i
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     with_vpt(cache->block, cache->head_dim, [&](auto vpt) {
         constexpr int V = decltype(vpt)::value;
-        if (cache->code == DT_KV_E4M3) k_kv_append<true, V><<<grid, kAppendThreads, 0, s>>>(a);
-        else k_kv_append<false, V><<<grid, kAppendThreads, 0, s>>>(a);
+        st = launch_kernel("dt_kv_append", cache->code == DT_KV_E4M3 ? k_kv_append<true, V> : k_kv_append<false, V>, dim3(grid),
+                           kAppendThreads, 0, s, 1, a);
     });
-    return check_launch("dt_kv_append");
+    return st;
 }
 
 int dt_kv_read(const dt_kv_cache* cache, const int32_t* lengths, const int32_t* first, int64_t first_all,
@@ -1471,9 +1454,7 @@ int dt_kv_read(const dt_kv_cache* cache, const int32_t* lengths, const int32_t* 
     const dim3 grid(static_cast<unsigned>((count + rows - 1) / rows), 2,
                     static_cast<unsigned>(std::min<int64_t>(a.all_heads, 65535)));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (cache->code == DT_KV_E4M3) k_kv_read<true><<<grid, 256, 0, s>>>(a);
-    else k_kv_read<false><<<grid, 256, 0, s>>>(a);
-    return check_launch("dt_kv_read");
+    return launch_kernel("dt_kv_read", cache->code == DT_KV_E4M3 ? k_kv_read<true> : k_kv_read<false>, grid, 256, 0, s, 1, a);
 }
 
 static int check_queries(const dt_kv_cache* cache, int64_t query_heads, int64_t tokens, const char* who) {
@@ -1638,35 +1619,19 @@ int dt_kv_evict(const dt_kv_cache* src, const dt_kv_cache* dst, const int32_t* l
     // CTAs for a head: one for each 16384 tokens that it can hold, 8 at most (16 keys a thread and pass)
     unsigned ctas = 1;
     while (ctas < 8 && src->capacity > static_cast<int64_t>(ctas) * 16384) ctas *= 2;
-    cudaLaunchAttribute attr{};
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = ctas;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = dim3(static_cast<unsigned>(heads) * ctas);
-    cfg.blockDim = dim3(kSelectThreads);
-    cfg.stream = s;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, k_kv_select, a, aligned16(weights));
-    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_evict: ") + cudaGetErrorString(e));
-    st = check_launch("dt_kv_evict");
+    st = launch_kernel("dt_kv_evict", k_kv_select, dim3(static_cast<unsigned>(heads) * ctas), kSelectThreads, 0, s, ctas, a,
+                       aligned16(weights));
     if (st != DT_OK) return st;
     if (grid > 0) {
-        const int smem = static_cast<int>(2 * src->block * src->head_dim);
-        const auto kernel = src->code == DT_KV_E4M3 ? k_kv_gather<true> : k_kv_gather<false>;
-        const cudaError_t err = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-        if (err != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_evict: ") + cudaGetErrorString(err));
-        kernel<<<grid, kAppendThreads, smem, s>>>(a);
-        st = check_launch("dt_kv_evict");
+        st = launch_kernel("dt_kv_evict", src->code == DT_KV_E4M3 ? k_kv_gather<true> : k_kv_gather<false>, dim3(grid),
+                           kAppendThreads, static_cast<size_t>(2 * src->block * src->head_dim), s, 1, a);
         if (st != DT_OK) return st;
     }
     const int64_t written = static_cast<int64_t>(a.spans) * src->block;
     if (dst_weights != nullptr && written < dst->capacity) {
         const int64_t tail = static_cast<int64_t>(heads) * (dst->capacity - written);
-        k_kv_zero_tail<<<static_cast<unsigned>(std::min<int64_t>((tail + 255) / 256, 148 * 16)), 256, 0, s>>>(
-            dst_weights, static_cast<int64_t>(heads), dst->capacity, written);
-        st = check_launch("dt_kv_evict");
+        st = launch_kernel("dt_kv_evict", k_kv_zero_tail, dim3(static_cast<unsigned>(std::min<int64_t>((tail + 255) / 256, 148 * 16))),
+                           256, 0, s, 1, dst_weights, static_cast<int64_t>(heads), dst->capacity, written);
     }
     return st;
 }

@@ -409,6 +409,7 @@ __device__ __forceinline__ int key_tile_rows(const KvAttnArgs& a, int kt, int le
 template <bool COLUMNS>
 __global__ void __launch_bounds__(1024) k_kv_prompt_plan(KvAttnArgs a, PromptList* list, PromptStart* starts,
                                                          int64_t* prefix, int64_t* base, int row_tiles, int ctas) {
+    enter_kernel();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     for (int n = warp; n < a.batch; n += 32) {
         const int len = kv_length(a.lengths, n, a.capacity), cnt = kv_count(a.counts, n, a.tokens);
@@ -519,6 +520,7 @@ struct PromptItem {
 
 template <bool E4M3, int EP>
 __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, PromptParts w, int row_tiles) {
+    enter_kernel();
     using S = PromptShape<EP>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_addr(smem);
@@ -913,6 +915,7 @@ constexpr int kMergeRows = 64;
 // stretches and 64 of an item's 256 rows, four threads a row. The item's first boundary does the work.
 template <int EP>
 __global__ void __launch_bounds__(256) k_kv_prompt_merge(KvAttnArgs a, PromptParts w, int row_tiles) {
+    enter_kernel();
     const PromptList list = *w.list;
     if (list.each * (blockIdx.x + 1) >= list.total) return;
     const PromptItem pos(w, row_tiles, w.starts[blockIdx.x + 1]);
@@ -974,23 +977,19 @@ __global__ void __launch_bounds__(256) k_kv_prompt_merge(KvAttnArgs a, PromptPar
 template <bool E4M3, int EP>
 int launch(const KvAttnArgs& a, const KvPromptPlan& p, char* ws, float* lse2, cudaStream_t stream) {
     using S = PromptShape<EP>;
-    cudaError_t e = cudaFuncSetAttribute(k_kv_prompt<E4M3, EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
     const int row_tiles = (a.rows + kItemRows - 1) / kItemRows;
     int64_t* const prefix = reinterpret_cast<int64_t*>(ws + p.prefix);
     PromptList* const list = reinterpret_cast<PromptList*>(ws + p.list);
     PromptStart* const starts = reinterpret_cast<PromptStart*>(ws + p.starts);
     const PromptParts w{reinterpret_cast<float*>(ws + p.out), reinterpret_cast<float2*>(ws + p.stats), list, starts, prefix,
                         lse2};
-    k_kv_prompt_plan<false><<<1, 1024, 0, stream>>>(a, list, starts, prefix,
-                                             prefix + static_cast<int64_t>(a.batch) * (row_tiles + 1), row_tiles, p.ctas);
-    int st = check_launch("dt_kv_attention");
+    int st = launch_kernel("dt_kv_attention", k_kv_prompt_plan<false>, dim3(1), 1024, 0, stream, 1, a, list, starts, prefix,
+                           prefix + static_cast<int64_t>(a.batch) * (row_tiles + 1), row_tiles, p.ctas);
     if (st != DT_OK) return st;
-    k_kv_prompt<E4M3, EP><<<p.ctas, kPromptThreads, S::kSmem, stream>>>(a, w, row_tiles);
-    st = check_launch("dt_kv_attention");
+    st = launch_kernel("dt_kv_attention", k_kv_prompt<E4M3, EP>, dim3(p.ctas), kPromptThreads, S::kSmem, stream, 1, a, w, row_tiles);
     if (st != DT_OK || p.ctas < 2) return st;
-    k_kv_prompt_merge<EP><<<dim3(p.ctas - 1, kItemRows / kMergeRows), 256, 0, stream>>>(a, w, row_tiles);
-    return check_launch("dt_kv_attention");
+    return launch_kernel("dt_kv_attention", k_kv_prompt_merge<EP>, dim3(p.ctas - 1, kItemRows / kMergeRows), 256, 0, stream, 1,
+                         a, w, row_tiles);
 }
 
 // ---------------------------------------------------------------------------------------------------------------
@@ -1023,6 +1022,7 @@ enum ColumnBar { kBFull = 0, kBEmpty = 3, kTFull = 6, kTEmpty = 10, kKReady = 14
 // for rows that give no weight: 2^-infinity is 0) and limit.
 template <bool E4M3, int EP>
 __global__ void __launch_bounds__(128) k_kv_row_blocks(KvAttnArgs a, const float* __restrict__ lse2, uint8_t* blocks) {
+    enter_kernel();
     const int tiles = (a.rows + kRowTile - 1) / kRowTile;
     const size_t head = blockIdx.x / tiles;
     const int n = static_cast<int>(head / a.kv_heads), h = static_cast<int>(head % a.kv_heads);
@@ -1064,6 +1064,7 @@ struct ColumnParts {
 
 template <bool E4M3, int EP>
 __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, ColumnParts w, int key_tiles) {
+    enter_kernel();
     using S = ColumnShape<EP>;
     extern __shared__ __align__(1024) uint8_t smem[];
     const uint32_t base = smem_addr(smem);
@@ -1267,6 +1268,7 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
 
 // Adds up the parts of the key tiles that more than one CTA of k_kv_columns worked on.
 __global__ void __launch_bounds__(128) k_kv_columns_merge(KvAttnArgs a, PromptParts w, int key_tiles) {
+    enter_kernel();
     const PromptList list = *w.list;
     if (list.each * (blockIdx.x + 1) >= list.total) return;
     const PromptItem pos(w, key_tiles, w.starts[blockIdx.x + 1]);
@@ -1283,8 +1285,6 @@ __global__ void __launch_bounds__(128) k_kv_columns_merge(KvAttnArgs a, PromptPa
 template <bool E4M3, int EP>
 int launch_columns(const KvAttnArgs& a, const KvColumnPlan& p, char* ws, const float* lse2, cudaStream_t stream) {
     using S = ColumnShape<EP>;
-    cudaError_t e = cudaFuncSetAttribute(k_kv_columns<E4M3, EP>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem);
-    if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string("dt_kv_attention: ") + cudaGetErrorString(e));
     const int key_tiles = static_cast<int>((a.capacity + kTokTile - 1) / kTokTile);
     const int64_t blocks = static_cast<int64_t>(a.batch) * a.kv_heads * ((a.rows + kRowTile - 1) / kRowTile);
     if (blocks > INT32_MAX) return set_error(DT_ERR_INVALID, "dt_kv_attention: too many blocks");
@@ -1293,18 +1293,15 @@ int launch_columns(const KvAttnArgs& a, const KvColumnPlan& p, char* ws, const f
     PromptStart* const starts = reinterpret_cast<PromptStart*>(ws + p.starts);
     uint8_t* const rows = reinterpret_cast<uint8_t*>(ws + p.blocks);
     const ColumnParts w{PromptParts{reinterpret_cast<float*>(ws + p.sums), nullptr, list, starts, prefix, nullptr}, rows};
-    k_kv_row_blocks<E4M3, EP><<<static_cast<unsigned>(blocks), 128, 0, stream>>>(a, lse2, rows);
-    int st = check_launch("dt_kv_attention");
+    int st = launch_kernel("dt_kv_attention", k_kv_row_blocks<E4M3, EP>, dim3(static_cast<unsigned>(blocks)), 128, 0, stream, 1, a,
+                           lse2, rows);
     if (st != DT_OK) return st;
-    k_kv_prompt_plan<true><<<1, 1024, 0, stream>>>(a, list, starts, prefix,
-                                                   prefix + static_cast<int64_t>(a.batch) * (key_tiles + 1), key_tiles, p.ctas);
-    st = check_launch("dt_kv_attention");
+    st = launch_kernel("dt_kv_attention", k_kv_prompt_plan<true>, dim3(1), 1024, 0, stream, 1, a, list, starts, prefix,
+                       prefix + static_cast<int64_t>(a.batch) * (key_tiles + 1), key_tiles, p.ctas);
     if (st != DT_OK) return st;
-    k_kv_columns<E4M3, EP><<<p.ctas, kColumnThreads, S::kSmem, stream>>>(a, w, key_tiles);
-    st = check_launch("dt_kv_attention");
+    st = launch_kernel("dt_kv_attention", k_kv_columns<E4M3, EP>, dim3(p.ctas), kColumnThreads, S::kSmem, stream, 1, a, w, key_tiles);
     if (st != DT_OK || p.ctas < 2) return st;
-    k_kv_columns_merge<<<p.ctas - 1, 128, 0, stream>>>(a, w.list, key_tiles);
-    return check_launch("dt_kv_attention");
+    return launch_kernel("dt_kv_attention", k_kv_columns_merge, dim3(p.ctas - 1), 128, 0, stream, 1, a, w.list, key_tiles);
 }
 
 }  // namespace
