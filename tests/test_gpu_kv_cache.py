@@ -623,3 +623,85 @@ def test_context_parallel_attention_with_a_cache(mode, group):
     step(6, dt.Shard(2))
     with pytest.raises(ValueError, match="evict"):
         step(250, dt.Shard(1))
+
+
+def test_two_captured_graphs_side_by_side():
+    """A prompt with weights and a token, captured apart and replayed at once and again, with other lengths each time."""
+    gen = torch.Generator().manual_seed(31)
+    cap, h, g, e = 1024, 2, 4, 128
+    made = []
+    for t, code in ((96, E4M3), (1, INT8)):
+        cache, _, _ = filled(gen, [700, 900], h, cap, e, code, 64)
+        cache.key_scale.nan_to_num_(0.01)  # other lengths come to lie on what was junk
+        cache.value_scale.nan_to_num_(0.01)
+        if code == E4M3:
+            cache.key.view(torch.int8)[:, :, 700:] = 3
+            cache.value.view(torch.int8)[:, :, 700:] = 5
+        q = torch.randn((2, h * g, t, e), generator=gen).to(BF16).cuda()
+        lengths, w = ints([700, 900]), torch.zeros((2, h, cap), device="cuda")
+        dt.kv_cache_attention(q, cache, lengths, weights=w, accumulate=False)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = dt.kv_cache_attention(q, cache, lengths, weights=w, accumulate=False)
+            kept = dt.kv_cache_evict(cache, lengths, w, 128, 16)
+        made.append((graph, cache, q, lengths, w, out, kept))
+    streams = [torch.cuda.Stream() for _ in made]
+    for lens in ([700, 900], [1, 64], [1024, 0], [333, 1000]):
+        for m in made:
+            m[3].copy_(ints(lens))
+        torch.cuda.synchronize()
+        for _ in range(3):
+            for s, m in zip(streams, made):
+                with torch.cuda.stream(s):
+                    m[0].replay()
+        torch.cuda.synchronize()
+        for _, cache, q, lengths, w, out, kept in made:
+            w2 = w.clone()
+            want = dt.kv_cache_attention(q, cache, lengths, weights=w2, accumulate=False)
+            assert torch.equal(out, want) and torch.equal(w, w2)
+            want = dt.kv_cache_evict(cache, lengths, w, 128, 16)
+            assert torch.equal(kept[1], want[1]) and torch.equal(kept[3], want[3])
+            a, b = (dt.kv_cache_read(c[0], c[1], dtype=torch.float32) for c in (kept, want))
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_c_abi_calls():
+    """The entry points by pointers, without kept positions and with a workspace, against the Python calls."""
+    from dtorch_b200 import capi
+
+    gen = torch.Generator().manual_seed(33)
+    n, h, cap, e, t = 2, 2, 256, 64, 40
+    cache = dt.QuantizedKVCache(n, h, cap, e, block=32)
+    same = dt.QuantizedKVCache(n, h, cap, e, block=32)
+    abi = capi.KvCache(cache.key.data_ptr(), cache.value.data_ptr(), cache.key_scale.data_ptr(), cache.value_scale.data_ptr(),
+                       n, h, cap, e, 32, capi.DT_KV_INT8)
+    k, v = tokens(gen, n, h, 150, e, FP16).cuda(), tokens(gen, n, h, 150, e, FP16).cuda()
+    q = torch.randn((n, 4, t, e), generator=gen).to(FP16).cuda()
+    zero, lengths = ints([0, 0]), ints([150, 150])
+    stream = torch.cuda.current_stream().cuda_stream
+    capi.kv_append(abi, k.data_ptr(), v.data_ptr(), 150, k.stride()[:3], v.stride()[:3], capi.DT_FLOAT16, zero.data_ptr(), None,
+                   stream)
+    dt.kv_cache_append(same, k, v, zero)
+    assert torch.equal(cache.key, same.key) and torch.equal(cache.value_scale, same.value_scale)
+    out, w = torch.empty_like(q), torch.zeros((n, h, cap), device="cuda")
+    nbytes = capi.kv_attention_workspace(abi, 4, t, True)
+    ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    with pytest.raises(capi.DtError, match="workspace"):
+        capi.kv_attention(abi, q.data_ptr(), 4, t, q.stride()[:3], capi.DT_FLOAT16, lengths.data_ptr(), None, 0.125,
+                          capi.DT_KV_CAUSAL, out.data_ptr(), None, w.data_ptr(), ws.data_ptr(), nbytes - 1, stream)
+    capi.kv_attention(abi, q.data_ptr(), 4, t, q.stride()[:3], capi.DT_FLOAT16, lengths.data_ptr(), None, 0.125,
+                      capi.DT_KV_CAUSAL, out.data_ptr(), None, w.data_ptr(), ws.data_ptr(), nbytes, stream)
+    w2 = torch.zeros_like(w)
+    assert torch.equal(out, dt.kv_cache_attention(q, same, lengths, weights=w2)) and torch.equal(w, w2)
+    value = torch.empty((n, h, 10, e), device="cuda")
+    capi.kv_read(abi, lengths.data_ptr(), None, 145, 10, None, value.data_ptr(), capi.DT_FLOAT32, stream)
+    assert torch.equal(value, dt.kv_cache_read(same, lengths, first=145, count=10, dtype=torch.float32)[1])
+    into = dt.QuantizedKVCache(n, h, 64, e, block=32)
+    abi2 = capi.KvCache(into.key.data_ptr(), into.value.data_ptr(), into.key_scale.data_ptr(), into.value_scale.data_ptr(),
+                        n, h, 64, e, 32, capi.DT_KV_INT8)
+    l2 = torch.empty_like(lengths)
+    ws = torch.empty(capi.kv_evict_workspace(abi, 50), dtype=torch.uint8, device="cuda")
+    capi.kv_evict(abi, abi2, lengths.data_ptr(), w.data_ptr(), 50, 7, l2.data_ptr(), None, None, ws.data_ptr(), ws.numel(), stream)
+    want = dt.kv_cache_evict(same, lengths, w, 50, 7)
+    assert l2.tolist() == [50, 50]
+    assert torch.equal(into.key[:, :, :50], want[0].key[:, :, :50]) and torch.equal(into.value_scale, want[0].value_scale)
