@@ -216,9 +216,11 @@ def scaled_dot_product_attention_with_cp(query: DTensor, key: DTensor, value: DT
                                          ring_cp_dim: Optional[Union[int, str]] = None,
                                          ring_overlap: bool = False, ulysses_overlap_groups: int = 1,
                                          kv_cache: Optional[DistributedKVCache] = None) -> DTensor:
-    """With `kv_cache` the new keys and values are appended to it and the queries attend over what it then holds, with
-    `is_causal` each up to its own token; no dropout, ring dim or overlap. `ulysses_overlap_groups` > 1 pipelines a pure-Ulysses call over that many head groups (batch 1, q/k/v of
-    one shape, heads divisible by groups * Ulysses size): swaps of one group overlap attention of another."""
+    """`ulysses_overlap_groups` > 1 pipelines a pure-Ulysses call over that many head groups (batch 1, q/k/v of
+    one shape, heads divisible by groups * Ulysses size): swaps of one group overlap attention of another.
+
+    With `kv_cache` the new keys and values are appended to it and the queries attend over what it then holds, with
+    `is_causal` each up to its own token; no dropout, ring dim or overlap."""
     u = _dim_index(query, ulysses_cp_dim)
     r = _dim_index(query, ring_cp_dim)
     if ring_overlap and (r is None or is_causal or dropout_p > 0.0):

@@ -1357,7 +1357,7 @@ int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, v
     if (p.many_rows) st = kv_prompt_attention(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.prompt, workspace, w.lse2, stream);
     else if (tile_rows(p.rows) == 8) st = launch_few_rows<E4M3, EP, 1>(a, w, p, stream);
     else st = launch_few_rows<E4M3, EP, 2>(a, w, p, stream);
-    if (st != DT_OK || !weights) return st;
+    if (st != DT_OK || !weights || a.capacity == 0) return st;
     const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
     if (w.scores != nullptr) {
         const unsigned y = static_cast<unsigned>(std::min<int64_t>(heads, 32768));
