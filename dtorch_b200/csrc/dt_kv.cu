@@ -1242,12 +1242,12 @@ int check_cache(const dt_kv_cache* c, const char* name) {
         return set_error(DT_ERR_INVALID, who + "block must be 32, 64 or 128 tokens");
     if (c->head_dim < 16 || c->head_dim > 256 || c->head_dim % 16 != 0)
         return set_error(DT_ERR_INVALID, who + "head_dim must be a multiple of 16 up to 256");
-    if (c->batch < 0 || c->kv_heads < 1 || c->capacity < 0 || c->capacity % c->block != 0)
-        return set_error(DT_ERR_INVALID, who + "capacity must be a multiple of block, heads at least 1");
+    if (c->batch < 0 || c->kv_heads < 1 || c->capacity < 1 || c->capacity % c->block != 0)
+        return set_error(DT_ERR_INVALID, who + "capacity must be a positive multiple of block, heads at least 1");
     if (c->capacity > (int64_t{1} << 30) || c->batch > (int64_t{1} << 20) || c->kv_heads > (int64_t{1} << 16) ||
         c->batch * c->kv_heads > (int64_t{1} << 24))
         return set_error(DT_ERR_INVALID, who + "too many tokens, sequences or heads");
-    if (c->batch == 0 || c->capacity == 0) return DT_OK;
+    if (c->batch == 0) return DT_OK;
     if (c->key == nullptr || c->value == nullptr || c->key_scale == nullptr || c->value_scale == nullptr)
         return set_error(DT_ERR_INVALID, who + "null buffer");
     if (!aligned16(c->key) || !aligned16(c->value)) return set_error(DT_ERR_INVALID, who + "codes must be 16-byte aligned");
@@ -1357,7 +1357,7 @@ int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, v
     if (p.many_rows) st = kv_prompt_attention(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.prompt, workspace, w.lse2, stream);
     else if (tile_rows(p.rows) == 8) st = launch_few_rows<E4M3, EP, 1>(a, w, p, stream);
     else st = launch_few_rows<E4M3, EP, 2>(a, w, p, stream);
-    if (st != DT_OK || !weights || a.capacity == 0) return st;
+    if (st != DT_OK || !weights) return st;
     const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
     if (w.scores != nullptr) {
         const unsigned y = static_cast<unsigned>(std::min<int64_t>(heads, 32768));
@@ -1387,7 +1387,7 @@ int dt_kv_append(const dt_kv_cache* cache, const void* key, const void* value, i
     if (dtype != DT_BFLOAT16 && dtype != DT_FLOAT16)
         return set_error(DT_ERR_INVALID, "dt_kv_append: keys and values must be bf16 or fp16");
     if (tokens < 0 || tokens > (int64_t{1} << 30)) return set_error(DT_ERR_INVALID, "dt_kv_append: bad token count");
-    if (cache->batch == 0 || cache->capacity == 0 || tokens == 0) return DT_OK;
+    if (cache->batch == 0 || tokens == 0) return DT_OK;
     if (key == nullptr || value == nullptr || key_strides == nullptr || value_strides == nullptr || lengths == nullptr)
         return set_error(DT_ERR_INVALID, "dt_kv_append: null argument");
     KvAppendArgs a{};

@@ -317,7 +317,8 @@ int dt_local_all_to_all(int n, const void* const* ins, void* const* outs, int nd
  * All entry points run on the current device and stream, allocate nothing, and can be captured in a CUDA graph.
  * `lengths`, `counts` and `first` are device arrays of `batch` int32. Lengths are taken as 0 where they are negative
  * and as the capacity where they are larger. Slots behind a sequence's length are never read as values: they may
- * hold anything. head_dim: a multiple of 16, up to 256; block: 32, 64 or 128; capacity: a multiple of block. */
+ * hold anything. head_dim: a multiple of 16, up to 256; block: 32, 64 or 128; capacity: a positive multiple
+ * of block. */
 
 typedef enum dt_kv_code {
     DT_KV_INT8 = 0, /* -127..127 */

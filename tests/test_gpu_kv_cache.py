@@ -705,18 +705,3 @@ def test_c_abi_calls():
     want = dt.kv_cache_evict(same, lengths, w, 50, 7)
     assert l2.tolist() == [50, 50]
     assert torch.equal(into.key[:, :, :50], want[0].key[:, :, :50]) and torch.equal(into.value_scale, want[0].value_scale)
-
-
-def test_c_abi_of_a_cache_without_capacity():
-    from dtorch_b200 import capi
-
-    abi = capi.KvCache(None, None, None, None, 2, 1, 0, 32, 32, capi.DT_KV_E4M3)
-    stream, lengths = torch.cuda.current_stream().cuda_stream, ints([0, 5])
-    for t in (1, 40):
-        q = torch.randn((2, 1, t, 32), device="cuda").to(BF16)
-        out, w = torch.full_like(q, 3.0), torch.zeros(4, device="cuda")
-        nbytes = capi.kv_attention_workspace(abi, 1, t, True)
-        ws = torch.empty(nbytes, dtype=torch.uint8, device="cuda")
-        capi.kv_attention(abi, q.data_ptr(), 1, t, q.stride()[:3], capi.DT_BFLOAT16, lengths.data_ptr(), None, 1.0, 0,
-                          out.data_ptr(), None, w.data_ptr(), ws.data_ptr(), nbytes, stream)
-        assert not out.any() and not w.any()

@@ -113,7 +113,7 @@ def abi(**kw):
 
 @pytest.mark.parametrize("kw", [dict(code=2), dict(block=8), dict(head_dim=20), dict(head_dim=512), dict(capacity=65),
                                 dict(batch=-1), dict(kv_heads=0), dict(key=None), dict(value_scale=None), dict(key=4100),
-                                dict(capacity=1 << 31)])
+                                dict(capacity=1 << 31), dict(capacity=0)])
 def test_c_abi_refuses_caches(kw):
     L, c, ptr = capi.lib(), abi(**kw), 4096
     s = capi.i64_array([1, 1, 1])
