@@ -627,6 +627,12 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
                     }
             // values: 8 x 8 pairs of bytes transposed on the way in; even elements are rows 0-7 of the operand, odd 8-15
             const uint32_t vst = stages_s + st * S::kStageBytes + S::kSliceBytes;
+            // rows that see nothing of the slice take nothing, whatever its scale: a marked block's is NaN
+            float vs[NT][2];
+#pragma unroll
+            for (int j = 0; j < NT; ++j)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) vs[j][i] = lim[j][i] > tok ? vscale : 0.0f;
 #pragma unroll
             for (int e = 0; e < EP / 16; ++e) {
                 uint32_t v[4];
@@ -647,7 +653,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
 #pragma unroll
                 for (int j = 0; j < NT; ++j)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) o[e][j][i] = fmaf(vscale, acc[j][i], o[e][j][i]);
+                    for (int i = 0; i < 4; ++i) o[e][j][i] = fmaf(vs[j][i & 1], acc[j][i], o[e][j][i]);
             }
         }
 

@@ -1,0 +1,72 @@
+"""GPU: attention over the 8-bit key/value cache where masks, marked blocks, large scores and block scales far apart
+meet, and calls that are refused as a whole."""
+
+import math
+
+import pytest
+import torch
+
+import dtorch_b200 as dt
+from tests import kv_oracle as ko
+from tests.test_gpu_kv_cache import BF16, E4M3, FP16, INT8, check_attention, filled, ints, tokens
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(autouse=True)
+def _need_gpu():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+
+
+def check_with_nan(cache, ok, ov, lengths, q, counts, causal):
+    """As check_attention, for oracles that hold NaN: NaN where the oracle has one and nowhere else."""
+    w = torch.zeros((cache.batch, cache.kv_heads, cache.capacity), device="cuda")
+    out, lse = dt.kv_cache_attention(q, cache, ints(lengths), counts=None if counts is None else ints(counts),
+                                     is_causal=causal, weights=w, return_lse=True)
+    eo, el, ew, mag, size = ko.attention(q.cpu().double(), ok.values(), ov.values(), lengths, counts, causal)
+    out, lse, w = out.cpu().double(), lse.cpu().double(), w.cpu().double()
+    assert torch.equal(out.isnan(), eo.isnan()), "outputs that are NaN"
+    good = ~eo.isnan()
+    assert ((out - eo).abs() <= ko.attention_bounds(eo, mag, size, q.dtype))[good].all()
+    assert torch.equal(lse.isnan(), el.isnan()), "log-sum-exps that are NaN"
+    good = ~el.isnan() & ~el.isinf()
+    assert torch.equal(lse.isinf(), el.isinf())
+    assert ((lse - el).abs() <= 2.0 ** -19 * size + 2.0 ** -21 * el.abs() + 2.0 ** -20)[good].all()
+    assert torch.equal(w.isnan(), ew.isnan()), "weights that are NaN"
+    good = ~ew.isnan()
+    dmax = size.nan_to_num().amax()
+    assert ((w - ew).abs() <= (2 * 2.0 ** -19 * dmax + 2.0 ** -18) * ew + 2.0 ** -100)[good].all()
+
+
+@pytest.mark.parametrize("which", ["value", "key"])
+@pytest.mark.parametrize("code,e,g,t", [(E4M3, 64, 2, 1), (INT8, 128, 2, 5), (INT8, 128, 1, 24), (E4M3, 128, 2, 66),
+                                        (INT8, 64, 1, 66), (INT8, 256, 1, 5), (E4M3, 192, 1, 40)])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("padded", [False, True])
+def test_a_marked_block_reaches_only_queries_that_see_it(which, code, e, g, t, causal, padded):
+    # blocks of 32; in sequence i block i is marked: in front of all queries' limits, across them, behind the first ones,
+    # behind some of the padded batch's
+    gen = torch.Generator().manual_seed(t + e)
+    lengths = [70, 96, 100, 130, 158, 160, 161, 200]
+    marked = [0, 2, 3, 4, 4, 4, 5, 4]
+    counts = [t, 0, t, max(t // 2, 1), t, 1, t - 1, t] if padded else None
+    cache, ok, ov = filled(gen, lengths, 2, 224, e, code, 32)
+    for i, b in enumerate(marked):
+        (cache.value_scale if which == "value" else cache.key_scale)[i, 1, b] = math.nan
+        (ov if which == "value" else ok).scale[i, 1, b] = math.nan
+    q = torch.randn((len(lengths), 2 * g, t, e), generator=gen).to(BF16).cuda()
+    check_with_nan(cache, ok, ov, lengths, q, counts, causal)
+
+
+@pytest.mark.parametrize("t", [8, 70])
+def test_a_marked_block_in_a_sequence_that_many_ctas_share(t):
+    # the last block is marked; most queries end before it, and their parts come from many CTAs
+    gen = torch.Generator().manual_seed(t)
+    l = 6000 - 6000 % 32 + 2
+    cache, ok, ov = filled(gen, [l], 1, 6016, 64, INT8, 32)
+    cache.value_scale[0, 0, l // 32] = math.nan
+    ov.scale[0, 0, l // 32] = math.nan
+    q = torch.randn((1, 2, t, 64), generator=gen).to(BF16).cuda()
+    check_with_nan(cache, ok, ov, [l], q, None, True)
+    assert dt.kv_cache_attention(q, cache, ints([l])).isnan().any(-1).sum() == 2 * 2
