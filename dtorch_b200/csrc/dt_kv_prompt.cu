@@ -61,7 +61,7 @@ struct PromptShape {
     static constexpr int kCodeBytes = 128 * EP;
     static constexpr int kScales = kCodes + 2 * kCodeBytes;    // [ring][keys, values][4]
     static constexpr int kBars = kScales + kScaleRing * 2 * 4 * 4;
-    static constexpr int kTops = kBars + 256;                  // 8 bytes a row: bfloat16 [parity][half], or float [half]
+    static constexpr int kTops = kBars + 256;                  // a float for each softmax thread: [half][256 rows]
     static constexpr int kSmem = kTops + 2 * 128 * 8;
     static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
     static constexpr int kTmemCols = 512;
@@ -188,13 +188,6 @@ __device__ __forceinline__ uint32_t operand_offset(int r, int c) {
     return (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) << 4);
 }
 
-// The least bfloat16 that is not below x (its upper 16 bits), and back.
-__device__ __forceinline__ uint16_t round_up16(float x) {
-    const uint32_t b = __float_as_uint(x);
-    return static_cast<uint16_t>(((b >> 31) != 0 || b == 0x7f800000u ? b : b + 0xffffu) >> 16);
-}
-__device__ __forceinline__ float from16(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
-
 // Barrier of two warps.
 __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
@@ -203,14 +196,14 @@ __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 6
 // softmax scale, so that the score factor is not negative.
 template <int EP>
 __device__ __forceinline__ float stage_query(const KvAttnArgs& a, const uint16_t* p, uint8_t* smem, int r, int half,
-                                             volatile uint16_t* mine, volatile uint16_t* other, int id, float sign) {
+                                             volatile float* mine, volatile float* other, int id, float sign) {
     uint32_t x[EP / 4];
     load_row<EP / 16>(a, p, half * (EP / 2), x);
     const float amax = row_max<EP / 4>(a, x);
-    *mine = round_up16(amax);
+    *mine = amax;
     pair_sync(id);
     float mul, inv;
-    row_power(fmaxf(from16(*mine), from16(*other)), mul, inv);
+    row_power(fmaxf(amax, *other), mul, inv);
     mul *= sign;
 #pragma unroll
     for (int c = 0; c < EP / 16; ++c) {
@@ -682,8 +675,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
         // row tile, half of the columns, row, and the barrier and places shared with the row's other thread
         const int g = warp >> 3, half = (warp >> 2) & 1, r = tid & 127;
         const int pair = 1 + g * 4 + (warp & 3);
-        volatile uint16_t* const tops = reinterpret_cast<volatile uint16_t*>(smem + S::kTops) + (g * 128 + r) * 4;
-        volatile float* const sums = reinterpret_cast<volatile float*>(tops);
+        // What the thread hands to the row's other one: |q|, each tile's top, the sum. One place serves all: it is written
+        // again only behind a completed S (or O), which the issuing warp asked for after every warp of the row tile
+        // had reported its queries or weights, and those come after its reads.
+        volatile float* const mine = reinterpret_cast<volatile float*>(smem + S::kTops) + half * 256 + g * 128 + r;
+        volatile float* const other = reinterpret_cast<volatile float*>(smem + S::kTops) + (half ^ 1) * 256 + g * 128 + r;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
         // this thread's columns of S; a span's weights lie over its own scores
         const uint32_t s_col = (tmem + g * 128 + half * 64) | lanes, o_col = (tmem + 256 + g * EP + half * (EP / 2)) | lanes;
@@ -703,9 +699,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 if (row < a.rows)
                     qp = static_cast<const uint16_t*>(a.query) + pos.n * a.q_stride_n +
                          static_cast<int64_t>(pos.h * a.group + jj) * a.q_stride_h + t * a.q_stride_t;
-                // in the places of odd tiles: the first tile's are written before the other thread has read these
-                const float inv = stage_query<EP>(a, qp, smem + S::kQuery + g * S::kOperand, r, half, tops + 2 + half,
-                                                  tops + 2 + (half ^ 1), pair, a.scale_log2 < 0.0f ? -1.0f : 1.0f);
+                const float inv = stage_query<EP>(a, qp, smem + S::kQuery + g * S::kOperand, r, half, mine, other, pair,
+                                                  a.scale_log2 < 0.0f ? -1.0f : 1.0f);
                 factor = inv * fabsf(a.scale_log2);
                 tc_fence_before();  // the reads of O of the item before
                 async_proxy_fence();
@@ -762,12 +757,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                     const float m = fmaxf(mx[0], mx[1]);
                     if (m != -INFINITY) top = fmaxf(top, m * (factor * sc[k]));  // masked stays so where the scale is 0
                 }
-                // the row's largest, of both halves, as bfloat16 rounded up: a reference need not be exact. The next use
-                // of these places is two tiles on, behind the other thread's barrier of the next.
-                const uint16_t top16 = round_up16(top);
-                tops[(j & 1) * 2 + half] = top16;
+                // the row's largest, of both halves, in fp32: large scores leave a 16-bit float's step no room above it
+                *mine = top;
                 pair_sync(pair);
-                top = fmaxf(from16(top16), from16(tops[(j & 1) * 2 + (half ^ 1)]));
+                top = fmaxf(top, *other);
                 const bool grow = top > ref + kGrowth;  // also the first: ref is -infinity
                 if (__any_sync(0xffffffffu, grow)) {    // the same for both warps of the pair
                     const float now = grow ? top : ref;
@@ -821,11 +814,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
             ++phase;
             __syncwarp();
             tc_fence_after();
-            pair_sync(pair);  // the other thread has read the last tile's top
-            sums[half] = l;
+            *mine = l;
             pair_sync(pair);
-            l += sums[half ^ 1];
-            pair_sync(pair);  // and both have read the sums, whose places take the next queries' tops
+            l += *other;
+            pair_sync(pair);  // both have read the sums, whose places take the next queries' tops
             if (*dead) l = __int_as_float(0x7fc00000);
             const float v_up = 1.0f / v_down;  // powers of two
             if (item_steps < pos.tiles) {

@@ -19,6 +19,17 @@ def _need_gpu():
         pytest.skip("no CUDA device")
 
 
+def appended(k, v, cap, code, block):
+    """A cache that holds k and v (N, H, cap, E) whole, and its oracle."""
+    n, h, _, e = k.shape
+    cache = dt.QuantizedKVCache(n, h, cap, e, dtype=code, block=block)
+    dt.kv_cache_append(cache, k.cuda(), v.cuda(), ints([0] * n))
+    ok, ov = ko.Cache(n, h, cap, e, code, block), ko.Cache(n, h, cap, e, code, block)
+    ok.append(k, [0] * n)
+    ov.append(v, [0] * n)
+    return cache, ok, ov
+
+
 def check_with_nan(cache, ok, ov, lengths, q, counts, causal):
     """As check_attention, for oracles that hold NaN: NaN where the oracle has one and nowhere else."""
     w = torch.zeros((cache.batch, cache.kv_heads, cache.capacity), device="cuda")
@@ -70,3 +81,23 @@ def test_a_marked_block_in_a_sequence_that_many_ctas_share(t):
     q = torch.randn((1, 2, t, 64), generator=gen).to(BF16).cuda()
     check_with_nan(cache, ok, ov, [l], q, None, True)
     assert dt.kv_cache_attention(q, cache, ints([l])).isnan().any(-1).sum() == 2 * 2
+
+
+@pytest.mark.parametrize("t", [1, 12, 66])
+@pytest.mark.parametrize("size", [3000.0, -3000.0, 6000.0, -6000.0, 10000.0, -10000.0, 50000.0])
+@pytest.mark.parametrize("code,e", [(INT8, 64), (E4M3, 128)])
+def test_attention_of_large_scores(t, size, code, e):
+    # Scores of one size and sign in all tokens, apart by up to about 8: the products of one channel are nearly all of
+    # a score, so sum |q k| is little above |score| and the bound stays tight enough to tell (2^-18 of the size: 4 % of
+    # a weight at 10000). Every query has another size, so that the largest score is anywhere between two bfloat16.
+    gen = torch.Generator().manual_seed(int(abs(size)) + t)
+    n, h, cap = 2, 1, 320
+    k = torch.zeros((n, h, cap, e))
+    k[..., 0] = 1.0
+    k[..., 1:9] = (torch.rand((n, h, cap, 8), generator=gen) - 0.5) * 2
+    v = torch.randn((n, h, cap, e), generator=gen)
+    cache, ok, ov = appended(k.to(BF16), v.to(BF16), cap, code, 64)
+    q = torch.zeros((n, 2, t, e))
+    q[..., 0] = size * (1 + torch.rand((n, 2, t), generator=gen))
+    q[..., 1:9] = torch.randn((n, 2, t, 8), generator=gen)
+    check_attention(cache, ok, ov, [cap, 300], q.to(BF16).cuda(), scale=1.0)
