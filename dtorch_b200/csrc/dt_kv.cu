@@ -292,7 +292,9 @@ __global__ void __launch_bounds__(256) k_kv_read(KvReadArgs a) {
 constexpr int kTile = 128;
 constexpr int kWarpTokens = 32;
 constexpr int kAttnThreads = 128;
-constexpr float kShift = 10.0f;  // weights are kept as 2^(x - max + 10): fp16 then reaches down to 2^-34 of the largest
+// A weight is rounded to fp16 as 2^(x - top + 10), top the largest score of the row in the warp's slice: 11 significant
+// bits down to 2^-24 of the slice's largest. What the slice's largest is to the row's goes into the value scale, in fp32.
+constexpr float kShift = 10.0f;
 
 struct KvPartials {
     float* out;     // [slot][row tile's rows][EP]
@@ -563,7 +565,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
             }
             const bool ragged = __any_sync(0xffffffffu, tok + kWarpTokens > least);
             bool grown = false;
-            float alpha[NT][2], base[NT][2];
+            float alpha[NT][2], base[NT][2], gain[NT][2], vs[NT][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j)
 #pragma unroll
@@ -581,11 +583,18 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
                         }
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, d));
-                    const float now = fmaxf(m[j][i], top);
-                    alpha[j][i] = now == m[j][i] ? 1.0f : ex2(m[j][i] - now);
-                    grown |= now != m[j][i];
-                    m[j][i] = now;
-                    base[j][i] = now == -INFINITY ? 0.0f : now - kShift;  // a row that saw nothing: 2^-inf = 0
+                    // the smaller of the running and the slice's largest, to the larger
+                    const bool over = top > m[j][i];
+                    const float ratio = ex2(over ? m[j][i] - top : top - m[j][i]);
+                    alpha[j][i] = over ? ratio : 1.0f;
+                    gain[j][i] = over ? 1.0f : ratio;
+                    base[j][i] = top - kShift;
+                    vs[j][i] = vscale * gain[j][i];
+                    if (top == -INFINITY) {  // nothing seen here: no weight, and no value whatever its scale (NaN of a marked block)
+                        gain[j][i] = vs[j][i] = base[j][i] = 0.0f;
+                    }
+                    grown |= over;
+                    m[j][i] = over ? top : m[j][i];
                 }
             if (scores != nullptr) {
 #pragma unroll
@@ -615,24 +624,22 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
             // weights: fp16 (11 significant bits, half a bf16 output's rounding at most), as the B operand of 16 tokens
             uint32_t p[2][NT][2];
 #pragma unroll
-            for (int t = 0; t < 2; ++t)
+            for (int j = 0; j < NT; ++j) {
+                float sum[2] = {0.0f, 0.0f};
 #pragma unroll
-                for (int j = 0; j < NT; ++j)
+                for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
                         const float u = ex2(s[t][j][k * 2] - base[j][0]), v = ex2(s[t][j][k * 2 + 1] - base[j][1]);
-                        l[j][0] += u;
-                        l[j][1] += v;
+                        sum[0] += u;
+                        sum[1] += v;
                         p[t][j][k] = transpose8(pack_half2(u, v));
                     }
+                l[j][0] = fmaf(sum[0], gain[j][0], l[j][0]);
+                l[j][1] = fmaf(sum[1], gain[j][1], l[j][1]);
+            }
             // values: 8 x 8 pairs of bytes transposed on the way in; even elements are rows 0-7 of the operand, odd 8-15
             const uint32_t vst = stages_s + st * S::kStageBytes + S::kSliceBytes;
-            // rows that see nothing of the slice take nothing, whatever its scale: a marked block's is NaN
-            float vs[NT][2];
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) vs[j][i] = lim[j][i] > tok ? vscale : 0.0f;
 #pragma unroll
             for (int e = 0; e < EP / 16; ++e) {
                 uint32_t v[4];

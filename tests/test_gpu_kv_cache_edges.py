@@ -101,3 +101,21 @@ def test_attention_of_large_scores(t, size, code, e):
     q[..., 0] = size * (1 + torch.rand((n, 2, t), generator=gen))
     q[..., 1:9] = torch.randn((n, 2, t, 8), generator=gen)
     check_attention(cache, ok, ov, [cap, 300], q.to(BF16).cuda(), scale=1.0)
+
+
+@pytest.mark.parametrize("t", [1, 9])
+@pytest.mark.parametrize("down,up", [(40, 38), (100, 98)])
+@pytest.mark.parametrize("code,e", [(INT8, 64), (E4M3, 128), (INT8, 256)])
+def test_small_weights_of_large_values_behind_others_in_a_stretch(t, down, up, code, e):
+    # as many tiles as make a CTA take several of a sequence: the same tokens of each tile, block by block, share a state
+    gen = torch.Generator().manual_seed(down + t)
+    n, cap = 160, 512
+    k, v = torch.randn((n, 1, cap, e), generator=gen) * 0.25, torch.randn((n, 1, cap, e), generator=gen)
+    k[..., 0] = 1.0
+    for b in (128, 384 + 32):
+        k[:, :, b:b + 32, 0] = -1.0
+        v[:, :, b:b + 32] *= 2.0 ** up
+    cache, ok, ov = appended(k.to(BF16), v.to(BF16), cap, code, 32)
+    q = torch.randn((n, 2, t, e), generator=gen) * 0.2
+    q[..., 0] = down * math.log(2) / 2
+    check_attention(cache, ok, ov, [cap] * n, q.to(BF16).cuda(), causal=False, scale=1.0)
