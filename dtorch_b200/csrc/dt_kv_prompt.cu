@@ -31,11 +31,12 @@ namespace {
 // product's burst rate. Bound by the chain of each row tile (scores, softmax, weights, products: 4000 cycles, of which
 // the tensor core works 1024, twice a step) and by issue slots; exponentials and products alone would take 2048.
 //
-// A softmax row keeps a reference instead of its exact maximum: it moves (and O is scaled, in TMEM) only when the
-// maximum has grown by more than 2^3, so weights stay below 2^3 and the scaling is rare. Block scales: a key scale is
-// constant over 32 columns and goes into the row's factor; a value scale, relative to a power of two above all of the
-// sequence's, into the weight before it is rounded to fp16 (11 bits; 2^kPromptShift keeps values down to 2^-26 of the
-// largest normal).
+// Block scales are constant over 32 columns: a key scale goes into the row's factor, a value scale into the weight before
+// it is rounded to fp16. What is rounded is therefore 2^x * (value scale), and its reference is the row's largest of
+// those: x plus the scale's exponent, of the tokens that the row sees. Times 2^kPromptShift it keeps 11 significant bits
+// down to 2^-26 of the row's largest, whatever the sizes of values that the row does not see or gives no weight. The sum
+// of the weights goes without the value scale, so it has a reference of its own, each thread's largest x. References
+// move only when their maximum has grown by more than 2^3 (for the first, O is then scaled, in TMEM), which is rare.
 constexpr int kRowTile = 128;
 constexpr int kTokTile = 128;
 constexpr int kPromptThreads = 768;
@@ -47,6 +48,8 @@ static_assert(512 * kSoftmaxRegs + 128 * kConvertRegs + 128 * kIssueRegs <= kPro
 constexpr float kGrowth = 3.0f;
 constexpr float kPromptShift = 12.0f;
 constexpr int kScaleRing = 4;
+// Exponents of value scales that count; scales of 0 and NaN have the least: their tokens do not set the reference.
+constexpr int kLeastExponent = -100;
 constexpr uint64_t kWaitLimitNs = 10000000000ull;  // waits of one CTA for its own work last microseconds
 
 template <int EP>
@@ -59,8 +62,8 @@ struct PromptShape {
     static constexpr int kValues = 4 * kOperand;               // two stages
     static constexpr int kCodes = 6 * kOperand;                // a tile's codes of keys and of values, on their way
     static constexpr int kCodeBytes = 128 * EP;
-    static constexpr int kScales = kCodes + 2 * kCodeBytes;    // [ring][keys, values][4]
-    static constexpr int kBars = kScales + kScaleRing * 2 * 4 * 4;
+    static constexpr int kScales = kCodes + 2 * kCodeBytes;    // [ring][keys, values, values' exponents][4]
+    static constexpr int kBars = kScales + kScaleRing * 3 * 4 * 4;
     static constexpr int kTops = kBars + 256;                  // a float for each softmax thread: [half][256 rows]
     static constexpr int kSmem = kTops + 2 * 128 * 8;
     static_assert(kSmem <= 227 * 1024, "shared memory of one CTA");
@@ -651,7 +654,11 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                     if (tok < len) sc = sbase[tok >> a.block_shift];
                 }
                 mbar_wait(bars + (kKEmpty + st) * 8, free_parity, dead);
-                if (t < 8) scales[(c % kScaleRing) * 8 + t] = sc;
+                if (t < 8) scales[(c % kScaleRing) * 12 + t] = sc;
+                if (t >= 4 && t < 8) {  // sc < 2^ex
+                    const int bits = (__float_as_uint(sc) >> 23) & 255, ex = bits == 255 ? kLeastExponent : bits - 126;
+                    scales[(c % kScaleRing) * 12 + t + 4] = static_cast<float>(max(ex, kLeastExponent));
+                }
                 asm volatile("cp.async.wait_group 1;" ::: "memory");
                 store_operand<E4M3, EP>(smem + S::kKeys + st * S::kOperand, kcodes, t);
                 async_proxy_fence();
@@ -675,9 +682,9 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
         // row tile, half of the columns, row, and the barrier and places shared with the row's other thread
         const int g = warp >> 3, half = (warp >> 2) & 1, r = tid & 127;
         const int pair = 1 + g * 4 + (warp & 3);
-        // What the thread hands to the row's other one: |q|, each tile's top, the sum. One place serves all: it is written
-        // again only behind a completed S (or O), which the issuing warp asked for after every warp of the row tile
-        // had reported its queries or weights, and those come after its reads.
+        // What the thread hands to the row's other one: |q| and each tile's top. One place serves all: it is written again
+        // only behind a completed S, which the issuing warp asked for after every warp of the row tile had reported its
+        // queries or weights, and those come after its reads; and by an item's queries behind the last product of O.
         volatile float* const mine = reinterpret_cast<volatile float*>(smem + S::kTops) + half * 256 + g * 128 + r;
         volatile float* const other = reinterpret_cast<volatile float*>(smem + S::kTops) + (half ^ 1) * 256 + g * 128 + r;
         const uint32_t lanes = static_cast<uint32_t>((warp & 3) * 32) << 16;
@@ -707,33 +714,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bars + kQReady * 8);
             }
-            // a power of two that no value scale of these tiles exceeds
-            float vtop = 0.0f;
-            {
-                const float* const vs = a.value_scale + head * a.nblocks;
-                const int first = (pos.tile * kTokTile) >> a.block_shift;
-                const int end = min((pos.tile + item_steps) * kTokTile, len);
-                for (int i = first + lane; i < (end + (1 << a.block_shift) - 1) >> a.block_shift; i += 32)
-                    vtop = fmaxf(vtop, vs[i]);
-#pragma unroll
-                for (int d = 16; d > 0; d >>= 1) vtop = fmaxf(vtop, __shfl_xor_sync(0xffffffffu, vtop, d));
-            }
-            int ve = static_cast<int>(__float_as_uint(vtop) >> 23) - 126;  // vtop < 2^ve
-            ve = ve < -100 ? -100 : ve > 126 ? 126 : ve;
-            const float v_down = __uint_as_float(static_cast<uint32_t>(127 - ve) << 23) * exp2f(kPromptShift);
             int live = kv_limit(a, row, len, cnt) - pos.tile * kTokTile - half * 64;  // of this thread's columns
 
-            float ref = -INFINITY, l = 0.0f;
+            // largest x of this thread's columns, and of the row's x + exponent of the value scale, as references
+            float ref = -INFINITY, out_ref = -INFINITY, l = 0.0f;
             const int steps = live_group ? item_steps : 0;
             for (int j = 0; j < steps; ++j) {
                 mbar_wait(s_full, phase & 1, dead);
                 ++phase;
                 __syncwarp();
                 tc_fence_after();
-                const float* const sc = scales + ((c + j) % kScaleRing) * 8 + half * 2;
+                const float* const sc = scales + ((c + j) % kScaleRing) * 12 + half * 2;
                 const bool ragged = __any_sync(0xffffffffu, live < 64);
                 uint32_t s[32], s0[32];
-                float top = -INFINITY;
+                float top = -INFINITY, out_top = -INFINITY;
                 // span 0 is loaded again for its weights: 32 scores fewer to hold meanwhile
                 tmem_load32(s_col, s0);
                 tmem_load32(s_col + 32, s);
@@ -755,18 +749,25 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                         mx[1] = max3(mx[1], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
                     }
                     const float m = fmaxf(mx[0], mx[1]);
-                    if (m != -INFINITY) top = fmaxf(top, m * (factor * sc[k]));  // masked stays so where the scale is 0
+                    if (m != -INFINITY) {  // masked stays so where the scale is 0
+                        const float x = m * (factor * sc[k]);
+                        top = fmaxf(top, x);
+                        out_top = fmaxf(out_top, x + sc[8 + k]);
+                    }
                 }
                 // the row's largest, of both halves, in fp32: large scores leave a 16-bit float's step no room above it
-                *mine = top;
+                *mine = out_top;
                 pair_sync(pair);
-                top = fmaxf(top, *other);
-                const bool grow = top > ref + kGrowth;  // also the first: ref is -infinity
-                if (__any_sync(0xffffffffu, grow)) {    // the same for both warps of the pair
-                    const float now = grow ? top : ref;
-                    const float alpha = grow ? ex2(ref - now) : 1.0f;
-                    ref = now;
-                    l *= alpha;
+                out_top = fmaxf(out_top, *other);
+                if (top > ref + kGrowth) {  // also the first: ref is -infinity
+                    l *= ex2(ref - top);
+                    ref = top;
+                }
+                const bool grow = out_top > out_ref + kGrowth;
+                if (__any_sync(0xffffffffu, grow)) {  // the same for both warps of the pair
+                    const float now = grow ? out_top : out_ref;
+                    const float alpha = grow ? ex2(out_ref - now) : 1.0f;
+                    out_ref = now;
                     if (j > 0) {
 #pragma unroll 1
                         for (int k = 0; k < EP / 2; k += 32) {
@@ -779,12 +780,17 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                         }
                     }
                 }
-                const float down = ref == -INFINITY ? 0.0f : ref;
+                const bool none = ref == -INFINITY;
+                const float down = none ? 0.0f : ref;
+                // ref - out_ref is below 2^7: out_ref counts ref's own token with an exponent of at least kLeastExponent
+                const float v_down = none ? 0.0f : ex2(ref - out_ref + kPromptShift);
                 Pair sum[2] = {0, 0};
 #pragma unroll
                 for (int k = 1; k >= 0; --k) {
                     uint32_t p[16];
-                    const float f = factor * sc[k], vf = sc[4 + k] * v_down;
+                    const float f = factor * sc[k];
+                    float vf = sc[4 + k] * v_down;
+                    if (vf > 0x1p126f) vf = 0x1p126f;  // only where all weights are below 2^-111; a NaN scale stays
                     if (k == 0) {
                         tmem_load32(s_col, s);
                         tmem_wait_load32(s);
@@ -814,12 +820,19 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
             ++phase;
             __syncwarp();
             tc_fence_after();
-            *mine = l;
+            // The sums of both threads, through the memory of the row's queries, which are done with.
+            uint8_t* const rows = smem + S::kQuery + g * S::kOperand;
+            *reinterpret_cast<float2*>(rows + operand_offset(r, half)) = make_float2(ref, l);
             pair_sync(pair);
-            l += *other;
-            pair_sync(pair);  // both have read the sums, whose places take the next queries' tops
+            {
+                const float2 o = *reinterpret_cast<const float2*>(rows + operand_offset(r, half ^ 1));
+                const float most = fmaxf(ref, o.x);
+                l = l * (ref == most ? 1.0f : ex2(ref - most)) + o.y * (o.x == most ? 1.0f : ex2(o.x - most));
+                ref = most;
+            }
+            pair_sync(pair);  // both have read them: outputs, or the next queries, take their places
             if (*dead) l = __int_as_float(0x7fc00000);
-            const float v_up = 1.0f / v_down;  // powers of two
+            const float v_up = ref == -INFINITY ? 0.0f : exp2f(out_ref - ref - kPromptShift);
             if (item_steps < pos.tiles) {
                 // an item that other CTAs work on too: one that began before this stretch, or goes on behind it
                 const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (pos.tile > 0 ? 0 : 1);
@@ -842,7 +855,6 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
             }
             const float inv_l = v_up / l;
             // the rows go through the memory of their queries, which are done with, so that stores are of whole rows
-            uint8_t* const rows = smem + S::kQuery + g * S::kOperand;
 #pragma unroll 1
             for (int k0 = 0; k0 < EP / 2; k0 += 32) {
                 uint32_t o[32];

@@ -103,6 +103,41 @@ def test_attention_of_large_scores(t, size, code, e):
     check_attention(cache, ok, ov, [cap, 300], q.to(BF16).cuda(), scale=1.0)
 
 
+@pytest.mark.parametrize("t", [3, 66])
+@pytest.mark.parametrize("power", [24, 30, 36, 100])
+@pytest.mark.parametrize("code,e", [(INT8, 64), (E4M3, 128)])
+def test_values_far_larger_behind_a_querys_limit(t, power, code, e):
+    # the last block's values are 2^power larger than the others; only the last query sees one token of it
+    gen = torch.Generator().manual_seed(power)
+    n, h, cap = 2, 1, 416
+    k, v = torch.randn((n, h, cap, e), generator=gen), torch.randn((n, h, cap, e), generator=gen)
+    v[:, :, 384:] *= 2.0 ** power
+    cache, ok, ov = appended(k.to(BF16), v.to(BF16), cap, code, 32)
+    q = torch.randn((n, 2, t, e), generator=gen).to(BF16).cuda()
+    check_attention(cache, ok, ov, [385, 400], q)
+
+
+@pytest.mark.parametrize("t", [1, 12, 66])
+@pytest.mark.parametrize("down,up", [(20, 18), (40, 30), (60, 60), (90, 85), (100, 90)])
+@pytest.mark.parametrize("where", ["other_tile", "same_tile"])
+@pytest.mark.parametrize("code,e", [(INT8, 64), (E4M3, 128)])
+def test_small_weights_of_large_values(t, down, up, where, code, e):
+    # one block has weights of about 2^-down and values 2^up larger: its part of the output is 2^(up - down) of the others'
+    gen = torch.Generator().manual_seed(down)
+    n, h, cap = 1, 1, 512
+    k, v = torch.randn((n, h, cap, e), generator=gen) * 0.25, torch.randn((n, h, cap, e), generator=gen)
+    b = 64 if where == "same_tile" else 256
+    k[..., 0] = 1.0
+    k[:, :, b:b + 32, 0] = -1.0
+    v[:, :, b:b + 32] *= 2.0 ** up
+    # a part of a tile that holds nothing but the small weights must not set the others' scale, nor the other way round
+    k[:, :, 480:, 0] = -1.0
+    cache, ok, ov = appended(k.to(BF16), v.to(BF16), cap, code, 32)
+    q = torch.randn((n, 2, t, e), generator=gen) * 0.2
+    q[..., 0] = down * math.log(2) / 2
+    check_attention(cache, ok, ov, [cap], q.to(BF16).cuda(), causal=False, scale=1.0)
+
+
 @pytest.mark.parametrize("t", [1, 9])
 @pytest.mark.parametrize("down,up", [(40, 38), (100, 98)])
 @pytest.mark.parametrize("code,e", [(INT8, 64), (E4M3, 128), (INT8, 256)])
@@ -119,3 +154,19 @@ def test_small_weights_of_large_values_behind_others_in_a_stretch(t, down, up, c
     q = torch.randn((n, 2, t, e), generator=gen) * 0.2
     q[..., 0] = down * math.log(2) / 2
     check_attention(cache, ok, ov, [cap] * n, q.to(BF16).cuda(), causal=False, scale=1.0)
+
+
+@pytest.mark.parametrize("t", [1, 12, 66])
+@pytest.mark.parametrize("code,e", [(INT8, 64), (E4M3, 128)])
+def test_the_largest_scores_on_values_of_zero(t, code, e):
+    # a first block that takes nearly all of the weight and holds zeros: the output is the others', 2^-60 of their size
+    gen = torch.Generator().manual_seed(5)
+    n, h, cap = 1, 1, 256
+    k, v = torch.randn((n, h, cap, e), generator=gen) * 0.25, torch.randn((n, h, cap, e), generator=gen) * 2.0 ** 60
+    k[..., 0] = -1.0
+    k[:, :, :32, 0] = 1.0
+    v[:, :, :32] = 0
+    cache, ok, ov = appended(k.to(BF16), v.to(BF16), cap, code, 32)
+    q = torch.randn((n, 2, t, e), generator=gen) * 0.2
+    q[..., 0] = 60 * math.log(2) / 2
+    check_attention(cache, ok, ov, [cap], q.to(BF16).cuda(), causal=False, scale=1.0)
