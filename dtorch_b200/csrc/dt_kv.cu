@@ -571,7 +571,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
                     const float g = f[j][i] * kscale;
-                    float top = -INFINITY;
+                    float top = kNothing;
 #pragma unroll
                     for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -589,10 +589,8 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
                     alpha[j][i] = over ? ratio : 1.0f;
                     gain[j][i] = over ? 1.0f : ratio;
                     base[j][i] = top - kShift;
-                    vs[j][i] = vscale * gain[j][i];
-                    if (top == -INFINITY) {  // nothing seen here: no weight, and no value whatever its scale (NaN of a marked block)
-                        gain[j][i] = vs[j][i] = base[j][i] = 0.0f;
-                    }
+                    // where nothing is seen there are no weights, and no values whatever their scale (NaN of a marked block)
+                    vs[j][i] = top == kNothing ? 0.0f : vscale * gain[j][i];
                     grown |= over;
                     m[j][i] = over ? top : m[j][i];
                 }
@@ -625,18 +623,17 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
             uint32_t p[2][NT][2];
 #pragma unroll
             for (int j = 0; j < NT; ++j) {
-                float sum[2] = {0.0f, 0.0f};
+                float u[4], v[4];
 #pragma unroll
                 for (int t = 0; t < 2; ++t)
 #pragma unroll
                     for (int k = 0; k < 2; ++k) {
-                        const float u = ex2(s[t][j][k * 2] - base[j][0]), v = ex2(s[t][j][k * 2 + 1] - base[j][1]);
-                        sum[0] += u;
-                        sum[1] += v;
-                        p[t][j][k] = transpose8(pack_half2(u, v));
+                        u[t * 2 + k] = ex2(s[t][j][k * 2] - base[j][0]);
+                        v[t * 2 + k] = ex2(s[t][j][k * 2 + 1] - base[j][1]);
+                        p[t][j][k] = transpose8(pack_half2(u[t * 2 + k], v[t * 2 + k]));
                     }
-                l[j][0] = fmaf(sum[0], gain[j][0], l[j][0]);
-                l[j][1] = fmaf(sum[1], gain[j][1], l[j][1]);
+                l[j][0] = fmaf((u[0] + u[1]) + (u[2] + u[3]), gain[j][0], l[j][0]);
+                l[j][1] = fmaf((v[0] + v[1]) + (v[2] + v[3]), gain[j][1], l[j][1]);
             }
             // values: 8 x 8 pairs of bytes transposed on the way in; even elements are rows 0-7 of the operand, odd 8-15
             const uint32_t vst = stages_s + st * S::kStageBytes + S::kSliceBytes;
@@ -702,6 +699,7 @@ __global__ void __launch_bounds__(kAttnThreads, AttnShape<EP, NT>::kCtas) k_kv_a
                 acc.z = fmaf(v.z, g, acc.z);
                 acc.w = fmaf(v.w, g, acc.w);
             }
+            if (whole && ll == 0.0f) ll = row_sum(ll, kv_limit(a, row, len, cnt) > 0);
             if (!whole) {
                 reinterpret_cast<float4*>(w.out)[(slot * S::kRows + r) * (EP / 4) + e / 4] = acc;
                 if (e == 0) w.stats[slot * S::kRows + r] = make_float2(mm, ll);
@@ -797,6 +795,8 @@ __global__ void __launch_bounds__(128) k_kv_merge(KvAttnArgs a, KvPartials w, in
             acc[v].y += u.y;
         }
     }
+    if (ll == 0.0f)
+        ll = row_sum(ll, kv_limit(a, row, kv_length(a.lengths, n, a.capacity), kv_count(a.counts, n, a.tokens)) > 0);
     const float g = ll == 0.0f ? 0.0f : 1.0f / ll;
     const int t = row / a.group, j = row - t * a.group;
     const size_t head = static_cast<size_t>(n) * a.kv_heads + h;
@@ -821,14 +821,14 @@ __global__ void __launch_bounds__(128) k_kv_merge(KvAttnArgs a, KvPartials w, in
     }
 }
 
-// 2^(score - lse2); 0 for a masked token, also of a row that saw nothing.
+// 2^(score - lse2); 0 for a masked token.
 __device__ __forceinline__ float weight_of(float score, float lse2) {
     return score == -INFINITY ? 0.0f : ex2(score - lse2);
 }
 
 // Weights from the stored scores: a thread sums four tokens' columns over the (at most 16) rows of a head. 8 rows of 8
 // heads and 131071 tokens (38 MB, most of it still in L2): 9 us.
-__global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w, int tile_rows) {
+__global__ void __launch_bounds__(256, 8) k_kv_weights(KvAttnArgs a, KvPartials w, int tile_rows) {
     enter_kernel();
     const size_t head = blockIdx.y + static_cast<size_t>(gridDim.y) * blockIdx.z;
     const int n = static_cast<int>(head / a.kv_heads);
@@ -838,9 +838,11 @@ __global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w, 
     if (t >= len) return;
     const float* sc = w.scores + head * tile_rows * static_cast<size_t>(a.capacity) + t;
     float v[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    bool undefined = false;
 #pragma unroll 4
     for (int r = 0; r < a.rows; ++r) {
         const float lse2 = w.lse2[head * a.rows + r];
+        undefined |= lse2 != lse2;
         const float4 x = *reinterpret_cast<const float4*>(sc + r * static_cast<size_t>(a.capacity));
         v[0] += weight_of(x.x, lse2);
         v[1] += weight_of(x.y, lse2);
@@ -851,6 +853,17 @@ __global__ void __launch_bounds__(256) k_kv_weights(KvAttnArgs a, KvPartials w, 
 #pragma unroll
     for (int i = 0; i < 4; ++i)
         if (t + i < len) o[i] = a.accumulate ? o[i] + v[i] : v[i];
+    if (!undefined) return;
+    // rows without a softmax: all that they see, scores of -infinity too
+#pragma unroll 1
+    for (int r = 0; r < a.rows; ++r) {
+        const float lse2 = w.lse2[head * a.rows + r];
+        if (lse2 == lse2) continue;
+        const int lim = kv_limit(a, r, len, kv_count(a.counts, n, a.tokens));
+#pragma unroll 1
+        for (int i = 0; i < 4; ++i)
+            if (t + i < lim) o[i] = lse2;
+    }
 }
 
 // Weights of heads larger than the tensor-core kernels take: the scores are computed again, 128 tokens of a head a CTA,

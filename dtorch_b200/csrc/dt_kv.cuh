@@ -16,6 +16,9 @@ namespace dtb {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
+// Maxima of scores begin here rather than at -infinity: differences of two of them are not NaN, and a score of -infinity
+// less one is -infinity.
+constexpr float kNothing = -3.0e38f;
 
 // What the attention kernels read. Query row r of key head h is query r / group of the sequence and query head
 // h * group + r % group: rows in the order of the tokens, so the rows of a tile see nearly the same tokens.
@@ -68,6 +71,10 @@ __device__ __forceinline__ int kv_limit(const KvAttnArgs& a, int row, int len, i
     const int lim = a.causal ? len - cnt + t + 1 : len;
     return lim < 0 ? 0 : lim;
 }
+
+// A row's sum of weights, by which its outputs are divided. 0 is that of a row that sees nothing, whose outputs are 0; a row
+// that sees nothing but scores of -infinity has it too, but no softmax: NaN.
+__device__ __forceinline__ float row_sum(float l, bool sees) { return l == 0.0f && sees ? __int_as_float(0x7fc00000) : l; }
 
 __device__ __forceinline__ uint32_t prmt(uint32_t a, uint32_t b, uint32_t sel) {
     uint32_t d;

@@ -312,6 +312,12 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     return d;
 }
 
+__device__ __forceinline__ float min_or_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
 // In the place that the program gives it: an exponential occupies its unit for 8 cycles, in which the warp can issue
 // the arithmetic of other columns.
 __device__ __forceinline__ void ex2_here(float& x) { asm volatile("ex2.approx.ftz.f32 %0, %0;" : "+f"(x)); }
@@ -727,7 +733,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 const float* const sc = scales + ((c + j) % kScaleRing) * 12 + half * 2;
                 const bool ragged = __any_sync(0xffffffffu, live < 64);
                 uint32_t s[32], s0[32];
-                float top = -INFINITY, out_top = -INFINITY;
+                float top = kNothing, out_top = kNothing;
                 // span 0 is loaded again for its weights: 32 scores fewer to hold meanwhile
                 tmem_load32(s_col, s0);
                 tmem_load32(s_col + 32, s);
@@ -749,26 +755,24 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                         mx[1] = max3(mx[1], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
                     }
                     const float m = fmaxf(mx[0], mx[1]);
-                    if (m != -INFINITY) {  // masked stays so where the scale is 0
-                        const float x = m * (factor * sc[k]);
-                        top = fmaxf(top, x);
-                        out_top = fmaxf(out_top, x + sc[8 + k]);
-                    }
+                    const float x = m * (factor * sc[k]);  // NaN (a masked span where the scale is 0) is passed over
+                    top = fmaxf(top, x);
+                    out_top = fmaxf(out_top, x + sc[8 + k]);
                 }
                 // the row's largest, of both halves, in fp32: large scores leave a 16-bit float's step no room above it
                 *mine = out_top;
                 pair_sync(pair);
                 out_top = fmaxf(out_top, *other);
-                if (top > ref + kGrowth) {  // also the first: ref is -infinity
-                    l *= ex2(ref - top);
-                    ref = top;
-                }
-                const bool grow = out_top > out_ref + kGrowth;
-                if (__any_sync(0xffffffffu, grow)) {  // the same for both warps of the pair
-                    const float now = grow ? out_top : out_ref;
-                    const float alpha = grow ? ex2(out_ref - now) : 1.0f;
+                const bool grow = top > ref + kGrowth, out_grow = out_top > out_ref + kGrowth;  // also the first: from -infinity
+                if (__any_sync(0xffffffffu, grow || out_grow)) {
+                    if (grow) {
+                        l *= ex2(ref - top);
+                        ref = top;
+                    }
+                    const float now = out_grow ? out_top : out_ref;
+                    const float alpha = out_grow ? ex2(out_ref - now) : 1.0f;
                     out_ref = now;
-                    if (j > 0) {
+                    if (j > 0 && __any_sync(0xffffffffu, out_grow)) {
 #pragma unroll 1
                         for (int k = 0; k < EP / 2; k += 32) {
                             uint32_t o[32];
@@ -780,23 +784,20 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                         }
                     }
                 }
-                const bool none = ref == -INFINITY;
-                const float down = none ? 0.0f : ref;
                 // ref - out_ref is below 2^7: out_ref counts ref's own token with an exponent of at least kLeastExponent
-                const float v_down = none ? 0.0f : ex2(ref - out_ref + kPromptShift);
+                const float v_down = ex2(ref - out_ref + kPromptShift);
                 Pair sum[2] = {0, 0};
 #pragma unroll
                 for (int k = 1; k >= 0; --k) {
                     uint32_t p[16];
-                    const float f = factor * sc[k];
-                    float vf = sc[4 + k] * v_down;
-                    if (vf > 0x1p126f) vf = 0x1p126f;  // only where all weights are below 2^-111; a NaN scale stays
+                    // above 2^126 only where all weights are below 2^-111; a NaN scale stays
+                    const float f = factor * sc[k], vf = min_or_nan(sc[4 + k] * v_down, 0x1p126f);
                     if (k == 0) {
                         tmem_load32(s_col, s);
                         tmem_wait_load32(s);
                     }
-                    if (ragged) weigh<true>(s, f, vf, down, live - k * 32, p, sum);
-                    else weigh<false>(s, f, vf, down, 32, p, sum);
+                    if (ragged) weigh<true>(s, f, vf, ref, live - k * 32, p, sum);
+                    else weigh<false>(s, f, vf, ref, 32, p, sum);
                     tmem_store16(s_col + k * 32, p);
                 }
                 tmem_wait_store();
@@ -831,8 +832,10 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 ref = most;
             }
             pair_sync(pair);  // both have read them: outputs, or the next queries, take their places
+            // only an item's end divides by its sum; `live` is the limit less the columns of these tiles and those before
+            if (item_steps == pos.tiles) l = row_sum(l, live + (pos.tile + item_steps) * kTokTile + half * 64 > 0);
             if (*dead) l = __int_as_float(0x7fc00000);
-            const float v_up = ref == -INFINITY ? 0.0f : exp2f(out_ref - ref - kPromptShift);
+            const float v_up = exp2f(out_ref - ref - kPromptShift);
             if (item_steps < pos.tiles) {
                 // an item that other CTAs work on too: one that began before this stretch, or goes on behind it
                 const size_t slot = static_cast<size_t>(blockIdx.x) * 2 + (pos.tile > 0 ? 0 : 1);
@@ -954,6 +957,7 @@ __global__ void __launch_bounds__(256) k_kv_prompt_merge(KvAttnArgs a, PromptPar
             acc[v].w = fmaf(o.w, f, acc[v].w);
         }
     }
+    l = row_sum(l, kv_limit(a, row, kv_length(a.lengths, pos.n, a.capacity), kv_count(a.counts, pos.n, a.tokens)) > 0);
     const float g = l == 0.0f ? 0.0f : 1.0f / l;
     const int t = row / a.group, jj = row - t * a.group;
     const size_t orow = (head * a.group + jj) * a.tokens + t;
@@ -1056,8 +1060,7 @@ __global__ void __launch_bounds__(128) k_kv_row_blocks(KvAttnArgs a, const float
         *reinterpret_cast<uint4*>(out + operand_offset(r, c)) = make_uint4(q[0], q[1], q[2], q[3]);
     }
     const float l = lim > 0 ? lse2[head * a.rows + row] : INFINITY;
-    reinterpret_cast<float2*>(out + ColumnShape<EP>::kOperand)[r] =
-        make_float2(inv * a.scale_log2, l == -INFINITY ? INFINITY : l);
+    reinterpret_cast<float2*>(out + ColumnShape<EP>::kOperand)[r] = make_float2(inv * a.scale_log2, l);
     reinterpret_cast<int*>(out + ColumnShape<EP>::kOperand + 128 * 8)[r] = lim;
 }
 

@@ -170,3 +170,25 @@ def test_the_largest_scores_on_values_of_zero(t, code, e):
     q = torch.randn((n, 2, t, e), generator=gen) * 0.2
     q[..., 0] = 60 * math.log(2) / 2
     check_attention(cache, ok, ov, [cap], q.to(BF16).cuda(), causal=False, scale=1.0)
+
+
+@pytest.mark.parametrize("e,t", [(64, 1), (128, 9), (64, 40), (256, 3)])
+@pytest.mark.parametrize("bad_value", [math.inf, -math.inf, math.nan])
+def test_queries_of_infinities(e, t, bad_value):
+    # all scores of a query are +infinity, or all -infinity: its softmax is not defined, and says so; others are not touched
+    gen = torch.Generator().manual_seed(e + t)
+    k, v = torch.rand((2, 1, 96, e), generator=gen) + 0.5, torch.randn((2, 1, 96, e), generator=gen)
+    cache, ok, ov = appended(k.to(BF16), v.to(BF16), 96, INT8, 32)
+    q = torch.randn((2, 2, t, e), generator=gen).to(BF16)
+    q[0, 1, t // 2] = 0
+    q[0, 1, t // 2, 3] = bad_value
+    w = torch.zeros((2, 1, 96), device="cuda")
+    # the second sequence holds nothing that its queries see
+    out, lse = dt.kv_cache_attention(q.cuda(), cache, ints([90, 0]), is_causal=False, weights=w, return_lse=True)
+    bad = torch.zeros((2, 2, t), dtype=torch.bool)
+    bad[0, 1, t // 2] = True
+    assert torch.equal(out.cpu().isnan().all(-1), bad) and torch.equal(out.cpu().isnan().any(-1), bad)
+    assert w[0, 0, :90].isnan().all() and not w[0, 0, 90:].any() and not w[1].any()
+    assert not out[1].any() and (lse[1] == -math.inf).all() and lse.cpu()[0][~bad[0]].isfinite().all()
+    q[0, 1, t // 2] = 0
+    check_attention(cache, ok, ov, [90, 0], q.cuda(), causal=False)
