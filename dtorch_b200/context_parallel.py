@@ -40,7 +40,7 @@ from typing import Dict, Optional, Union
 import torch
 import torch.nn.functional as F
 
-from .dtensor import DTensor, Replicate, Shard, _host, redistribute_many
+from .dtensor import DTensor, Placement, Replicate, Shard, _host, redistribute_many
 from .kv_cache import DistributedKVCache
 
 
@@ -197,16 +197,22 @@ def _attention_with_cache(query: DTensor, key: DTensor, value: DTensor, kv_cache
                           is_causal: bool, scale: Optional[float]) -> DTensor:
     placements = list(query.placements)
     swap = u is not None and placements[u] == Shard(2)
+    head = list(placements)
     if swap:
-        head = list(placements)
         head[u] = Shard(1)
-        if query.shape == key.shape == value.shape:
+        head = [Placement(p) for p in _host.normalize([repr(p) for p in head], list(query.device_mesh.shape),
+                                                      query.device_mesh.ids, 4)]  # as the swap will give them
+    # everything that can be refused is, before the swap and before a token is written: a refused call changes nothing
+    kv_cache._check_new(key, value, head)
+    kv_cache._check_query(query, scale, head)
+    if swap:
+        if query.shape == key.shape and query.dtype == key.dtype:
             query, key, value = redistribute_many([query, key, value], head)
         else:
             query = query.redistribute(placements=head)
             key, value = redistribute_many([key, value], head)
-    kv_cache.append(key, value)
-    out = kv_cache.attend(query, is_causal=is_causal, scale=scale)
+    kv_cache._append(key, value)
+    out = kv_cache._attend(query, is_causal, scale)
     return out.redistribute(placements=placements) if swap else out
 
 
@@ -220,7 +226,8 @@ def scaled_dot_product_attention_with_cp(query: DTensor, key: DTensor, value: DT
     one shape, heads divisible by groups * Ulysses size): swaps of one group overlap attention of another.
 
     With `kv_cache` the new keys and values are appended to it and the queries attend over what it then holds, with
-    `is_causal` each up to its own token; no dropout, ring dim or overlap."""
+    `is_causal` each up to its own token; no dropout, ring dim or overlap. A call that is refused leaves the cache as it
+    was."""
     u = _dim_index(query, ulysses_cp_dim)
     r = _dim_index(query, ring_cp_dim)
     if ring_overlap and (r is None or is_causal or dropout_p > 0.0):

@@ -161,6 +161,7 @@ PYBIND11_MODULE(_host, m) {
         .def_property_readonly("capacity", [](const QuantizedKVCache& c) { return c.abi.capacity; })
         .def_property_readonly("head_dim", [](const QuantizedKVCache& c) { return c.abi.head_dim; })
         .def_property_readonly("block", [](const QuantizedKVCache& c) { return c.abi.block; });
+    m.def("kv_cache_check_rows", &KVCacheCheckRows);
     m.def("kv_cache_append", &KVCacheAppend, py::call_guard<py::gil_scoped_release>());
     m.def("kv_cache_read",
           [](const QuantizedKVCache& c, const torch::Tensor& lengths, const std::optional<torch::Tensor>& first,

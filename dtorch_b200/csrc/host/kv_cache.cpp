@@ -49,6 +49,14 @@ void CheckRows(const QuantizedKVCache& c, const torch::Tensor& t, const char* wh
     CheckNoGrad(t, where);
 }
 
+}  // namespace
+
+void KVCacheCheckRows(const QuantizedKVCache& c, const torch::Tensor& t, const std::string& where, const std::string& name) {
+    CheckRows(c, t, where.c_str(), name.c_str());
+}
+
+namespace {
+
 torch::Tensor InnerContiguous(const torch::Tensor& t) { return t.stride(3) == 1 ? t : t.contiguous(); }
 
 void CheckWeights(const QuantizedKVCache& c, const torch::Tensor& t, const char* where) {

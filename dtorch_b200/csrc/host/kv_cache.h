@@ -3,6 +3,7 @@
 #pragma once
 
 #include <optional>
+#include <string>
 #include <tuple>
 
 #include <torch/torch.h>
@@ -20,6 +21,10 @@ class QuantizedKVCache {
     torch::Tensor key, value, keyScale, valueScale;
     dt_kv_cache abi;
 };
+
+// What append and attention ask of rows of tokens by themselves: type, batch and head size, place, no gradient.
+void KVCacheCheckRows(const QuantizedKVCache& cache, const torch::Tensor& rows, const std::string& where,
+                      const std::string& name);
 
 void KVCacheAppend(const QuantizedKVCache& cache, const torch::Tensor& key, const torch::Tensor& value,
                    const torch::Tensor& lengths, const std::optional<torch::Tensor>& counts);

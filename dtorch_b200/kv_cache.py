@@ -155,38 +155,62 @@ class DistributedKVCache:
             if track_weights:
                 self.weights[gid] = torch.zeros(s[:3], device=dev)
 
-    def _check(self, t: DTensor, name: str) -> None:
-        if t.device_mesh != self.device_mesh or t.placements != self.placements:
-            raise ValueError(f"DistributedKVCache: {name} is {t.placements} on {t.device_mesh}, the cache "
+    def _check(self, t: DTensor, name: str, placements: Sequence[Placement]) -> None:
+        """That `t`, which will come with `placements`, fits the cache on every device."""
+        if t.device_mesh != self.device_mesh or list(placements) != self.placements:
+            raise ValueError(f"DistributedKVCache: {name} is {list(placements)} on {t.device_mesh}, the cache "
                              f"{self.placements} on {self.device_mesh}")
+        if len(t.shape) != 4 or t.shape[0] != self.shape[0] or t.shape[3] != self.shape[3]:
+            raise ValueError(f"DistributedKVCache: {name} {t.shape} does not fit {self.shape}")
+        shapes = _host.compute_local_shapes(list(t.shape), list(self.device_mesh.shape), self.device_mesh.ids,
+                                            [repr(p) for p in t.placements])
+        for gid, cache in self.locals.items():
+            if list(t.local(gid).shape) != list(shapes[gid]):
+                raise ValueError(f"DistributedKVCache: device {gid} holds {tuple(t.local(gid).shape)} of {name}, not "
+                                 f"{tuple(shapes[gid])}")
+            _host.kv_cache_check_rows(cache._c, t.local(gid), "DistributedKVCache", name)
 
-    def append(self, key: DTensor, value: DTensor) -> None:
-        """Append T tokens (batch, kv_heads, T, head_dim) to every sequence."""
-        self._check(key, "key")
-        self._check(value, "value")
-        if key.shape != value.shape or len(key.shape) != 4 or key.shape[:2] + key.shape[3:] != \
-                self.shape[:2] + self.shape[3:]:
+    def _check_new(self, key: DTensor, value: DTensor, placements: Sequence[Placement]) -> None:
+        self._check(key, "key", placements)
+        self._check(value, "value", placements)
+        if key.shape != value.shape or key.shape[1] != self.shape[1]:
             raise ValueError(f"DistributedKVCache: key {key.shape} and value {value.shape} do not fit {self.shape}")
-        tokens = key.shape[2]
-        if self.max_length + tokens > self.shape[2]:
-            raise ValueError(f"DistributedKVCache: {tokens} more tokens than {self.max_length} do not fit the capacity "
-                             f"of {self.shape[2]}; evict first")
+        if any(key.local(gid).dtype != value.local(gid).dtype for gid in self.locals):
+            raise TypeError("DistributedKVCache: key and value differ in type")
+        if self.max_length + key.shape[2] > self.shape[2]:
+            raise ValueError(f"DistributedKVCache: {key.shape[2]} more tokens than {self.max_length} do not fit the "
+                             f"capacity of {self.shape[2]}; evict first")
+
+    def _check_query(self, query: DTensor, scale: Optional[float], placements: Sequence[Placement]) -> None:
+        self._check(query, "query", placements)
+        if query.shape[1] == 0 or query.shape[1] % self.shape[1]:
+            raise ValueError(f"DistributedKVCache: query {query.shape} does not fit {self.shape}")
+        if scale is not None and not math.fabs(scale) <= torch.finfo(torch.float32).max:
+            raise ValueError("DistributedKVCache: scale must be finite")
+
+    def _append(self, key: DTensor, value: DTensor) -> None:
         for gid, cache in self.locals.items():
             kv_cache_append(cache, key.local(gid), value.local(gid), self.lengths[gid])
             with torch.cuda.device(cache.device):
-                self.lengths[gid] += tokens
-        self.max_length += tokens
+                self.lengths[gid] += key.shape[2]
+        self.max_length += key.shape[2]
+
+    def _attend(self, query: DTensor, is_causal: bool, scale: Optional[float]) -> DTensor:
+        out = {gid: kv_cache_attention(query.local(gid), cache, self.lengths[gid], is_causal=bool(is_causal), scale=scale,
+                                       weights=self.weights.get(gid)) for gid, cache in self.locals.items()}
+        return DTensor(out, self.device_mesh, query.placements, query.shape)
+
+    def append(self, key: DTensor, value: DTensor) -> None:
+        """Append T tokens (batch, kv_heads, T, head_dim) to every sequence. What is refused is refused before anything
+        is written on any device."""
+        self._check_new(key, value, key.placements)
+        self._append(key, value)
 
     def attend(self, query: DTensor, is_causal: bool = True, scale: Optional[float] = None) -> DTensor:
         """Attention of the last T tokens' queries (batch, query_heads, T, head_dim), as kv_cache_attention; adds to the
         weights where they are tracked."""
-        self._check(query, "query")
-        if len(query.shape) != 4 or query.shape[0] != self.shape[0] or query.shape[3] != self.shape[3] or \
-                query.shape[1] % self.shape[1]:
-            raise ValueError(f"DistributedKVCache: query {query.shape} does not fit {self.shape}")
-        out = {gid: kv_cache_attention(query.local(gid), cache, self.lengths[gid], is_causal=is_causal, scale=scale,
-                                       weights=self.weights.get(gid)) for gid, cache in self.locals.items()}
-        return DTensor(out, self.device_mesh, query.placements, query.shape)
+        self._check_query(query, scale, query.placements)
+        return self._attend(query, is_causal, scale)
 
     def evict(self, budget: int, recent: int = 0) -> None:
         """kv_cache_evict on every device, by the tracked weights; the capacity stays."""
@@ -194,9 +218,11 @@ class DistributedKVCache:
             raise ValueError("DistributedKVCache: evict needs track_weights=True")
         if not 0 <= recent <= budget <= self.shape[2]:
             raise ValueError("DistributedKVCache: 0 <= recent <= budget <= capacity")
+        done = {}
         for gid, cache in self.locals.items():
             into = QuantizedKVCache(cache.batch, cache.kv_heads, cache.capacity, cache.head_dim, cache.dtype, cache.block,
                                     cache.device)
-            self.locals[gid], self.lengths[gid], self.weights[gid], _ = kv_cache_evict(
-                cache, self.lengths[gid], self.weights[gid], budget, recent, out=into)
+            done[gid] = kv_cache_evict(cache, self.lengths[gid], self.weights[gid], budget, recent, out=into)
+        for gid, (cache, lengths, weights, _) in done.items():  # of all devices or, where one fails, of none
+            self.locals[gid], self.lengths[gid], self.weights[gid] = cache, lengths, weights
         self.max_length = min(self.max_length, budget)

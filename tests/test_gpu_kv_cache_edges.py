@@ -192,3 +192,68 @@ def test_queries_of_infinities(e, t, bad_value):
     assert not out[1].any() and (lse[1] == -math.inf).all() and lse.cpu()[0][~bad[0]].isfinite().all()
     q[0, 1, t // 2] = 0
     check_attention(cache, ok, ov, [90, 0], q.cuda(), causal=False)
+
+
+@pytest.fixture
+def mesh(monkeypatch):
+    monkeypatch.setenv("DTORCH_DTENSOR_IN_SAME_DEVICE", "1")
+    monkeypatch.setenv("DTORCH_COMM_TIMEOUT_SECOND", "30")
+    dt.clear()
+    yield dt.init_device_mesh("cuda", (2,), mesh_dim_names=["cp"])
+    dt.clear()
+
+
+def untouched(cache, length):
+    torch.cuda.synchronize()
+    return cache.max_length == length and all(l.tolist() == [length] * 2 for l in cache.lengths.values())
+
+
+@pytest.mark.parametrize("place", [1, 2])
+def test_a_refused_step_leaves_the_distributed_cache_as_it_was(mesh, place):
+    n, h, e, cap = 2, 4, 64, 128
+    place = dt.Shard(place)
+    gen = torch.Generator().manual_seed(3)
+    cache = dt.DistributedKVCache(mesh, [dt.Shard(1)], n, h, cap, e, block=32, track_weights=True)
+
+    def made(heads=h, dtype=BF16, e=e, n=n):
+        return dt.DTensor.from_torch(torch.randn((n, heads, 6, e), generator=gen).to(dtype), mesh, [place])
+
+    def step(q, k, v, **kw):
+        return dt.scaled_dot_product_attention_with_cp(q, k, v, is_causal=True, ulysses_cp_dim="cp", kv_cache=cache, **kw)
+
+    k, v = made(), made()
+    step(made(), k, v)
+    assert untouched(cache, 6)
+    grad = made()
+    for t in grad.locals.values():
+        t.requires_grad_()
+    refused = [(ValueError, made(heads=6), {}), (ValueError, made(e=32), {}), (ValueError, made(n=4), {}),
+               (TypeError, made(dtype=torch.float32), {}), (ValueError, made(), dict(scale=math.inf)),
+               (ValueError, made(), dict(scale=math.nan)), (TypeError, made(), dict(scale="a quarter")),
+               (RuntimeError, grad, {})]
+    before = {g: c.key.clone() for g, c in cache.locals.items()}
+    for error, q, kw in refused:
+        with pytest.raises(error):
+            step(q, k, v, **kw)
+        assert untouched(cache, 6)
+    for bad in (made(dtype=torch.float32), made(dtype=FP16)):
+        with pytest.raises(TypeError):
+            step(made(), k, bad)
+        assert untouched(cache, 6)
+    assert all(torch.equal(c.key.view(torch.int8), before[g].view(torch.int8)) for g, c in cache.locals.items())
+    step(made(heads=8), k, v)  # the retry, with two query heads a key head
+    assert untouched(cache, 12)
+
+
+def test_append_checks_every_device_before_the_first_write(mesh):
+    n, h, e = 2, 4, 64
+    cache = dt.DistributedKVCache(mesh, [dt.Shard(1)], n, h, 128, e, block=32)
+    k = dt.DTensor.from_torch(torch.ones((n, h, 6, e), dtype=BF16), mesh, [dt.Shard(1)])
+    last = max(mesh.ids)
+    odd = {g: k.local(g).float() if g == last else k.local(g) for g in mesh.ids}
+    odd = dt.DTensor(odd, mesh, [dt.Shard(1)], (n, h, 6, e))
+    with pytest.raises(TypeError):
+        cache.append(k, odd)
+    assert untouched(cache, 0) and not any(c.key.any() or c.value.any() for c in cache.locals.values())
+    cache.append(k, k)
+    assert untouched(cache, 6)

@@ -194,3 +194,42 @@ def test_attention_with_cp_refuses_what_the_cache_does_not_serve():
         dt.scaled_dot_product_attention_with_cp(s0, s0, s0, kv_cache=fake, ulysses_cp_dim=0)
     with pytest.raises(ValueError, match="divided"):
         dt.scaled_dot_product_attention_with_cp(odd, odd, odd, kv_cache=fake, ulysses_cp_dim=0)
+
+
+def test_a_step_on_a_mesh_is_refused_before_it_begins():
+    mesh = dt.init_device_mesh("cuda", (2,))
+    c = object.__new__(dt.DistributedKVCache)  # on CPU tensors: nothing behind the checks can run
+    c.device_mesh, c.placements, c.shape, c.max_length = mesh, [dt.Shard(1)], (2, 4, 64, 64), 60
+    c.locals = {g: cache(cap=64) for g in mesh.ids}
+    c.lengths, c.weights = {g: ints(60, 60) for g in mesh.ids}, {}
+
+    def made(n=2, h=4, t=3, e=64, dtype=BF16, last=None, place=1):
+        local = {g: rows(n, h // 2, t, e, dtype) if place == 1 else rows(n, h, t // 2, e, dtype) for g in mesh.ids}
+        local[mesh.ids[-1]] = local[mesh.ids[-1]].to(last or dtype)
+        return dt.DTensor(local, mesh, [dt.Shard(place)], (n, h, t, e))
+
+    def step(q, k, v, **kw):
+        return dt.scaled_dot_product_attention_with_cp(q, k, v, is_causal=True, ulysses_cp_dim=0, kv_cache=c, **kw)
+
+    grad = made()
+    grad.local(mesh.ids[-1]).requires_grad_()
+    wrong = made()
+    wrong._locals[mesh.ids[0]] = rows(2, 2, 2, 64)
+    for error, q, k, v, kw in (
+            (ValueError, made(h=6), made(), made(), {}), (ValueError, made(e=32), made(), made(), {}),
+            (ValueError, made(n=4), made(), made(), {}), (TypeError, made(dtype=torch.float32), made(), made(), {}),
+            (TypeError, made(last=torch.float32), made(), made(), {}), (RuntimeError, grad, made(), made(), {}),
+            (ValueError, wrong, made(), made(), {}), (ValueError, made(), wrong, made(), {}),
+            (TypeError, made(), made(), made(last=torch.float16), {}), (RuntimeError, made(), made(), grad, {}),
+            (ValueError, made(), made(t=5), made(t=5), {}), (ValueError, made(), made(h=8), made(h=8), {}),
+            (ValueError, made(), made(), made(t=2), {}), (ValueError, made(), made(), made(), dict(scale=math.inf)),
+            (ValueError, made(), made(), made(), dict(scale=1e39)), (TypeError, made(), made(), made(), dict(scale="1")),
+            (ValueError, made(h=6, t=4, place=2), made(t=4, place=2), made(t=4, place=2), {}),
+            (TypeError, made(t=4, place=2), made(t=4, place=2), made(t=4, place=2, last=torch.float32), {})):
+        with pytest.raises(error) as e:
+            step(q, k, v, **kw)
+        assert "served on cuda" not in str(e.value)
+        assert c.max_length == 60 and all(l.tolist() == [60, 60] for l in c.lengths.values())
+    with pytest.raises(ValueError, match="cuda"):  # everything is right
+        step(made(h=8), made(), made())
+    assert c.max_length == 60
