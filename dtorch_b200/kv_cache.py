@@ -153,7 +153,7 @@ class DistributedKVCache:
             self.locals[gid] = QuantizedKVCache(s[0], s[1], capacity, head_dim, dtype, block, dev)
             self.lengths[gid] = torch.zeros(s[0], dtype=torch.int32, device=dev)
             if track_weights:
-                self.weights[gid] = torch.zeros(s[:3], device=dev)
+                self.weights[gid] = torch.zeros(s[:3], dtype=torch.float32, device=dev)
 
     def _check(self, t: DTensor, name: str, placements: Sequence[Placement]) -> None:
         """That `t`, which will come with `placements`, fits the cache on every device."""

@@ -257,3 +257,15 @@ def test_append_checks_every_device_before_the_first_write(mesh):
     assert untouched(cache, 0) and not any(c.key.any() or c.value.any() for c in cache.locals.values())
     cache.append(k, k)
     assert untouched(cache, 6)
+
+
+def test_the_tracked_weights_are_float32_under_another_default_type(mesh):
+    torch.set_default_dtype(BF16)
+    try:
+        cache = dt.DistributedKVCache(mesh, [dt.Shard(1)], 2, 4, 128, 64, block=32, track_weights=True)
+        x = dt.DTensor.from_torch(torch.ones((2, 4, 40, 64), dtype=BF16), mesh, [dt.Shard(1)])
+        dt.scaled_dot_product_attention_with_cp(x, x, x, is_causal=True, ulysses_cp_dim="cp", kv_cache=cache)
+        cache.evict(16, 4)
+        assert all(w.dtype == torch.float32 for w in cache.weights.values()) and untouched(cache, 16)
+    finally:
+        torch.set_default_dtype(torch.float32)
