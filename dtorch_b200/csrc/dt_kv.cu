@@ -1376,6 +1376,13 @@ int launch_few_rows(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p,
     return launch_kernel("dt_kv_attention", k_kv_merge<EP>, dim3(grid), 128, 0, stream, 1, a, w, row_tiles, S::kRows, p.grid);
 }
 
+int launch_weights(const KvAttnArgs& a, const KvPartials& w, int tile_rows, cudaStream_t stream) {
+    const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
+    const unsigned y = static_cast<unsigned>(std::min<int64_t>(heads, 32768));
+    const dim3 g(static_cast<unsigned>((a.capacity + 1023) / 1024), y, static_cast<unsigned>((heads + y - 1) / y));
+    return launch_kernel("dt_kv_attention", k_kv_weights, g, 256, 0, stream, 1, a, w, tile_rows);
+}
+
 template <bool E4M3, int EP>
 int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, void* workspace, bool weights,
                   cudaStream_t stream) {
@@ -1385,11 +1392,7 @@ int launch_attend(const KvAttnArgs& a, const KvPartials& w, const AttnPlan& p, v
     else st = launch_few_rows<E4M3, EP, 2>(a, w, p, stream);
     if (st != DT_OK || !weights) return st;
     const int64_t heads = static_cast<int64_t>(a.batch) * a.kv_heads;
-    if (w.scores != nullptr) {
-        const unsigned y = static_cast<unsigned>(std::min<int64_t>(heads, 32768));
-        const dim3 g(static_cast<unsigned>((a.capacity + 1023) / 1024), y, static_cast<unsigned>((heads + y - 1) / y));
-        return launch_kernel("dt_kv_attention", k_kv_weights, g, 256, 0, stream, 1, a, w, static_cast<int>(tile_rows(p.rows)));
-    }
+    if (w.scores != nullptr) return launch_weights(a, w, static_cast<int>(tile_rows(p.rows)), stream);
     if (p.column_tiles)
         return kv_column_sums(a, E4M3 ? DT_KV_E4M3 : DT_KV_INT8, p.columns, static_cast<char*>(workspace) + p.scores, w.lse2,
                               stream);
@@ -1517,7 +1520,18 @@ int dt_kv_attention(const dt_kv_cache* cache, const void* query, int64_t query_h
         return set_error(DT_ERR_INVALID, "dt_kv_attention: queries must be bf16 or fp16");
     if ((flags & ~(DT_KV_CAUSAL | DT_KV_ACCUMULATE)) != 0) return set_error(DT_ERR_INVALID, "dt_kv_attention: unknown flag");
     if (!std::isfinite(scale)) return set_error(DT_ERR_INVALID, "dt_kv_attention: scale must be finite");
-    if (cache->batch == 0 || tokens == 0) return DT_OK;
+    if (cache->batch == 0) return DT_OK;
+    if (tokens == 0) {  // no queries: nothing to add to weights, but sums of nothing to write
+        if (weights == nullptr || (flags & DT_KV_ACCUMULATE) != 0) return DT_OK;
+        if (lengths == nullptr) return set_error(DT_ERR_INVALID, "dt_kv_attention: null argument");
+        KvAttnArgs a{};
+        a.lengths = lengths;
+        a.weights = weights;
+        a.batch = static_cast<int>(cache->batch);
+        a.kv_heads = static_cast<int>(cache->kv_heads);
+        a.capacity = cache->capacity;
+        return launch_weights(a, KvPartials{}, 0, static_cast<cudaStream_t>(stream));
+    }
     if (query == nullptr || query_strides == nullptr || lengths == nullptr || out == nullptr)
         return set_error(DT_ERR_INVALID, "dt_kv_attention: null argument");
     if ((reinterpret_cast<uintptr_t>(out) & 15) != 0 || !aligned16(workspace))

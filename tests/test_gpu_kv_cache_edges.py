@@ -194,6 +194,17 @@ def test_queries_of_infinities(e, t, bad_value):
     check_attention(cache, ok, ov, [90, 0], q.cuda(), causal=False)
 
 
+@pytest.mark.parametrize("e", [64, 256])
+def test_weights_of_no_queries(e):
+    cache = dt.QuantizedKVCache(3, 2, 96, e, block=32)
+    none = torch.empty((3, 4, 0, e), dtype=BF16, device="cuda")
+    w = torch.full((3, 2, 96), 7.0, device="cuda")
+    dt.kv_cache_attention(none, cache, ints([0, 5, 200]), weights=w)
+    assert (w == 7).all()
+    dt.kv_cache_attention(none, cache, ints([0, 5, 200]), weights=w, accumulate=False)
+    assert (w[0] == 7).all() and not w[1, :, :5].any() and (w[1, :, 5:] == 7).all() and not w[2].any()
+
+
 @pytest.fixture
 def mesh(monkeypatch):
     monkeypatch.setenv("DTORCH_DTENSOR_IN_SAME_DEVICE", "1")
