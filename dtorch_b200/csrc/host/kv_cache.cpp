@@ -37,6 +37,7 @@ void CheckInts(const QuantizedKVCache& c, const torch::Tensor& t, const char* wh
 void CheckNoGrad(const torch::Tensor& t, const char* where) {
     TORCH_CHECK(!(t.requires_grad() && torch::GradMode::is_enabled()), where,
                 ": no backward pass through an 8-bit cache; call it under torch.no_grad()");
+    TORCH_CHECK(!t._fw_grad(0).defined(), where, ": no forward-mode derivative through an 8-bit cache; pass the primal");
 }
 
 // (N, H, T, E) rows of the model's type, E contiguous.

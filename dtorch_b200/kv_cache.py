@@ -16,7 +16,9 @@ graph and replayed while the lengths grow::
     cache, lengths, seen, _ = kv_cache_evict(cache, lengths, seen, budget=4096, recent=512)
 
 Lengths below 0 count as 0 and those above the capacity as the capacity; slots behind a length are never read. The
-operators run on the current stream of the cache's device, whichever device is current. There is no backward pass.
+operators run on the current stream of the cache's device, whichever device is current. They have no derivative:
+tensors that require a gradient (outside torch.no_grad()) and forward-mode duals are refused. torch.compile breaks its
+graph at them.
 """
 
 from __future__ import annotations

@@ -233,3 +233,18 @@ def test_a_step_on_a_mesh_is_refused_before_it_begins():
     with pytest.raises(ValueError, match="cuda"):  # everything is right
         step(made(h=8), made(), made())
     assert c.max_length == 60
+
+
+def test_no_forward_mode_derivatives():
+    import torch.autograd.forward_ad as fwd
+
+    c, l = cache(), ints(0, 0)
+    with fwd.dual_level():
+        x = fwd.make_dual(rows(), torch.ones_like(rows()))
+        q = fwd.make_dual(rows(h=4), torch.ones_like(rows(h=4)))
+        for call in (lambda: dt.kv_cache_append(c, x, rows(), l), lambda: dt.kv_cache_append(c, rows(), x, l),
+                     lambda: dt.kv_cache_attention(q, c, l)):
+            with pytest.raises(RuntimeError, match="derivative"):
+                call()
+        with torch.no_grad(), pytest.raises(ValueError, match="cuda"):  # values alone are asked for
+            dt.kv_cache_append(c, fwd.unpack_dual(x).primal, rows(), l)
