@@ -51,6 +51,7 @@ constexpr int kScaleRing = 4;
 // Exponents of value scales that count; scales of 0 and NaN have the least: their tokens do not set the reference.
 constexpr int kLeastExponent = -100;
 constexpr uint64_t kWaitLimitNs = 10000000000ull;  // waits of one CTA for its own work last microseconds
+constexpr uint64_t kDrainLimitNs = 1000000000ull;
 
 template <int EP>
 struct PromptShape {
@@ -100,6 +101,23 @@ __device__ __forceinline__ void mbar_wait(uint32_t bar, uint32_t parity, volatil
         if (now - start > kWaitLimitNs) break;
     }
     *dead = 1;
+}
+
+// Wait, also with a limit, for copies or products in flight before the CTA ends, whether a wait has run out or not: they
+// must not land in memory that has been given up.
+__device__ __forceinline__ void mbar_drain(uint32_t bar, uint32_t parity) {
+    uint64_t start, now;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(start));
+    do {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return;
+        asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(now));
+    } while (now - start < kDrainLimitNs);
 }
 
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -630,6 +648,8 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 if (left <= 0) break;
                 pos.next(w, row_tiles, a.kv_heads);
             }
+            // the last tile's values are free when every product is done: none is in flight when the tensor memory is given up
+            mbar_drain(bars + (kVEmpty + ((c - 1) & 1)) * 8, ((c - 1) >> 1) & 1);
         }
     } else if (warp >= kConvertWarp) {
         // ---- keys and values to fp16 operands ----
@@ -1125,6 +1145,10 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
                 const uint32_t st = c % S::kStages, full = bars + (kBFull + st) * 8;
                 mbar_wait(bars + (kBEmpty + st) * 8, (c / S::kStages & 1) ^ 1, dead);
                 __syncwarp();
+                if (__any_sync(0xffffffffu, *dead != 0)) {  // the stage may not be free
+                    left = 0;
+                    break;
+                }
                 if (elect_one()) {
                     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(full), "n"(S::kBlock) : "memory");
                     asm volatile(
@@ -1139,6 +1163,9 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
             if (left <= 0) break;
             pos.next(w.list, key_tiles, a.kv_heads);
         }
+        // the last copies have landed before the CTA ends
+        for (uint32_t k = c > S::kStages ? c - S::kStages : 0; k < c; ++k)
+            mbar_drain(bars + (kBFull + k % S::kStages) * 8, k / S::kStages & 1);
     } else if (warp == 8) {
         // ---- products ----
         const uint64_t k_desc = operand_desc(base + S::kKeys, 16, 1024);
@@ -1168,6 +1195,8 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
             if (left <= 0) break;
             pos.next(w.list, key_tiles, a.kv_heads);
         }
+        // the last products are done before the tensor memory is given up
+        mbar_drain(bars + (kTFull + ((c - 1) & 3)) * 8, ((c - 1) >> 2) & 1);
     } else {
         // ---- sums ----
         const int turn = warp >> 2;
