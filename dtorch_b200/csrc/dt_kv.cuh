@@ -16,9 +16,9 @@ namespace dtb {
 
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kLn2 = 0.6931471805599453f;
-// Maxima of scores begin here rather than at -infinity: differences of two of them are not NaN, and a score of -infinity
-// less one is -infinity.
-constexpr float kNothing = -3.0e38f;
+// Maxima of scores begin at the least finite number rather than -infinity: differences of two of them are not NaN, and a
+// score of -infinity less one is -infinity.
+constexpr float kNothing = -3.402823466e38f;
 
 // What the attention kernels read. Query row r of key head h is query r / group of the sequence and query head
 // h * group + r % group: rows in the order of the tokens, so the rows of a tile see nearly the same tokens.
