@@ -172,7 +172,9 @@ __device__ __forceinline__ float row_max(const KvAttnArgs& a, const uint32_t* x)
 template <typename... P, typename... A>
 int launch_kernel(const char* what, void (*kernel)(P...), dim3 grid, int threads, size_t smem, cudaStream_t stream,
                   unsigned cluster, A... args) {
-    if (smem > 48 * 1024) {  // per device and cheap: the limit belongs to the kernel in the current context
+    // Above 48 KB with the kernel's static shared memory, of which those that take both have less than 16 KB. Per device and
+    // cheap: the limit belongs to the kernel in the current context.
+    if (smem > 32 * 1024) {
         const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
         if (e != cudaSuccess) return set_error(DT_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
     }

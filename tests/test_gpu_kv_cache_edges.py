@@ -8,7 +8,7 @@ import torch
 
 import dtorch_b200 as dt
 from tests import kv_oracle as ko
-from tests.test_gpu_kv_cache import BF16, E4M3, FP16, INT8, check_attention, filled, ints, tokens
+from tests.test_gpu_kv_cache import BF16, E4M3, FP16, INT8, check_attention, evict_case, filled, ints, tokens
 
 pytestmark = pytest.mark.gpu
 
@@ -280,3 +280,12 @@ def test_the_tracked_weights_are_float32_under_another_default_type(mesh):
         assert all(w.dtype == torch.float32 for w in cache.weights.values()) and untouched(cache, 16)
     finally:
         torch.set_default_dtype(torch.float32)
+
+
+@pytest.mark.parametrize("code", [INT8, E4M3])
+@pytest.mark.parametrize("block", [32, 64, 128])
+@pytest.mark.parametrize("e", range(16, 257, 16))
+def test_evict_of_every_head_size_and_block(code, block, e):
+    # 128 tokens of 192 elements: keys and values together are 48 KB, to which the kernel's own shared memory comes
+    gen = torch.Generator().manual_seed(e)
+    evict_case(gen, [300, 70], 1, 384, e, code, block, 150, 20, torch.randn((2, 1, 384), generator=gen))
