@@ -289,3 +289,89 @@ def test_evict_of_every_head_size_and_block(code, block, e):
     # 128 tokens of 192 elements: keys and values together are 48 KB, to which the kernel's own shared memory comes
     gen = torch.Generator().manual_seed(e)
     evict_case(gen, [300, 70], 1, 384, e, code, block, 150, 20, torch.randn((2, 1, 384), generator=gen))
+
+
+@pytest.mark.parametrize("t", [1, 66])
+def test_captured_behind_copies_fills_and_joined_streams(t):
+    """A graph whose calls follow a memory fill, a copy and the join of two streams with calls of their own, replayed with
+    other lengths, queries and caches."""
+    gen = torch.Generator().manual_seed(41)
+    cap, h, g, e = 512, 2, 2, 128
+    caches = [filled(gen, [300, 511], h, cap, e, code, 64)[0] for code in (INT8, E4M3)]
+    for c in caches:
+        for s in (c.key_scale, c.value_scale):
+            s.nan_to_num_(0.01)
+        c.key.view(torch.int8)[:, :, 300:] = 3
+        c.value.view(torch.int8)[:, :, 300:] = 5
+    new_q = torch.randn((2, h * g, t, e), generator=gen).to(BF16).cuda()
+    q, lengths = torch.empty_like(new_q), ints([300, 511])
+    w = [torch.ones((2, h, cap), device="cuda") for _ in caches]
+    side = torch.cuda.Stream()
+
+    def calls():
+        main = torch.cuda.current_stream()
+        q.copy_(new_q)
+        for x in w:
+            x.zero_()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            a = dt.kv_cache_attention(q, caches[0], lengths, weights=w[0])
+        b = dt.kv_cache_attention(q, caches[1], lengths, weights=w[1])
+        main.wait_stream(side)
+        both = w[0] + w[1]
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            first = dt.kv_cache_evict(caches[0], lengths, both, 128, 16)
+        second = dt.kv_cache_evict(caches[1], lengths, both, 100, 0)
+        main.wait_stream(side)
+        k = dt.kv_cache_read(second[0], second[1], count=100, dtype=torch.float32)[0]
+        dt.kv_cache_append(first[0], k[:, :, :20].to(BF16), k[:, :, 20:40].to(BF16), first[1] - 20)
+        return a, b, both, first[3], second[3], k, *dt.kv_cache_read(first[0], first[1], dtype=torch.float32)
+
+    calls()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = calls()
+    for lens in ([300, 511], [0, 130], [512, 64], [150, 151]):
+        lengths.copy_(ints(lens))
+        new_q.copy_(torch.randn(new_q.shape, generator=gen).to(BF16))
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        kept = [x.clone() for x in got]
+        for x, y in zip(kept, calls()):
+            torch.cuda.synchronize()
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("shape,places", [((2,), [dt.Shard(0)]), ((2,), [dt.Replicate()]),
+                                          ((2, 2), [dt.Shard(0), dt.Shard(1)]), ((2, 2), [dt.Shard(1), dt.Replicate()])])
+def test_other_placements_of_a_distributed_cache(monkeypatch, shape, places):
+    monkeypatch.setenv("DTORCH_DTENSOR_IN_SAME_DEVICE", "1")
+    dt.clear()
+    mesh = dt.init_device_mesh("cuda", shape)
+    gen = torch.Generator().manual_seed(7)
+    n, h, e, cap = 4, 4, 64, 128
+    cache = dt.DistributedKVCache(mesh, places, n, h, cap, e, block=32, track_weights=True)
+    one = dt.QuantizedKVCache(n, h, cap, e, block=32)
+    lengths, seen = ints([0] * n), torch.zeros((n, h, cap), device="cuda")
+    for t in (70, 1, 9):
+        q, k, v = (tokens(gen, n, heads, t, e, BF16) for heads in (2 * h, h, h))
+        out = dt.scaled_dot_product_attention_with_cp(*(dt.DTensor.from_torch(x, mesh, places) for x in (q, k, v)),
+                                                      is_causal=True, kv_cache=cache)
+        dt.kv_cache_append(one, k.cuda(), v.cuda(), lengths)
+        lengths += t
+        want = dt.kv_cache_attention(q.cuda(), one, lengths, weights=seen)
+        torch.cuda.synchronize()
+        # the tiles are shared out by the numbers of sequences and heads: sums differ in their order
+        assert torch.allclose(out.to_torch().float(), want.float().cpu(), rtol=2.0 ** -7, atol=2.0 ** -9)
+    full = dt.DTensor(cache.weights, mesh, places, (n, h, cap)).to_torch()
+    assert torch.allclose(full.cpu(), seen.cpu(), rtol=1e-5, atol=1e-8)
+    for g in mesh.ids:
+        assert cache.lengths[g].tolist() == [80] * cache.locals[g].batch
+    codes = dt.DTensor({g: c.key for g, c in cache.locals.items()}, mesh, places, (n, h, cap, e)).to_torch()
+    assert torch.equal(codes.cpu(), one.key.cpu())
+    cache.evict(32, 8)
+    assert cache.max_length == 32 and all((l == 32).all() for l in cache.lengths.values())
+    dt.clear()
