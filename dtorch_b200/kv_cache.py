@@ -128,7 +128,11 @@ class DistributedKVCache:
     `track_weights`, what evict goes by. scaled_dot_product_attention_with_cp(..., kv_cache=cache) appends and attends.
 
     Attributes: locals (QuantizedKVCache of each device id), lengths and weights (tensors of each device id),
-    max_length (no sequence holds more tokens; known without asking the devices)."""
+    max_length (no sequence holds more tokens; known without asking the devices).
+
+    A step of single tokens can be captured in a CUDA graph. max_length counts calls: add a step's tokens to it for each
+    replay, and replay no step for which the capacity has no room (its tokens would not be written). Eviction moves the
+    cache to new tensors, so it is not captured, and graphs captured before it are of the old ones."""
 
     def __init__(self, device_mesh: DeviceMesh, placements: Sequence[Placement], batch: int, kv_heads: int, capacity: int,
                  head_dim: int, dtype: torch.dtype = torch.int8, block: int = 64, track_weights: bool = False):
@@ -220,6 +224,11 @@ class DistributedKVCache:
             raise ValueError("DistributedKVCache: evict needs track_weights=True")
         if not 0 <= recent <= budget <= self.shape[2]:
             raise ValueError("DistributedKVCache: 0 <= recent <= budget <= capacity")
+        for cache in self.locals.values():
+            with torch.cuda.device(cache.device):
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("DistributedKVCache: evict moves the cache to new tensors and cannot be captured; "
+                                       "capture kv_cache_evict")
         done = {}
         for gid, cache in self.locals.items():
             into = QuantizedKVCache(cache.batch, cache.kv_heads, cache.capacity, cache.head_dim, cache.dtype, cache.block,

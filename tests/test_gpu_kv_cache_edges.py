@@ -375,3 +375,44 @@ def test_other_placements_of_a_distributed_cache(monkeypatch, shape, places):
     cache.evict(32, 8)
     assert cache.max_length == 32 and all((l == 32).all() for l in cache.lengths.values())
     dt.clear()
+
+
+def test_a_captured_step_of_a_distributed_cache(mesh):
+    gen = torch.Generator().manual_seed(9)
+    n, h, e, cap = 2, 4, 64, 128
+    place = [dt.Shard(1)]
+    cache = dt.DistributedKVCache(mesh, place, n, h, cap, e, block=32, track_weights=True)
+    one = dt.QuantizedKVCache(n, h, cap, e, block=32)
+    lengths, seen = ints([0] * n), torch.zeros((n, h, cap), device="cuda")
+    new = [dt.DTensor.from_torch(torch.zeros((n, heads, 1, e), dtype=BF16), mesh, place) for heads in (2 * h, h, h)]
+
+    def step():
+        return dt.scaled_dot_product_attention_with_cp(*new, is_causal=True, ulysses_cp_dim="cp", kv_cache=cache)
+
+    step()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with pytest.raises(RuntimeError, match="captured"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            cache.evict(16)
+    with torch.cuda.graph(graph):
+        out = step()
+    assert cache.max_length == 2  # the second of them by the first replay
+    for l in cache.lengths.values():
+        l.zero_()
+    for w in cache.weights.values():
+        w.zero_()
+    for i in range(40):
+        x = [tokens(gen, n, heads, 1, e, BF16) for heads in (2 * h, h, h)]
+        for t, y in zip(new, x):
+            for g in mesh.ids:
+                t.local(g).copy_(y[:, g * y.shape[1] // 2:(g + 1) * y.shape[1] // 2])
+        graph.replay()
+        dt.kv_cache_append(one, x[1].cuda(), x[2].cuda(), lengths)
+        lengths += 1
+        want = dt.kv_cache_attention(x[0].cuda(), one, lengths, weights=seen)
+        torch.cuda.synchronize()
+        assert torch.allclose(out.to_torch().float(), want.float().cpu(), rtol=2.0 ** -7, atol=2.0 ** -9), i
+    cache.max_length = 40
+    cache.evict(16, 4)
+    assert untouched(cache, 16)
