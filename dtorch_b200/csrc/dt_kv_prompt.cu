@@ -27,9 +27,10 @@ namespace {
 // TMEM, 512 columns: S of both row tiles (128 each, P in the first half of each), O of both (EP each). Products run in
 // the order of their issue, so a completed S also says that the O += P V before it is done.
 //
-// 4096 tokens over 16384, 32 query and 8 key heads of 128, int8: 865 us, 1112 TFLOP/s back to back, 69 % of a library
-// product's burst rate. Bound by the chain of each row tile (scores, softmax, weights, products: 4000 cycles, of which
-// the tensor core works 1024, twice a step) and by issue slots; exponentials and products alone would take 2048.
+// 4096 tokens over 16384, 32 query and 8 key heads of 128, int8: 853 us, 1128 TFLOP/s, in a run of 20 calls, 70 % of a
+// library product's burst rate; 985 to 1005 us, 60 %, in calls that go on for seconds, when the clock falls to what the
+// power allows. Bound by the chain of each row tile (scores, softmax, weights, products: 4000 cycles, of which the tensor
+// core works 1024, twice a step) and by issue slots; exponentials and products alone would take 2048.
 //
 // Block scales are constant over 32 columns: a key scale goes into the row's factor, a value scale into the weight before
 // it is rounded to fp16. What is rounded is therefore 2^x * (value scale), and its reference is the row's largest of
@@ -783,7 +784,7 @@ __global__ void __launch_bounds__(kPromptThreads, 1) k_kv_prompt(KvAttnArgs a, P
                 *mine = out_top;
                 pair_sync(pair);
                 out_top = fmaxf(out_top, *other);
-                const bool grow = top > ref + kGrowth, out_grow = out_top > out_ref + kGrowth;  // also the first: from -infinity
+                const bool grow = top > ref + kGrowth, out_grow = out_top > out_ref + kGrowth;  // the first too
                 if (__any_sync(0xffffffffu, grow || out_grow)) {
                     if (grow) {
                         l *= ex2(ref - top);

@@ -101,7 +101,16 @@ def kv_cache_attention(query: torch.Tensor, cache: QuantizedKVCache, lengths: to
     queries and the query heads of its key head, for the tokens below lengths[n] (what kv_cache_evict goes by): added,
     or written where `accumulate` is False. A slot that a new token takes keeps what it had: set it to 0 first, or
     start from zeros. With `return_lse` also the log-sum-exp of the scaled scores, float32 (N, Hq, T), -inf for a
-    query that sees nothing. The same inputs give the same bits."""
+    query that sees nothing. The same inputs give the same bits.
+
+    Scores, sums and outputs are fp32. A softmax weight is rounded to fp16 for the product with the values: 11 significant
+    bits down to 2^-24 of the largest among the 32 tokens that share its step (up to 32 queries a key head, or heads above
+    128 elements) or, times its value scale, among all that the query sees (more queries). Weights below 2^-110 of the
+    largest may count as 0. NaN in a block (a non-finite value was appended) reaches the queries that see the block and no
+    others; a query with an infinity or NaN gives NaN, and so do the weights of what it sees.
+
+    Workspace: up to 1 GiB for weights of up to 16 queries a key head, by the cache's capacity; for those of more a copy of
+    the queries in fp16."""
     s = 1.0 / math.sqrt(cache.head_dim) if scale is None else scale
     out, lse = _host.kv_cache_attention(query, cache._c, lengths, counts, is_causal, s, weights, accumulate, return_lse)
     return (out, lse) if return_lse else out
@@ -110,8 +119,8 @@ def kv_cache_attention(query: torch.Tensor, cache: QuantizedKVCache, lengths: to
 def kv_cache_evict(cache: QuantizedKVCache, lengths: torch.Tensor, weights: torch.Tensor, budget: int, recent: int = 0,
                    out: Optional[QuantizedKVCache] = None):
     """Cut every sequence back to at most `budget` tokens: in each head the last `recent` stay, and of the others those
-    with the largest `weights` (N, H, capacity), ties to the lowest position; they keep their order. The kept tokens go
-    to the front of `out`, a cache that shares no memory with `cache` (default: a new one of the budget rounded up to
+    with the largest `weights` (N, H, capacity), ties to the lowest position and NaN above all; they keep their order. The
+    kept tokens go to the front of `out`, a cache that shares no memory with `cache` (default: a new one of the budget rounded up to
     blocks), in blocks that are scaled anew. Returns (out, lengths, weights, kept): the new cache's lengths (N,) and
     weights (N, H, out.capacity), 0 behind the kept tokens, and the kept positions (N, H, budget), -1 behind the last."""
     if out is None:
@@ -124,7 +133,8 @@ def kv_cache_evict(cache: QuantizedKVCache, lengths: torch.Tensor, weights: torc
 class DistributedKVCache:
     """The 8-bit cache of a decoder on a device mesh: every device holds a QuantizedKVCache of its part of (batch,
     kv_heads, capacity, head_dim) under `placements`, where a mesh dim may shard the batch (Shard(0)) or the heads
-    (Shard(1): the placement after the Ulysses swap), evenly, or replicate. It keeps the lengths and, with
+    (Shard(1): the placement after the Ulysses swap), evenly, or replicate. Every append adds as many tokens to all
+    sequences: a ragged batch uses a QuantizedKVCache and counts. It keeps the lengths and, with
     `track_weights`, what evict goes by. scaled_dot_product_attention_with_cp(..., kv_cache=cache) appends and attends.
 
     Attributes: locals (QuantizedKVCache of each device id), lengths and weights (tensors of each device id),

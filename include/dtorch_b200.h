@@ -371,8 +371,12 @@ int dt_kv_attention_workspace(const dt_kv_cache* cache, int64_t query_heads, int
  * log-sum-exp of -infinity. lse (NULL: not wanted) is (batch, query_heads, tokens) fp32, natural logarithm, of the
  * scaled scores. weights (NULL: not wanted) is (batch, kv_heads, capacity) fp32: the sum of each cached token's
  * softmax weights over the queries and the query heads of its key head, written (DT_KV_ACCUMULATE: added) for the
- * tokens below lengths[n]; slots behind are left as they were. Sums are fp32 in a fixed order: the same inputs give
- * the same bits. */
+ * tokens below lengths[n], also where there are no queries (tokens 0); slots behind are left as they were. Sums are fp32
+ * in a fixed order: the same inputs give the same bits. A softmax weight is rounded to fp16 for the product with the
+ * values: 11 bits down to 2^-24 of the largest among the 32 tokens that share a step (query_heads / kv_heads * tokens up to
+ * 32, or head_dim above 128) or, times its value scale, among all that the query sees (more). A block with the scale
+ * NaN reaches the queries that see it and no others. A query with an infinity or NaN gives NaN, also as the weights
+ * of what it sees. */
 int dt_kv_attention(const dt_kv_cache* cache, const void* query, int64_t query_heads, int64_t tokens,
                     const int64_t* query_strides, int dtype, const int32_t* lengths, const int32_t* counts,
                     float scale, int flags, void* out, float* lse, float* weights, void* workspace,
