@@ -880,7 +880,8 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv_column_sums(KvAttnArgs a, c
     if (tok >= len) return;
     const uint8_t* const kbase = a.key + (head * a.capacity + tok) * a.head_dim;
     const float kscale = a.key_scale[head * a.nblocks + (tok >> a.block_shift)];
-    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};  // tokens r4 + 8 k
+    // Of tokens r4 + 8 k, of 256 rows at a time and in all: thousands of small weights added to one number would lose bits.
+    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f}, total[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     uint4 keys[4][EP / 64];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
@@ -893,6 +894,13 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv_column_sums(KvAttnArgs a, c
         }
     const int row_tiles = (a.rows + 7) / 8;
     for (int rt = 0; rt < row_tiles; ++rt) {
+        if (rt % 32 == 0) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                total[k] += sum[k];
+                sum[k] = 0.0f;
+            }
+        }
         // the last row of a tile sees the most
         const int last = min(rt * 8 + 7, min(a.rows, cnt * a.group) - 1);
         if (last < rt * 8 || kv_limit(a, last, len, cnt) <= tok) continue;
@@ -931,6 +939,7 @@ __global__ void __launch_bounds__(kAttnThreads) k_kv_column_sums(KvAttnArgs a, c
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
+        sum[k] += total[k];
         sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 1);
         sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], 2);
         const int t = tok + k * 8 + r4;

@@ -1229,9 +1229,10 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
             const int span = tok + (warp & 3) * 32;
             const float ks = span < len ? a.key_scale[head * a.nblocks + (span >> a.block_shift)] : 0.0f;
             const Pair ks2 = pair_of(ks, ks);
-            Pair sum[2] = {0, 0};
+            Pair total = 0;
             for (int j = 0; j < steps; ++j, ++c) {
                 if ((c & 1) != static_cast<uint32_t>(turn)) continue;
+                Pair sum[2] = {0, 0};  // of this tile: thousands of small weights added to one number would lose bits
                 const uint32_t st = c % S::kStages, b = c & 3;
                 mbar_wait(bars + (kTFull + b) * 8, c >> 2 & 1, dead);
                 mbar_wait(bars + (kBFull + st) * 8, c / S::kStages & 1, dead);  // the block's numbers, for this thread too
@@ -1265,6 +1266,7 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
                         sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pair_of(u, v));
                     }
                 }
+                total = add2(total, add2(sum[0], sum[1]));
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) {
@@ -1273,7 +1275,7 @@ __global__ void __launch_bounds__(kColumnThreads, 1) k_kv_columns(KvAttnArgs a, 
                 }
             }
             float u, v;
-            unpair(add2(sum[0], sum[1]), u, v);
+            unpair(total, u, v);
             u += v;
             // both groups' tiles are done, and with them every product of these keys
             if (turn == 1) sums[tid & 127] = u;

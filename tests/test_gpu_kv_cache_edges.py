@@ -416,3 +416,29 @@ def test_a_captured_step_of_a_distributed_cache(mesh):
     cache.max_length = 40
     cache.evict(16, 4)
     assert untouched(cache, 16)
+
+
+@pytest.mark.parametrize("code,e,g,t", [(INT8, 64, 8, 4096), (E4M3, 128, 1, 20001), (INT8, 256, 8, 4096), (E4M3, 192, 3, 5003)])
+def test_weights_of_many_equal_rows(code, e, g, t):
+    # Scores of 0: every row gives every token the same weight, whose sum over up to 32768 rows is known. Adding n equal
+    # numbers one after another in fp32 is off by up to n 2^-26 of the sum (each addition by half a step of what there is).
+    # 64 rows, or 32 pairs of rows, at a time and then 128 of those: 2^-18 of the sum, as for few rows.
+    lengths = [43, 1, 96]
+    cache, _, _ = filled(torch.Generator().manual_seed(1), lengths, 1, 96, e, code, 32)
+    q = torch.zeros((3, g, t, e), dtype=BF16, device="cuda")
+    w = torch.zeros((3, 1, 96), device="cuda")
+    dt.kv_cache_attention(q, cache, ints(lengths), is_causal=False, weights=w)
+    for i, l in enumerate(lengths):
+        want = g * t / l
+        assert ((w[i, 0, :l].double() - want).abs() <= 2.0 ** -18 * want).all() and not w[i, 0, l:].any()
+
+
+def test_weights_of_many_equal_rows_over_many_tokens():
+    # As above where a CTA has all rows of its tokens. To the rows' sum comes that of the tokens' weights, 157 tiles one
+    # after another, and the log-sum-exp, rounded to 2^-21 at log2(20000): 2^-18 + 2^-18 + 2^-20 of a weight.
+    l, rows = 20000, 8 * 4096
+    cache, _, _ = filled(torch.Generator().manual_seed(1), [l], 1, 20032, 64, INT8, 64)
+    w = torch.zeros((1, 1, 20032), device="cuda")
+    dt.kv_cache_attention(torch.zeros((1, 8, 4096, 64), dtype=BF16, device="cuda"), cache, ints([l]), is_causal=False,
+                          weights=w)
+    assert ((w[0, 0, :l].double() - rows / l).abs() <= (2.0 ** -17 + 2.0 ** -20) * rows / l).all() and not w[0, 0, l:].any()
