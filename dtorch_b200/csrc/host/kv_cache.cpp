@@ -52,8 +52,15 @@ void CheckRows(const QuantizedKVCache& c, const torch::Tensor& t, const char* wh
 
 }  // namespace
 
-void KVCacheCheckRows(const QuantizedKVCache& c, const torch::Tensor& t, const std::string& where, const std::string& name) {
-    CheckRows(c, t, where.c_str(), name.c_str());
+void KVCacheCheckRows(const std::vector<const QuantizedKVCache*>& caches, const std::vector<torch::Tensor>& rows,
+                      const std::vector<std::vector<int64_t>>& shapes, const std::string& where, const std::string& name) {
+    TORCH_CHECK_VALUE(caches.size() == rows.size() && caches.size() == shapes.size(), where, ": ", name, " is of ", rows.size(),
+                      " devices, the cache of ", caches.size());
+    for (size_t i = 0; i < rows.size(); ++i) {
+        CheckRows(*caches[i], rows[i], where.c_str(), name.c_str());
+        TORCH_CHECK_VALUE(rows[i].sizes() == at::IntArrayRef(shapes[i]), where, ": ", name, " is ", rows[i].sizes(),
+                          " on one device, not ", at::IntArrayRef(shapes[i]));
+    }
 }
 
 namespace {

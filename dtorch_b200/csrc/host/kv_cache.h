@@ -5,6 +5,7 @@
 #include <optional>
 #include <string>
 #include <tuple>
+#include <vector>
 
 #include <torch/torch.h>
 
@@ -22,9 +23,10 @@ class QuantizedKVCache {
     dt_kv_cache abi;
 };
 
-// What append and attention ask of rows of tokens by themselves: type, batch and head size, place, no gradient.
-void KVCacheCheckRows(const QuantizedKVCache& cache, const torch::Tensor& rows, const std::string& where,
-                      const std::string& name);
+// What append and attention ask of rows of tokens by themselves, of several caches at once: type, shape, place, no
+// gradient.
+void KVCacheCheckRows(const std::vector<const QuantizedKVCache*>& caches, const std::vector<torch::Tensor>& rows,
+                      const std::vector<std::vector<int64_t>>& shapes, const std::string& where, const std::string& name);
 
 void KVCacheAppend(const QuantizedKVCache& cache, const torch::Tensor& key, const torch::Tensor& value,
                    const torch::Tensor& lengths, const std::optional<torch::Tensor>& counts);

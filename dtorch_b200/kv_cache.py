@@ -173,25 +173,30 @@ class DistributedKVCache:
 
     def _check(self, t: DTensor, name: str, placements: Sequence[Placement]) -> None:
         """That `t`, which will come with `placements`, fits the cache on every device."""
-        if t.device_mesh != self.device_mesh or list(placements) != self.placements:
+        if (t.device_mesh is not self.device_mesh and t.device_mesh != self.device_mesh) or \
+                list(placements) != self.placements:
             raise ValueError(f"DistributedKVCache: {name} is {list(placements)} on {t.device_mesh}, the cache "
                              f"{self.placements} on {self.device_mesh}")
         if len(t.shape) != 4 or t.shape[0] != self.shape[0] or t.shape[3] != self.shape[3]:
             raise ValueError(f"DistributedKVCache: {name} {t.shape} does not fit {self.shape}")
-        shapes = _host.compute_local_shapes(list(t.shape), list(self.device_mesh.shape), self.device_mesh.ids,
+        if t.placements == self.placements:  # as it comes: every part in its cache's proportion
+            shapes = [(c.batch, t.shape[1] * c.kv_heads // self.shape[1], t.shape[2], t.shape[3])
+                      for c in self.locals.values()]
+        else:
+            of = _host.compute_local_shapes(list(t.shape), list(self.device_mesh.shape), self.device_mesh.ids,
                                             [repr(p) for p in t.placements])
-        for gid, cache in self.locals.items():
-            if list(t.local(gid).shape) != list(shapes[gid]):
-                raise ValueError(f"DistributedKVCache: device {gid} holds {tuple(t.local(gid).shape)} of {name}, not "
-                                 f"{tuple(shapes[gid])}")
-            _host.kv_cache_check_rows(cache._c, t.local(gid), "DistributedKVCache", name)
+            shapes = [of[gid] for gid in self.locals]
+        parts = t.locals
+        _host.kv_cache_check_rows([c._c for c in self.locals.values()], [parts[gid] for gid in self.locals], shapes,
+                                  "DistributedKVCache", name)
 
     def _check_new(self, key: DTensor, value: DTensor, placements: Sequence[Placement]) -> None:
         self._check(key, "key", placements)
         self._check(value, "value", placements)
         if key.shape != value.shape or key.shape[1] != self.shape[1]:
             raise ValueError(f"DistributedKVCache: key {key.shape} and value {value.shape} do not fit {self.shape}")
-        if any(key.local(gid).dtype != value.local(gid).dtype for gid in self.locals):
+        keys, values = key.locals, value.locals
+        if any(keys[gid].dtype != values[gid].dtype for gid in self.locals):
             raise TypeError("DistributedKVCache: key and value differ in type")
         if self.max_length + key.shape[2] > self.shape[2]:
             raise ValueError(f"DistributedKVCache: {key.shape[2]} more tokens than {self.max_length} do not fit the "
